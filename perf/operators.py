@@ -174,7 +174,7 @@ def _plan_plain(s):
     need = torch.where(fits, last - have, 0)
     upto = need.cumsum(0)
     served = fits & ((need == 0) | (upto <= free.numel()))
-    taken = torch.where(served, upto, 0).max()
+    taken = torch.where(served & (need > 0), upto, 0).max()
     cols = torch.arange(width, device=table.device)
     fresh = (cols >= have[:, None]) & (cols < last[:, None]) & served[:, None]
     pick = ((upto - need)[:, None] + cols - have[:, None]).clamp(0, free.numel() - 1)

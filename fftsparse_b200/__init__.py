@@ -12,6 +12,10 @@ Public surface (mirrors attn_src/fft_attn/my_attn_v7.py):
   derive_mask_params(L, ...)                host-side parameter derivation
   calibrate.calibrate_from_qk(layers, t)    target-sparsity calibration on the device
   decode_attention(q, k_cache, v_cache)     one-token decode over the un-expanded KV cache
+  plan_pages(cached_lens, new_lens, ...)    page bookkeeping of a serving step: block tables and slot maps
+  rope_append(q, k, v, ...)                 rotary positions + append of k, v to a paged cache, one pass
+  paged_attention(q, k_pages, v_pages, ...) chunks and single tokens over a paged cache, window and sinks
+  rotary_inv_freq(rotary_dim, base, ...)    rotary frequencies, scaled for long contexts
   dist.sharded_prefill(...)                 KV-group sharded prefill (peer-memory all-gather)
   check_status(device=None)                 raise WaitTimeout if a kernel's bounded wait ran out
 """
@@ -29,6 +33,7 @@ from .prefill import (  # noqa: F401
     sparse_attention,
 )
 from .decode import decode_attention  # noqa: F401
+from .paged import PagePlan, paged_attention, plan_pages, rope_append, rotary_inv_freq  # noqa: F401
 from .status import WaitTimeout, check_status  # noqa: F401
 from ._lib import load as load_library, LIB_PATH  # noqa: F401
 

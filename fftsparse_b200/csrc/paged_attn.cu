@@ -1,0 +1,926 @@
+// paged_attn.cu -- causal attention of new tokens over a paged KV cache on sm_100a (tcgen05 + TMEM + TMA).
+//
+// Request r has q_len = cu_q[r+1] - cu_q[r] new tokens (rows of q) at the end of its kv_len cached ones;
+// token i sits at pos = kv_len - q_len + i and sees key c iff c <= pos and (no window, or c > pos - W, or
+// c < S): o = softmax(scale q k^T) v over the keys it sees, zeros if there are none.  q_len 1 is decoding,
+// longer ones are the chunks of a prompt; a batch may mix them.
+//
+// Work.  The G = H / Hkv query heads of a KV head share one 128-row tile with as many tokens as fit
+// (128 / G, row = token * G + head), so a key tile is loaded once for all of them.  A q tile visits the
+// 64-key tiles that any of its rows can see (the sinks' tiles, then the window's), in order.  All (q tile, KV
+// head, key tile) triples form one line of W units, cut into equal shares: CTA c of the persistent grid
+// takes units [c * per, (c + 1) * per).  A share that begins or ends inside a (q tile, head) leaves fp32
+// partial sums that merge_kernel joins.  So one decode request and a batch of ragged chunks alike load
+// every SM equally, and nothing about the lengths is needed on the host.
+//   schedule_kernel  one CTA: q tiles of every request and the running sum of their key tiles
+//   attn_kernel      two CTAs per SM, each walking its share
+//   merge_kernel     joins the (q tile, head)s that several shares cut
+//
+// attn_kernel's roles (192 threads):
+//   warp 4      producer: page numbers one tile ahead, Q per segment, K tiles into a three-stage ring, V
+//               into a two-stage ring; every lane issues its own TMA boxes (a page is one box per 64
+//               channels).  A page no row sees gets page number -1: TMA fills zeros, nothing is read.
+//   warp 5      MMA issuer (one thread): S = Q K^T into a double-buffered TMEM accumulator, O += P V with
+//               P from TMEM.
+//   warps 0-3   softmax: thread r owns row r; S(n) is read, masked and exponentiated against a running
+//               reference maximum (O and l rescaled only when a score outgrows it by 2^kRescale) while
+//               the tensor core computes S(n+1).  V rows behind a request's last key, or of no key a
+//               row sees, are zeroed in shared memory first: pages hold anything there, and 0 * NaN
+//               would reach the sum.
+// Every mbarrier wait is bounded (a status code instead of a hang).
+
+#include <cuda.h>
+#include <cuda_fp16.h>
+#include <cudaTypedefs.h>
+
+#include <algorithm>
+
+#include "ffts_common.cuh"
+#include "tc_sm100.cuh"
+
+namespace ffts {
+namespace paged {
+
+using namespace ::ffts::tc;
+
+constexpr int kBM = 128;      // rows of a q tile
+constexpr int kBN = 64;       // keys of a key tile
+constexpr int kThreads = 192;
+constexpr int kKStages = 3, kVStages = 2;
+constexpr int kTmemCols = 256;  // S0, S1 (64 columns each), O (D): two CTAs fill an SM's 512
+constexpr uint32_t kTmemO = 128;
+constexpr int kMaxCtas = 512;   // partial slots in the workspace (two per CTA)
+constexpr int kMinUnits = 4;    // key tiles per share, at least
+constexpr double kWaitSeconds = 2.0, kDrainSeconds = 4.0;
+
+constexpr int kErrProducer = 10, kErrMma = 11, kErrSoftmax = 12, kErrSmemAlign = 13;
+
+template <int D>
+struct Layout {
+  static constexpr int halves = D / 64;             // 64-channel swizzle boxes per row
+  static constexpr int q_half = kBM * 128;          // bytes of one half of a tile
+  static constexpr int kv_half = kBN * 128;
+  static constexpr int q_bytes = halves * q_half, kv_bytes = halves * kv_half;
+  static constexpr int q = 0;
+  static constexpr int k = q + q_bytes;
+  static constexpr int v = k + kKStages * kv_bytes;
+  static constexpr int bars = v + kVStages * kv_bytes;
+  static constexpr int nbars = 2 + 2 * kKStages + kVStages + 2 + 2 + 2 + 1;
+  static constexpr int tmem_slot = bars + nbars * 8;
+  static constexpr int abort = tmem_slot + 8;
+  static constexpr int bytes = abort + 8;
+  static_assert(2 * (bytes + 1024) <= 228 * 1024, "two CTAs must fit in an SM's shared memory");
+};
+
+// barriers; one per buffer, since the softmax can run a tile ahead of the MMA issuer
+constexpr int BQF = 0;                  // Q loaded
+constexpr int BQE = 1;                  // the segment's S products have read Q
+constexpr int BKF = 2;                  // K stage loaded    [kKStages]
+constexpr int BKE = BKF + kKStages;     // K stage free      [kKStages]
+constexpr int BVF = BKE + kKStages;     // V stage loaded    [kVStages]
+constexpr int BSF = BVF + kVStages;     // S(n) in buffer n % 2 [2]
+constexpr int BPV = BSF + 2;            // PV(n) complete, frees V stage n % 2 [2]
+constexpr int BPF = BPV + 2;            // P(n) written (128 arrivals) [2]
+constexpr int BDRAIN = BPF + 2;
+
+// One q tile: tokens [tok0, tok0 + ntok) of request r, the first at position pos0.
+struct Tile {
+  int tok0, pos0, ntok, r;
+};
+
+struct Params {
+  int T, R, H, Hkv, G, tpt;   // tpt: tokens per q tile
+  const int32_t *table;       // [R, width]
+  int64_t table_ld;
+  int width, n_pages, ps_shift;
+  const int32_t *cu_q, *kv_lens;
+  int window, sinks;          // window 0: none
+  uint16_t *out;
+  int64_t os_t, os_h;
+  float scale_log2;
+  Tile *tiles;                // [max_tiles]
+  long long *cum;             // [max_tiles + 1]: key tiles (of one head) before q tile x
+  int *header;                // [0]: q tiles
+  float *part;                // [2 * ctas][128][D], then m, l: [2 * ctas][128] float2
+  float2 *part_ml;
+  int max_tiles, ctas;
+  int *status;
+  long long wait_cycles, drain_cycles;
+};
+
+// The key tiles of a q tile: [0, st), then [wt0, ...); n of them in all (at least one, which may be all
+// masked).  Keys >= hi, and keys < lo that are not sinks, are seen by no row.
+struct Keys {
+  int hi, lo, st, wt0, n;
+};
+
+__device__ __forceinline__ Keys keys_of(int pos0, int ntok, int window, int sinks) {
+  Keys g;
+  g.hi = max(0, pos0 + ntok);
+  g.lo = window > 0 ? max(0, pos0 - window + 1) : 0;
+  const int nt = (g.hi + kBN - 1) / kBN;
+  g.wt0 = g.lo / kBN;
+  g.st = min((min(sinks, g.hi) + kBN - 1) / kBN, g.wt0);
+  g.n = max(1, g.st + nt - g.wt0);
+  return g;
+}
+
+__device__ __forceinline__ int key_tile(const Keys &g, int j) { return j < g.st ? j : j - g.st + g.wt0; }
+
+__device__ __forceinline__ long long share_of(const Params &p, long long units) {
+  const long long per = (units + p.ctas - 1) / p.ctas;
+  return per < kMinUnits ? kMinUnits : per;
+}
+
+// ---------------------------------------------------------------- schedule
+constexpr int kSchedThreads = 1024;
+
+__device__ __forceinline__ long long sched_scan(long long v, long long *warp_sums, long long *total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long u = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += u;
+  }
+  __syncthreads();
+  if (lane == 31) warp_sums[warp] = v;
+  __syncthreads();
+  long long s = warp_sums[lane];
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long u = __shfl_up_sync(0xffffffffu, s, o);
+    if (lane >= o) s += u;
+  }
+  const long long before = warp > 0 ? __shfl_sync(0xffffffffu, s, warp - 1) : 0;
+  *total = __shfl_sync(0xffffffffu, s, 31);
+  return v + before;
+}
+
+__global__ void __launch_bounds__(kSchedThreads) schedule_kernel(const __grid_constant__ Params p) {
+  __shared__ long long warp_sums[32];
+  __shared__ long long s_tiles[kSchedThreads];  // q tiles up to and with the request
+  __shared__ int s_q0[kSchedThreads], s_len[kSchedThreads], s_kv[kSchedThreads];
+  const int tid = threadIdx.x;
+  const long long cap = (long long)p.width << p.ps_shift;  // keys a table row can hold
+  long long tile_base = 0, unit_base = 0;
+  if (tid == 0) p.cum[0] = 0;
+  for (int r0 = 0; r0 < p.R; r0 += kSchedThreads) {
+    const int nr = min(kSchedThreads, p.R - r0);
+    int q0 = 0, len = 0, kv = 0;
+    if (tid < nr) {
+      // lengths are device data: kept inside q and the table whatever they hold
+      q0 = min(max(p.cu_q[r0 + tid], 0), p.T);
+      len = min(max(p.cu_q[r0 + tid + 1], q0), p.T) - q0;
+      kv = int(min((long long)max(p.kv_lens[r0 + tid], 0), cap));
+    }
+    long long total;
+    const long long upto = sched_scan((len + p.tpt - 1) / p.tpt, warp_sums, &total);
+    s_tiles[tid] = upto;
+    s_q0[tid] = q0;
+    s_len[tid] = len;
+    s_kv[tid] = kv;
+    __syncthreads();
+    const long long fit = min(total, (long long)p.max_tiles - tile_base);
+    for (long long x0 = 0; x0 < fit; x0 += kSchedThreads) {
+      const long long x = x0 + tid;
+      int n = 0;
+      if (x < fit) {
+        int lo = 0, hi = nr;  // the first request whose tiles reach past x
+        while (lo < hi) {
+          const int mid = (lo + hi) >> 1;
+          if (s_tiles[mid] > x) hi = mid; else lo = mid + 1;
+        }
+        const int i = int(x - (lo > 0 ? s_tiles[lo - 1] : 0)) * p.tpt;
+        Tile t;
+        t.tok0 = s_q0[lo] + i;
+        t.pos0 = s_kv[lo] - s_len[lo] + i;
+        t.ntok = min(p.tpt, s_len[lo] - i);
+        t.r = r0 + lo;
+        n = keys_of(t.pos0, t.ntok, p.window, p.sinks).n;
+        if (FFTS_IN_RANGE(tile_base + x, p.max_tiles)) p.tiles[tile_base + x] = t;
+      }
+      long long units;
+      const long long before = sched_scan(n, warp_sums, &units);
+      if (x < fit && FFTS_IN_RANGE(tile_base + x, p.max_tiles)) p.cum[tile_base + x + 1] = unit_base + before;
+      unit_base += units;
+    }
+    tile_base += max(fit, 0ll);
+    __syncthreads();  // the chunk's arrays have been read
+  }
+  if (tid == 0) p.header[0] = int(tile_base);
+}
+
+// Walks the (q tile, head, key tile) units [u, u1) segment by segment; the same in every lane.
+struct Walk {
+  const Params &p;
+  long long u, u1;
+  long long base, next;  // units before q tile x and behind it, all heads
+  int x;
+  Tile t;
+  Keys g;
+  int h, j0, j1;  // the segment: head and key tiles [j0, j1) of the g.n
+  __device__ __forceinline__ Walk(const Params &prm) : p(prm) {}
+
+  // Finds the q tile of unit u0 (whole warp; u0 < units).
+  __device__ __forceinline__ void seek(long long u0, long long end, int ntiles) {
+    u = u0;
+    u1 = end;
+    int lo = 0, n = ntiles;  // x is in [lo, lo + n): cum[lo] * Hkv <= u0
+    const int lane = threadIdx.x & 31;
+    while (n > 1) {
+      const int step = (n + 31) / 32;
+      const int i = lane * step;
+      const bool below = i < n && p.cum[lo + i] * p.Hkv <= u0;
+      const int last = 31 - __clz(__ballot_sync(0xffffffffu, below));
+      const int off = last * step;
+      lo += off;
+      n = min(step, n - off);
+    }
+    x = lo;
+    load();
+  }
+  __device__ __forceinline__ void load() {
+    t = p.tiles[FFTS_INDEX(x, p.max_tiles)];
+    base = p.cum[x] * p.Hkv;
+    next = p.cum[x + 1] * p.Hkv;
+    g = keys_of(t.pos0, t.ntok, p.window, p.sinks);
+  }
+  // The segment at u; false behind the share's end.
+  __device__ __forceinline__ bool segment() {
+    if (u >= u1) return false;
+    if (u >= next) {
+      ++x;
+      load();
+    }
+    const long long rem = u - base;
+    h = int(rem / g.n);
+    j0 = int(rem - (long long)h * g.n);
+    j1 = int(min((long long)g.n, j0 + (u1 - u)));
+    u += j1 - j0;
+    return true;
+  }
+};
+
+__device__ __forceinline__ uint64_t below(int k) { return k <= 0 ? 0ull : (k >= 64 ? ~0ull : (1ull << k) - 1ull); }
+
+template <typename E>
+struct Num;
+template <>
+struct Num<__nv_bfloat16> {
+  static constexpr uint32_t fmt = 1;
+  static constexpr CUtensorMapDataType map = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  // P <= 2^64 against the reference max: bf16 and the fp32 O have the exponents for it
+  static constexpr float rescale = 64.0f, pmax = 18446744073709551616.0f;
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    const __nv_bfloat162 r = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&r);
+  }
+};
+template <>
+struct Num<__half> {
+  static constexpr uint32_t fmt = 0;
+  static constexpr CUtensorMapDataType map = CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  // fp16 ends at 65504: P <= 2^8 after a rescale, 2^14 (a tile's row sum) before the next one; the row's
+  // top has P >= 1, so what is lost below 2^-24 is that far under it
+  static constexpr float rescale = 8.0f, pmax = 16384.0f;
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    const __half2 r = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&r);
+  }
+};
+
+constexpr uint32_t idesc(uint32_t fmt, bool b_mn_major, int n) {
+  return (1u << 4) | (fmt << 7) | (fmt << 10) | (b_mn_major ? (1u << 16) : 0u) | (uint32_t(n >> 3) << 17) |
+         (uint32_t(kBM >> 4) << 24);
+}
+
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *map, uint32_t bar, int c0, int c1, int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
+          dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
+
+template <typename E, int D>
+__global__ void __launch_bounds__(kThreads, 2)
+    attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ Params p) {
+  using Lay = Layout<D>;
+  extern __shared__ __align__(16) uint8_t smem[];
+  if (smem_u32(smem) & 1023u) {  // SWIZZLE_128B tiles need 1024-byte alignment
+    if (threadIdx.x == 0) *reinterpret_cast<volatile int *>(p.status) = kErrSmemAlign;
+    return;
+  }
+  const int ntiles = p.header[0];
+  const long long units = p.cum[FFTS_INDEX(ntiles, p.max_tiles + 1)] * p.Hkv;
+  const long long per = share_of(p, units);
+  const long long u0 = per * blockIdx.x, u1 = min(units, u0 + per);
+  if (u0 >= u1) return;  // uniform in the CTA, before any allocation
+  const uint32_t sbase = smem_u32(smem);
+  auto bar = [&](int i) { return sbase + Lay::bars + 8u * uint32_t(i); };
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + Lay::abort);
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + Lay::tmem_slot);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int qrows = p.tpt * p.G;  // rows a Q load fills
+
+  if (threadIdx.x == 0) {
+    *abort_flag = 0;
+    for (int i = 0; i < Lay::nbars; ++i) mbar_init(bar(i), (i == BPF || i == BPF + 1) ? 128u : 1u);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  // rows no Q load fills: zeros, so that they stay finite
+  for (int i = threadIdx.x; i < (kBM - qrows) * 8 * Lay::halves; i += kThreads) {
+    const int row = qrows + (i >> 3) / Lay::halves, hf = (i >> 3) % Lay::halves;
+    *reinterpret_cast<uint4 *>(smem + Lay::q + hf * Lay::q_half + row * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+  }
+  if (qrows < kBM) fence_proxy_async();
+  if (warp == 5) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                 "r"(kTmemCols));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  if (warp == 4 && lane == 0) {
+    prefetch_map(&tm_q);
+    prefetch_map(&tm_k);
+    prefetch_map(&tm_v);
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const uint32_t tm_o = tmem + kTmemO;
+  const int total = int(min(u1 - u0, (long long)0x7fffffff));
+
+  Walk w(p);
+  w.seek(u0, u1, ntiles);
+
+  if (warp == 4) {
+    // ============================================================ producer (whole warp)
+    const int ps = 1 << p.ps_shift;
+    const int box = min(ps, kBN);              // rows of one box
+    const int boxes = (kBN / box) * Lay::halves;
+    const int my_box = lane / Lay::halves, my_half = lane % Lay::halves;
+    const uint32_t my_dst = uint32_t(my_half * Lay::kv_half + my_box * box * 128);
+    // the lane's box of one key tile
+    struct Load {
+      int page, row, h;
+    };
+    int seg = -1, j = 0, j1 = 0;
+    bool fresh = false;  // the fetched tile is its segment's first
+    auto fetch = [&]() -> Load {
+      if (j >= j1) {
+        w.segment();
+        j = w.j0;
+        j1 = w.j1;
+        ++seg;
+        fresh = true;
+      } else {
+        fresh = false;
+      }
+      const int c = key_tile(w.g, j) * kBN + my_box * box;  // first key of the box
+      ++j;
+      Load l;
+      l.page = -1;
+      l.row = c & (ps - 1);
+      l.h = w.h;
+      if (lane < boxes && c < w.g.hi && (c + box > w.g.lo || c < p.sinks))
+        l.page = p.table[int64_t(w.t.r) * p.table_ld + FFTS_INDEX(c >> p.ps_shift, p.width)];
+      return l;
+    };
+    bool ok = true;
+    int nk = 0, nv = 0, nq = 0;  // loads issued
+    auto load = [&](const Load &l, bool is_k) {
+      const int n = is_k ? nk : nv;
+      const int stages = is_k ? kKStages : kVStages, s = n % stages;
+      const int full = (is_k ? BKF : BVF) + s, empty = (is_k ? BKE : BPV) + s;
+      ok = ok && __all_sync(0xffffffffu, mbar_wait(bar(empty), ((n / stages) & 1) ^ 1, abort_flag, p.wait_cycles));
+      if (!ok) return;
+      if (lane == 0) mbar_arrive_tx(bar(full), Lay::kv_bytes);
+      __syncwarp();
+      const uint32_t dst = sbase + (is_k ? Lay::k : Lay::v) + s * Lay::kv_bytes + my_dst;
+      if (lane < boxes) tma_load_4d(dst, is_k ? &tm_k : &tm_v, bar(full), my_half * 64, l.row, l.h, l.page);
+      if (is_k) ++nk; else ++nv;
+    };
+    Load cur = fetch(), prev = cur;
+    for (int n = 0; n < total && ok; ++n) {
+      const bool cur_fresh = fresh;
+      const int tok0 = w.t.tok0, qh = w.h * p.G;
+      Load next = cur;
+      // K(n), V(n - 1); a new segment's Q waits for the last S of the one before, so V(n - 1) goes first
+      if (cur_fresh && n > 0) load(prev, false);
+      load(cur, true);
+      if (cur_fresh && ok) {
+        ok = __all_sync(0xffffffffu, mbar_wait(bar(BQE), (nq & 1) ^ 1, abort_flag, p.wait_cycles));
+        if (ok && lane == 0) {
+          mbar_arrive_tx(bar(BQF), uint32_t(qrows * D * 2));
+          for (int hf = 0; hf < Lay::halves; ++hf)
+            tma_load_3d(sbase + Lay::q + hf * Lay::q_half, &tm_q, bar(BQF), hf * 64, qh, tok0);
+        }
+        if (ok) ++nq;
+      }
+      if (n + 1 < total) next = fetch();  // its page numbers arrive while the stages fill
+      if (!cur_fresh && n > 0) load(prev, false);
+      prev = cur;
+      cur = next;
+    }
+    if (ok) load(prev, false);
+    if (!ok) {
+      if (lane == 0) {
+        *abort_flag = 1;
+        *reinterpret_cast<volatile int *>(p.status) = kErrProducer;
+        // wait (bounded, ignoring the abort flag) for the copies in flight
+        volatile int never = 0;
+        if (nq > 0) mbar_wait(bar(BQF), (nq - 1) & 1, &never, p.drain_cycles);
+        for (int n = max(0, nk - kKStages); n < nk; ++n)
+          mbar_wait(bar(BKF + n % kKStages), (n / kKStages) & 1, &never, p.drain_cycles);
+        for (int n = max(0, nv - kVStages); n < nv; ++n)
+          mbar_wait(bar(BVF + n % kVStages), (n / kVStages) & 1, &never, p.drain_cycles);
+      }
+      __syncwarp();
+    }
+  } else if (warp == 5) {
+    // ============================================================ MMA issuer (one thread)
+    if (lane == 0) {
+      constexpr uint32_t idS = idesc(Num<E>::fmt, false, kBN), idPV = idesc(Num<E>::fmt, true, D);
+      const uint64_t dq = smem_desc(sbase + Lay::q, 16, 1024);
+      const uint64_t dk0 = smem_desc(sbase + Lay::k, 16, 1024);
+      const uint64_t dv0 = smem_desc(sbase + Lay::v, Lay::kv_half, 1024);
+      bool ok = true;
+      // S runs up to two tiles ahead of PV.  s_left: S tiles left in the walked segment; the PV side
+      // needs only to know which tiles begin a segment (bit n % 32 of firsts).
+      int s = 0, seg = 0, s_left = 0;
+      uint32_t firsts = 0;
+      for (int n = 0; n < total && ok; ++n) {
+        while (s < total && s < n + 2) {
+          const bool first = s_left == 0;
+          if (first) {
+            // a new segment's Q is not there yet: PV tiles that are due go first
+            if (s > n && !mbar_try(bar(BQF), seg & 1)) break;
+            ok = mbar_wait(bar(BQF), seg & 1, abort_flag, p.wait_cycles);
+            if (!ok) break;
+            w.segment();
+            s_left = w.j1 - w.j0;
+            ++seg;
+          }
+          const int ks = s % kKStages;
+          ok = mbar_wait(bar(BKF + ks), (s / kKStages) & 1, abort_flag, p.wait_cycles);
+          if (!ok) break;
+          fence_after();
+          const uint64_t dk = dk0 + uint64_t((ks * Lay::kv_bytes) >> 4);
+          const uint32_t td = tmem + (s & 1) * kBN;
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint32_t qoff = (kk >> 2) * Lay::q_half + (kk & 3) * 32;
+            const uint32_t koff = (kk >> 2) * Lay::kv_half + (kk & 3) * 32;
+            umma_f16(td, dq + (qoff >> 4), dk + (koff >> 4), idS, kk > 0 ? 1u : 0u);
+          }
+          umma_commit(bar(BSF + (s & 1)));
+          umma_commit(bar(BKE + ks));
+          if (--s_left == 0) umma_commit(bar(BQE));
+          firsts = (firsts & ~(1u << (s & 31))) | (uint32_t(first) << (s & 31));
+          ++s;
+        }
+        if (!ok) break;
+        const int b = n & 1;
+        ok = mbar_wait(bar(BVF + b), (n >> 1) & 1, abort_flag, p.wait_cycles) &&
+             mbar_wait(bar(BPF + b), (n >> 1) & 1, abort_flag, p.wait_cycles);
+        if (!ok) break;
+        fence_after();
+        const bool first = (firsts >> (n & 31)) & 1u;
+        const uint64_t dv = dv0 + uint64_t((b * Lay::kv_bytes) >> 4);
+        const uint32_t pt = tmem + b * kBN;  // P(n): pairs in the first 32 columns of S buffer n % 2
+#pragma unroll
+        for (int kk = 0; kk < kBN / 16; ++kk)
+          umma_f16_ts(tm_o, pt + kk * 8, dv + uint64_t((kk * 2048) >> 4), idPV, (!first || kk > 0) ? 1u : 0u);
+        umma_commit(bar(BPV + b));
+      }
+      if (!ok) {
+        *abort_flag = 1;
+        *reinterpret_cast<volatile int *>(p.status) = kErrMma;
+      }
+      // wait (bounded) until every MMA this thread issued has completed
+      umma_commit(bar(BDRAIN));
+      volatile int never = 0;
+      mbar_wait(bar(BDRAIN), 0, &never, p.drain_cycles);
+    }
+  } else {
+    // ============================================================ softmax (warps 0-3)
+    const int r = threadIdx.x;
+    const int tl = r / p.G, hg = r - tl * p.G;  // the row's token in the tile and head in the group
+    const uint32_t lane_off = uint32_t(warp * 32) << 16;
+    const float2 sc2 = make_float2(p.scale_log2, p.scale_log2);
+    bool ok = true, first_seg = true;
+    int n = 0;
+    while (ok && w.segment()) {
+      const Keys g = w.g;
+      const int nrows = w.t.ntok * p.G;
+      const bool active = warp * 32 < nrows;
+      // rows of no token take the last token's mask; nobody reads them
+      const int pos = w.t.pos0 + min(tl, w.t.ntok - 1);
+      float m_ref = -INFINITY, l_run = 0.0f;
+      for (int j = w.j0; j < w.j1; ++j, ++n) {
+        const int b = n & 1;
+        const uint32_t parity = (n >> 1) & 1;
+        if (!__all_sync(0xffffffffu, mbar_wait(bar(BSF + b), parity, abort_flag, p.wait_cycles))) { ok = false; break; }
+        fence_after();
+        const int c0 = key_tile(g, j) * kBN;
+        if (c0 + kBN > g.hi || (c0 < g.lo && c0 + kBN > p.sinks)) {
+          // V rows that no row sees
+          if (!__all_sync(0xffffffffu, mbar_wait(bar(BVF + b), parity, abort_flag, p.wait_cycles))) { ok = false; break; }
+          const int key = c0 + (r & 63);
+          if (r < 64 * Lay::halves && (key >= g.hi || (key < g.lo && key >= p.sinks))) {
+            uint8_t *vr = smem + Lay::v + b * Lay::kv_bytes + (r >> 6) * Lay::kv_half + (r & 63) * 128;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4 *>(vr + i * 16) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async();
+        }
+        if (active) {
+          uint64_t mask = below(pos + 1 - c0);
+          if (p.window > 0) mask &= ~below(pos - p.window + 1 - c0) | below(p.sinks - c0);
+          const bool edge = __any_sync(0xffffffffu, mask != ~0ull);
+          const uint32_t s_addr = tmem + b * kBN + lane_off;
+          float x[kBN];
+          tmem_ld32(s_addr, x);
+          tmem_wait_ld();
+          tmem_ld32(s_addr + 32, x + 32);  // lands while the first half is processed
+          if (edge) {
+#pragma unroll
+            for (int c = 0; c < 32; ++c)
+              if (!((uint32_t(mask) >> c) & 1u)) x[c] = -INFINITY;
+          }
+          // P = exp2(s * scale - m_ref) as pairs over the first 32 columns of this S buffer (columns
+          // already read).  The common path takes m_ref as it stands and keeps the result when every
+          // P of the row is small enough (by the tile's row sum); a row's first tile with a key, or one
+          // that outgrows m_ref, takes the max path: new m_ref, O and l rescaled, P again.
+          float2 rs2[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+          float alpha = 1.0f;
+          bool fast = !__any_sync(0xffffffffu, m_ref == -INFINITY);
+          auto exp_half = [&](int cc, float2 off2) {
+            uint32_t pk[16];
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              const int c = cc * 32 + e;
+              const float2 a = __ffma2_rn(make_float2(x[c], x[c + 1]), sc2, off2);
+              float2 ex;
+              ex.x = fast_exp2(a.x);
+              ex.y = fast_exp2(a.y);
+              rs2[(e >> 1) & 1] = __fadd2_rn(rs2[(e >> 1) & 1], ex);
+              pk[e >> 1] = Num<E>::pack(ex.x, ex.y);
+            }
+            tmem_st16u(s_addr + cc * 16, pk);
+          };
+          auto mask_high = [&]() {
+            if (edge) {
+#pragma unroll
+              for (int c = 0; c < 32; ++c)
+                if (!((uint32_t(mask >> 32) >> c) & 1u)) x[32 + c] = -INFINITY;
+            }
+          };
+          if (fast) {
+            const float moff = m_ref * p.scale_log2;
+            exp_half(0, make_float2(-moff, -moff));
+            tmem_wait_ld();
+            mask_high();
+            exp_half(1, make_float2(-moff, -moff));
+            const float tsum = (rs2[0].x + rs2[0].y) + (rs2[1].x + rs2[1].y);
+            if (__any_sync(0xffffffffu, !(tsum <= Num<E>::pmax))) {
+              fast = false;
+              tmem_wait_st();  // the max path below rewrites P
+              rs2[0] = rs2[1] = make_float2(0.0f, 0.0f);
+            }
+          } else {
+            tmem_wait_ld();
+            mask_high();
+          }
+          if (!fast) {
+            float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int c = 0; c < kBN; c += 2) mx4[(c >> 1) & 3] = max3f(mx4[(c >> 1) & 3], x[c], x[c + 1]);
+            const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+            if (mx > m_ref && (m_ref == -INFINITY || (mx - m_ref) * p.scale_log2 > Num<E>::rescale)) {
+              alpha = m_ref == -INFINITY ? 0.0f : fast_exp2((m_ref - mx) * p.scale_log2);
+              m_ref = mx;
+            }
+            const float moff = (m_ref == -INFINITY ? 0.0f : m_ref) * p.scale_log2;
+            exp_half(0, make_float2(-moff, -moff));
+            exp_half(1, make_float2(-moff, -moff));
+          }
+          const float2 rsum = __fadd2_rn(rs2[0], rs2[1]);
+          l_run = l_run * alpha + (rsum.x + rsum.y);
+          tmem_wait_st();
+          if (j > w.j0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
+            // O must hold PV(n-1) before it is rescaled; its barrier's next phase needs P(n+1)
+            if (!__all_sync(0xffffffffu,
+                            mbar_wait(bar(BPV + (n - 1) % 2), ((n - 1) >> 1) & 1, abort_flag, p.wait_cycles))) {
+              ok = false;
+              break;
+            }
+            fence_after();
+#pragma unroll 1
+            for (int c = 0; c < D / 32; ++c) {
+              float o[32];
+              tmem_ld32(tm_o + lane_off + c * 32, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; e += 2) {
+                const float2 v = __fmul2_rn(make_float2(o[e], o[e + 1]), make_float2(alpha, alpha));
+                o[e] = v.x;
+                o[e + 1] = v.y;
+              }
+              tmem_st32(tm_o + lane_off + c * 32, o);
+            }
+            tmem_wait_st();
+          }
+        }
+        fence_before();
+        mbar_arrive(bar(BPF + b));
+      }
+      if (!ok) break;
+      // O is final once the segment's last PV is complete (its barrier's next phase needs our P)
+      if (!__all_sync(0xffffffffu, mbar_wait(bar(BPV + (n - 1) % 2), ((n - 1) >> 1) & 1, abort_flag, p.wait_cycles))) {
+        ok = false;
+        break;
+      }
+      fence_after();
+      if (active) {
+        const bool whole = w.j0 == 0 && w.j1 == g.n;
+        const bool live = r < nrows;
+        const int slot = 2 * int(blockIdx.x) + (first_seg ? 0 : 1);
+        const float inv_l = l_run > 0.0f ? 1.0f / l_run : 0.0f;
+        uint16_t *dst = p.out + int64_t(w.t.tok0 + tl) * p.os_t + int64_t(w.h * p.G + hg) * p.os_h;
+        float *pd = p.part + (int64_t(slot) * kBM + r) * D;
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          float o[32];
+          tmem_ld32(tm_o + lane_off + c * 32, o);
+          tmem_wait_ld();
+          if (!live) continue;
+          if (whole) {
+            if (!FFTS_IN_RANGE(w.t.tok0 + tl, p.T)) continue;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              uint32_t v[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                v[e] = Num<E>::pack(l_run > 0.0f ? o[q * 8 + 2 * e] * inv_l : 0.0f,
+                                    l_run > 0.0f ? o[q * 8 + 2 * e + 1] * inv_l : 0.0f);
+              *reinterpret_cast<uint4 *>(dst + c * 32 + q * 8) = make_uint4(v[0], v[1], v[2], v[3]);
+            }
+          } else if (FFTS_IN_RANGE(slot, 2 * p.ctas)) {
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+              *reinterpret_cast<float4 *>(pd + c * 32 + q * 4) =
+                  make_float4(o[q * 4], o[q * 4 + 1], o[q * 4 + 2], o[q * 4 + 3]);
+          }
+        }
+        if (live && !whole && FFTS_IN_RANGE(slot, 2 * p.ctas))
+          p.part_ml[int64_t(slot) * kBM + r] = make_float2(m_ref * p.scale_log2, l_run);
+      }
+      first_seg = false;
+    }
+    if (!ok) {
+      *abort_flag = 1;
+      *reinterpret_cast<volatile int *>(p.status) = kErrSoftmax;
+    }
+  }
+
+  fence_before();
+  __syncthreads();
+  fence_after();
+  if (warp == 5) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
+}
+
+// ---------------------------------------------------------------- merge
+constexpr int kMergeWarps = 4;
+
+// Block (c, y): the (q tile, head) that share c - 1 begins and share c goes on with, rows y * 4 + warp of
+// every gridDim.y * 4.  Its partials are share c - 1's last segment and the first ones of c, c + 1, ...
+template <typename E, int D>
+__global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const __grid_constant__ Params p) {
+  const int ntiles = p.header[0];
+  const long long units = p.cum[FFTS_INDEX(ntiles, p.max_tiles + 1)] * p.Hkv;
+  const long long per = share_of(p, units);
+  const int c = int(blockIdx.x) + 1;
+  const long long u = per * c;
+  if (u >= units) return;
+  Walk w(p);
+  w.seek(u, u + 1, ntiles);
+  w.segment();
+  if (w.j0 == 0) return;  // the cut lies between two
+  const long long begin = u - w.j0, end = begin + w.g.n;
+  if (begin / per != c - 1) return;  // an earlier block's
+  const int last = int((end - 1) / per);
+  const int first_slot = 2 * (c - 1) + (begin % per == 0 ? 0 : 1);
+  const int lane = threadIdx.x & 31;
+  const int nrows = w.t.ntok * p.G;
+  constexpr int kC = D / 32;  // channels per lane
+  for (int r = int(blockIdx.y) * kMergeWarps + (threadIdx.x >> 5); r < nrows; r += int(gridDim.y) * kMergeWarps) {
+    float m = -INFINITY;
+    for (int s = c - 1 + lane; s <= last; s += 32) {
+      const int slot = s == c - 1 ? first_slot : 2 * s;
+      m = fmaxf(m, p.part_ml[int64_t(FFTS_INDEX(slot, 2 * p.ctas)) * kBM + r].x);
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    float acc[kC], l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kC; ++i) acc[i] = 0.0f;
+#pragma unroll 4
+    for (int s = c - 1; s <= last; ++s) {
+      const int slot = FFTS_INDEX(s == c - 1 ? first_slot : 2 * s, 2 * p.ctas);
+      const float2 ml = p.part_ml[int64_t(slot) * kBM + r];
+      const float *src = p.part + (int64_t(slot) * kBM + r) * D + lane * kC;
+      float v[kC];
+      if (kC == 4) {
+        const float4 q = *reinterpret_cast<const float4 *>(src);
+        v[0] = q.x; v[1] = q.y; v[kC - 2] = q.z; v[kC - 1] = q.w;
+      } else {
+        const float2 q = *reinterpret_cast<const float2 *>(src);
+        v[0] = q.x; v[1] = q.y;
+      }
+      // a share whose keys the row does not see has l = 0 and m = -inf: nothing of it counts
+      const float f = ml.x == -INFINITY ? 0.0f : exp2f(ml.x - m);
+      l = fmaf(f, ml.y, l);
+#pragma unroll
+      for (int i = 0; i < kC; ++i) acc[i] = fmaf(f, f > 0.0f ? v[i] : 0.0f, acc[i]);
+    }
+    const float inv_l = l > 0.0f ? 1.0f / l : 0.0f;
+    const int tl = r / p.G, hg = r - tl * p.G;
+    uint16_t *dst = p.out + int64_t(w.t.tok0 + tl) * p.os_t + int64_t(w.h * p.G + hg) * p.os_h + lane * kC;
+    if (FFTS_IN_RANGE(w.t.tok0 + tl, p.T)) {
+#pragma unroll
+      for (int i = 0; i < kC; i += 2)
+        *reinterpret_cast<uint32_t *>(dst + i) = Num<E>::pack(l > 0.0f ? acc[i] * inv_l : 0.0f,
+                                                              l > 0.0f ? acc[i + 1] * inv_l : 0.0f);
+    }
+  }
+}
+
+// ---------------------------------------------------------------- host side
+static PFN_cuTensorMapEncodeTiled_v12000 get_encode() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+    void *ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
+    return static_cast<PFN_cuTensorMapEncodeTiled_v12000>(nullptr);
+  }();
+  return fn;
+}
+
+static int encode(CUtensorMap *map, CUtensorMapDataType type, int rank, const void *base, const cuuint64_t *dims,
+                  const cuuint64_t *strides, const cuuint32_t *box) {
+  auto enc = get_encode();
+  if (!enc) {
+    set_error(FFTS_E_CUDA, "cuTensorMapEncodeTiled is unavailable");
+    return FFTS_E_CUDA;
+  }
+  const cuuint32_t ones[5] = {1, 1, 1, 1, 1};
+  const CUresult r = enc(map, type, rank, const_cast<void *>(base), dims, strides, box, ones,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_error(FFTS_E_INVALID, "paged_attn: cuTensorMapEncodeTiled failed (%d)", int(r));
+    return FFTS_E_INVALID;
+  }
+  return FFTS_OK;
+}
+
+__device__ int g_status_sink;
+
+// Workspace: cum, tiles, header, partial (m, l), partial O; every part a multiple of 16 bytes.
+struct Space {
+  int64_t max_tiles, cum, tiles, header, ml, part, bytes;
+  Space(int64_t T, int64_t R, int64_t G, int64_t D) {
+    const int64_t tpt = kBM / G;
+    max_tiles = T / tpt + std::min(R, T);  // sum of ceil(len / tpt)
+    cum = 0;
+    tiles = cum + (max_tiles + 2) / 2 * 16;
+    header = tiles + max_tiles * 16;
+    ml = header + 16;
+    part = ml + int64_t(2 * kMaxCtas) * kBM * 8;
+    bytes = part + int64_t(2 * kMaxCtas) * kBM * D * 4;
+  }
+};
+
+template <typename E, int D>
+static int launch(const Params &p, const void *q, const int64_t *qs, const void *k, const int64_t *ks, const void *v,
+                  const int64_t *vs, cudaStream_t stream) {
+  CUtensorMap mq, mk, mv;
+  const cuuint64_t qd[3] = {D, cuuint64_t(p.H), cuuint64_t(p.T)};
+  const cuuint64_t qst[2] = {cuuint64_t(qs[1]) * 2, cuuint64_t(qs[0]) * 2};
+  const cuuint32_t qbox[3] = {64, cuuint32_t(p.G), cuuint32_t(p.tpt)};
+  int rc = encode(&mq, Num<E>::map, 3, q, qd, qst, qbox);
+  if (rc) return rc;
+  const cuuint64_t ps = 1ull << p.ps_shift;
+  const cuuint64_t kd[4] = {D, ps, cuuint64_t(p.Hkv), cuuint64_t(p.n_pages)};
+  const cuuint32_t kbox[4] = {64, cuuint32_t(std::min<cuuint64_t>(ps, kBN)), 1, 1};
+  const cuuint64_t kst[3] = {cuuint64_t(ks[2]) * 2, cuuint64_t(ks[1]) * 2, cuuint64_t(ks[0]) * 2};
+  const cuuint64_t vst[3] = {cuuint64_t(vs[2]) * 2, cuuint64_t(vs[1]) * 2, cuuint64_t(vs[0]) * 2};
+  rc = encode(&mk, Num<E>::map, 4, k, kd, kst, kbox);
+  if (!rc) rc = encode(&mv, Num<E>::map, 4, v, kd, vst, kbox);
+  if (!rc)
+    rc = ensure_func_smem(reinterpret_cast<const void *>(&attn_kernel<E, D>), Layout<D>::bytes,
+                          int(cudaSharedmemCarveoutMaxShared));
+  if (rc) return rc;
+  schedule_kernel<<<1, kSchedThreads, 0, stream>>>(p);
+  FFTS_CUDA(cudaGetLastError());
+  attn_kernel<E, D><<<unsigned(p.ctas), kThreads, Layout<D>::bytes, stream>>>(mq, mk, mv, p);
+  FFTS_CUDA(cudaGetLastError());
+  if (p.ctas > 1) {
+    // rows of the largest tile, in 8 blocks
+    const dim3 grid(unsigned(p.ctas - 1), unsigned(std::min<int64_t>(8, ceil_div(int64_t(p.tpt) * p.G, kMergeWarps))));
+    merge_kernel<E, D><<<grid, kMergeWarps * 32, 0, stream>>>(p);
+    FFTS_CUDA(cudaGetLastError());
+  }
+  return FFTS_OK;
+}
+
+}  // namespace paged
+
+int64_t paged_workspace_bytes(int64_t T, int64_t R, int64_t H, int64_t Hkv, int64_t D) {
+  if (T <= 0 || R <= 0 || H <= 0 || Hkv <= 0 || D <= 0 || H % Hkv || H / Hkv > paged::kBM) return 0;
+  return paged::Space(T, R, H / Hkv, D).bytes;
+}
+
+int paged_attn(const void *q, const int64_t *qs, const void *k_pages, const int64_t *ks, const void *v_pages,
+               const int64_t *vs, int dtype, int64_t T, int64_t R, int64_t H, int64_t Hkv, int64_t D, int64_t n_pages,
+               int64_t page_size, const int32_t *table, int64_t table_ld, int64_t width, const int32_t *cu_q,
+               const int32_t *kv_lens, float scale, int64_t window, int64_t sinks, void *out, const int64_t *os,
+               void *ws, int64_t ws_bytes, int32_t *status, cudaStream_t stream) {
+  using namespace paged;
+  FFTS_REQUIRE(dtype == FFTS_DTYPE_BF16 || dtype == FFTS_DTYPE_F16, "paged_attn: dtype must be bf16 or fp16");
+  FFTS_REQUIRE(D == 64 || D == 128, "paged_attn: head_dim must be 64 or 128 (got %lld)", (long long)D);
+  FFTS_REQUIRE(T >= 0 && R >= 0 && H >= 1 && Hkv >= 1 && H % Hkv == 0 && H / Hkv <= kBM,
+               "paged_attn: bad shape (T %lld, R %lld, H %lld, Hkv %lld; at most %d query heads per KV head)",
+               (long long)T, (long long)R, (long long)H, (long long)Hkv, kBM);
+  FFTS_REQUIRE(page_size >= 16 && page_size <= 256 && (page_size & (page_size - 1)) == 0,
+               "paged_attn: page_size must be 16, 32, 64, 128 or 256 (got %lld)", (long long)page_size);
+  FFTS_REQUIRE(T <= (int64_t(1) << 30) && R <= (int64_t(1) << 30) && H <= 65536 && n_pages < (int64_t(1) << 31) &&
+                   width >= 0 && width * page_size <= (int64_t(1) << 30),
+               "paged_attn: shape too large (a table row spans at most 2^30 tokens)");
+  FFTS_REQUIRE(window >= 0 && sinks >= 0, "paged_attn: window and sinks must not be negative");
+  FFTS_REQUIRE(scale > 0.0f && scale < 3.0e38f, "paged_attn: scale must be positive and finite");
+  if (T == 0 || R == 0) return FFTS_OK;
+  FFTS_REQUIRE(q && qs && k_pages && ks && v_pages && vs && cu_q && kv_lens && out && os && ws &&
+                   (width == 0 || table) && n_pages >= 1,
+               "paged_attn: NULL argument or empty pool");
+  FFTS_REQUIRE(table_ld >= width || R == 1, "paged_attn: table rows overlap");
+  auto aligned = [](const void *x) { return (reinterpret_cast<uintptr_t>(x) & 15) == 0; };
+  FFTS_REQUIRE(aligned(q) && aligned(k_pages) && aligned(v_pages) && aligned(out) && aligned(ws),
+               "paged_attn: tensors must be 16-byte aligned");
+  FFTS_REQUIRE(qs[0] > 0 && qs[1] > 0 && qs[0] % 8 == 0 && qs[1] % 8 == 0 && os[0] % 8 == 0 && os[1] % 8 == 0,
+               "paged_attn: q and out strides must be positive multiples of 8 elements (16 bytes)");
+  for (const int64_t *st : {ks, vs})
+    for (int i = 0; i < 3; ++i)
+      FFTS_REQUIRE(st[i] > 0 && st[i] % 8 == 0 && st[i] < (int64_t(1) << 38),
+                   "paged_attn: page strides must be positive multiples of 8 elements (16 bytes)");
+  FFTS_REQUIRE(ws_bytes >= paged_workspace_bytes(T, R, H, Hkv, D), "paged_attn: workspace too small");
+  const int64_t G = H / Hkv;
+  const Space sp(T, R, G, D);
+  uint8_t *base = static_cast<uint8_t *>(ws);
+  Params p{};
+  p.T = int(T); p.R = int(R); p.H = int(H); p.Hkv = int(Hkv); p.G = int(G); p.tpt = int(kBM / G);
+  p.table = table;
+  p.table_ld = table_ld;
+  p.width = int(width);
+  p.n_pages = int(n_pages);
+  p.ps_shift = ilog2_ceil(page_size);
+  p.cu_q = cu_q;
+  p.kv_lens = kv_lens;
+  p.window = int(std::min<int64_t>(window, int64_t(1) << 30));
+  p.sinks = window > 0 ? int(std::min<int64_t>(sinks, int64_t(1) << 30)) : 0;
+  p.out = static_cast<uint16_t *>(out);
+  p.os_t = os[0];
+  p.os_h = os[1];
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.max_tiles = int(sp.max_tiles);
+  p.cum = reinterpret_cast<long long *>(base + sp.cum);
+  p.tiles = reinterpret_cast<Tile *>(base + sp.tiles);
+  p.header = reinterpret_cast<int *>(base + sp.header);
+  p.part_ml = reinterpret_cast<float2 *>(base + sp.ml);
+  p.part = reinterpret_cast<float *>(base + sp.part);
+  int sms = 0;
+  int rc = device_sm_count(&sms);
+  if (!rc) rc = device_wait_cycles(kWaitSeconds, &p.wait_cycles);
+  if (!rc) rc = device_wait_cycles(kDrainSeconds, &p.drain_cycles);
+  if (rc) return rc;
+  p.ctas = std::min(2 * sms, kMaxCtas);
+  if (status) {
+    p.status = status;
+  } else {
+    void *sink = nullptr;
+    FFTS_CUDA(cudaGetSymbolAddress(&sink, g_status_sink));
+    p.status = static_cast<int *>(sink);
+  }
+  if (dtype == FFTS_DTYPE_BF16)
+    return D == 128 ? launch<__nv_bfloat16, 128>(p, q, qs, k_pages, ks, v_pages, vs, stream)
+                    : launch<__nv_bfloat16, 64>(p, q, qs, k_pages, ks, v_pages, vs, stream);
+  return D == 128 ? launch<__half, 128>(p, q, qs, k_pages, ks, v_pages, vs, stream)
+                  : launch<__half, 64>(p, q, qs, k_pages, ks, v_pages, vs, stream);
+}
+
+}  // namespace ffts

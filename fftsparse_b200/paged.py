@@ -1,0 +1,327 @@
+"""Paged serving: many requests over one pool of KV pages (ffts_page_plan, ffts_rope_append, ffts_paged_attn).
+
+The reference's callers prefill one prompt and decode it over one contiguous
+cache (eval/LongBench/pred.py:177-322).  A server keeps many requests whose caches grow token by token in
+pages of a shared pool.  One step of it:
+
+    plan = plan_pages(cached_lens, new_lens, block_table, free_pages, page_size, num_tokens)   # once
+    for each layer:
+        q = rope_append(q, k, v, plan.positions, plan.slot_map, k_pages, v_pages, inv_freq)
+        out = paged_attention(q, k_pages, v_pages, block_table, plan.cu_q, plan.kv_lens)
+
+New tokens are packed: request r owns rows ``cu_q[r] .. cu_q[r + 1] - 1`` of q, k, v and out.  One token is
+decoding, more are a chunk of its prompt; a step may mix them.  Lengths and tables are device tensors that the
+host never reads, so a step can be captured into a CUDA graph and replayed with other lengths.
+
+The pool's tensors are [pages, Hkv, page_size, D], the head-major layout the other
+operators use; a token-major pool [pages, page_size, Hkv, D] is passed as
+``pool.transpose(1, 2)``.  A prompt that ``myattn_prefill`` has attended is
+handed over with ``rope_append(None, k[0].transpose(0, 1), v[0].transpose(0, 1), ..., inv_freq=None)``,
+which copies the already rotated k.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import NamedTuple, Optional, Tuple
+
+import torch
+
+from . import _lib
+from .status import device_status
+
+__all__ = ["PagePlan", "plan_pages", "rotary_inv_freq", "rope_append", "paged_attention"]
+
+_DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
+_I64x2 = ctypes.c_int64 * 2
+_I64x3 = ctypes.c_int64 * 3
+
+
+def _on_device(device: torch.device, fn, *args) -> None:
+    """One C call with ``device`` current, on its current stream."""
+    if device.index == torch.cuda.current_device():
+        _lib.check(fn(*args, torch.cuda.current_stream(device).cuda_stream))
+    else:
+        with torch.cuda.device(device):
+            _lib.check(fn(*args, torch.cuda.current_stream(device).cuda_stream))
+
+
+def _check_ints(name: str, t: torch.Tensor, shape, device) -> None:
+    if t.dtype != torch.int32:
+        raise TypeError(f"{name} must be int32, got {t.dtype}")
+    if t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous tensor of shape {tuple(shape)}, got {tuple(t.shape)}")
+    if t.device != device:
+        raise ValueError(f"{name} must be on {device}, got {t.device}")
+
+
+def _check_table(t: torch.Tensor, rows: int, device) -> None:
+    if t.dtype != torch.int32:
+        raise TypeError(f"block_table must be int32, got {t.dtype}")
+    if t.dim() != 2 or t.shape[0] != rows or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise ValueError(f"block_table must be [{rows}, pages] with unit stride along a row, got {tuple(t.shape)}")
+    if t.device != device:
+        raise ValueError(f"block_table must be on {device}, got {t.device}")
+
+
+def _check_heads(name: str, t: torch.Tensor, dtype, device) -> None:
+    if t.dim() != 3:
+        raise ValueError(f"{name} must be [tokens, heads, head_dim], got shape {tuple(t.shape)}")
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.device != device:
+        raise ValueError(f"{name} must be on {device}, got {t.device}")
+    if t.stride(2) != 1:
+        raise ValueError(f"{name} must be contiguous in the head dimension")
+
+
+def _check_pool(k_pages: torch.Tensor, v_pages: torch.Tensor, dtype, device) -> None:
+    if k_pages.dim() != 4 or v_pages.shape != k_pages.shape:
+        raise ValueError(f"k_pages and v_pages must both be [pages, Hkv, page_size, D], got "
+                         f"{tuple(k_pages.shape)} / {tuple(v_pages.shape)}")
+    if k_pages.dtype != dtype or v_pages.dtype != dtype:
+        raise TypeError(f"k_pages and v_pages must be {dtype}, got {k_pages.dtype} / {v_pages.dtype}")
+    if k_pages.device != device or v_pages.device != device:
+        raise ValueError(f"k_pages and v_pages must be on {device}")
+    if k_pages.stride(3) != 1 or v_pages.stride(3) != 1:
+        raise ValueError("k_pages and v_pages must be contiguous in the head dimension")
+
+
+def _check_cuda(name: str, t: torch.Tensor) -> None:
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor")
+
+
+class PagePlan(NamedTuple):
+    """The bookkeeping of one step (``plan_pages``)."""
+
+    cu_q: torch.Tensor       # int32 [R + 1]: first row of each request's new tokens
+    kv_lens: torch.Tensor    # int32 [R]: cached + new tokens, 0 for a request that is not served
+    positions: torch.Tensor  # int32 [num_tokens]
+    slot_map: torch.Tensor   # int32 [num_tokens]: page * page_size + row in the pool, -1 for none
+    info: torch.Tensor       # int32 [2]: pages taken from the free list, requests not served
+
+
+def plan_pages(cached_lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Tensor,
+               free_pages: torch.Tensor, page_size: int, num_tokens: int) -> PagePlan:
+    """Page bookkeeping of one step on the GPU (ffts_page_plan).
+
+    ``cached_lens`` / ``new_lens`` int32 [R]: tokens each request has in the cache, and adds in this step.
+    ``block_table`` int32 [R, width]: its page numbers, the first ceil(cached / page_size) of a row valid; the
+    entries of the pages that the new tokens begin are filled in place with ``free_pages`` (int32, taken
+    from the front in the order of the requests).  ``num_tokens``: rows of the step's token
+    arrays, at least the sum of ``new_lens``; rows behind the last token get position 0 and slot -1, so a
+    batch padded to a fixed size can be replayed from a graph.
+
+    A request is served if its pages fit its row, its tokens fit ``num_tokens`` and its new pages, counted on
+    from those of the requests before it, fit the free list.  Otherwise its kv_len is 0 and its slots are -1:
+    its tokens are not appended and attend to nothing.  ``info`` holds the pages taken and the requests
+    not served; the caller drops that many entries from the front of its list.  Nothing is read back.
+    """
+    dev = cached_lens.device
+    if cached_lens.dim() != 1 or free_pages.dim() != 1:
+        raise ValueError("cached_lens and free_pages must be 1-D")
+    R = cached_lens.shape[0]
+    _check_ints("cached_lens", cached_lens, (R,), dev)
+    _check_ints("new_lens", new_lens, (R,), dev)
+    _check_table(block_table, R, dev)
+    _check_ints("free_pages", free_pages, free_pages.shape, dev)
+    if num_tokens < 0:
+        raise ValueError(f"num_tokens must not be negative, got {num_tokens}")
+    _check_cuda("cached_lens", cached_lens)
+    buf = torch.empty(2 * R + 3 + 2 * num_tokens, dtype=torch.int32, device=dev)
+    plan = PagePlan(*buf.split([R + 1, R, num_tokens, num_tokens, 2]))
+    width = block_table.shape[1]
+    _on_device(dev, _lib.load().ffts_page_plan, cached_lens.data_ptr(), new_lens.data_ptr(), R,
+               block_table.data_ptr(), block_table.stride(0) if R > 1 else width, width, free_pages.data_ptr(),
+               free_pages.shape[0], page_size, num_tokens, *[t.data_ptr() for t in plan])
+    return plan
+
+
+def rotary_inv_freq(rotary_dim: int, base: float = 10000.0, scaling: Optional[dict] = None,
+                    seq_len: Optional[int] = None, device=None) -> Tuple[torch.Tensor, float]:
+    """(inv_freq fp32 [rotary_dim / 2], attn_factor) of a rotary embedding, as ``rope_append`` takes them.
+
+    ``scaling`` is a model configuration's ``rope_scaling`` dict; its ``rope_type`` is one of
+
+      default  f_i = base^(-2i / d)
+      linear   f_i / factor
+      dynamic  base grown to base (factor L / L0 - factor + 1)^(d / (d - 2)), L = max(seq_len, L0)
+      llama3   f_i / factor for wavelengths above L0 / low_freq_factor, f_i below L0 / high_freq_factor, a linear
+               blend between
+      yarn     f_i / factor and f_i blended over the channels that turn beta_slow to beta_fast times within L0;
+               attn_factor = attention_factor or 0.1 ln(factor) + 1
+
+    with L0 = ``original_max_position_embeddings``.  Computed in 64 bits, rounded once.
+    """
+    if rotary_dim <= 0 or rotary_dim % 2:
+        raise ValueError(f"rotary_dim must be a positive even number, got {rotary_dim}")
+    d, scaling = rotary_dim, scaling or {}
+    kind = scaling.get("rope_type", scaling.get("type", "default"))
+    if kind == "dynamic" and d == 2:
+        raise ValueError("rope scaling 'dynamic' needs rotary_dim above 2")
+    i = torch.arange(0, d, 2, dtype=torch.float64)
+    attn = 1.0
+
+    def need(key):
+        if key not in scaling:
+            raise ValueError(f"rope scaling '{kind}' needs '{key}'")
+        return float(scaling[key])
+
+    if kind == "dynamic":
+        L0, s = need("original_max_position_embeddings"), need("factor")
+        L = max(float(seq_len or 0), L0)
+        base = base * (s * L / L0 - (s - 1.0)) ** (d / (d - 2))
+    f = float(base) ** (-i / d)
+    if kind == "linear":
+        f = f / need("factor")
+    elif kind == "llama3":
+        L0, s = need("original_max_position_embeddings"), need("factor")
+        low, high = need("low_freq_factor"), need("high_freq_factor")
+        turns = L0 * f / (2.0 * math.pi)  # within the original context
+        keep = ((turns - low) / (high - low)).clamp(0.0, 1.0)
+        f = keep * f + (1.0 - keep) * f / s
+    elif kind == "yarn":
+        L0, s = need("original_max_position_embeddings"), need("factor")
+
+        def channel(turns):  # the pair that turns so often within L0
+            return d * math.log(L0 / (turns * 2.0 * math.pi)) / (2.0 * math.log(base))
+
+        lo = max(math.floor(channel(float(scaling.get("beta_fast", 32.0)))), 0)
+        hi = min(math.ceil(channel(float(scaling.get("beta_slow", 1.0)))), d - 1)
+        slow = ((i / 2 - lo) / max(hi - lo, 1e-3)).clamp(0.0, 1.0)
+        f = slow * f / s + (1.0 - slow) * f
+        given = scaling.get("attention_factor")
+        attn = float(given) if given is not None else (0.1 * math.log(s) + 1.0 if s > 1.0 else 1.0)
+    elif kind not in ("default", "dynamic"):
+        raise ValueError(f"unknown rope scaling '{kind}'")
+    return f.to(torch.float32).to(device), attn
+
+
+def rope_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor,
+                slot_map: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                inv_freq: Optional[torch.Tensor], *, interleaved: bool = False, attn_factor: float = 1.0,
+                out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+    """Rotate q and k by their positions and append k and v to the paged cache, in one pass (ffts_rope_append).
+
+    q [T, H, D] (or None), k / v [T, Hkv, D]: bf16 or fp16, D 64 or 128, unit stride over D (views of one fused
+    QKV projection are fine).  ``positions`` / ``slot_map`` int32 [T] (``plan_pages``); a token whose
+    slot lies outside the pool is not appended.  ``inv_freq`` fp32 [rotary_dim / 2] (``rotary_inv_freq``), rotary_dim
+    a multiple of 16: the first rotary_dim channels turn by position * inv_freq, in pairs (i, i + rotary_dim / 2),
+    or (2i, 2i + 1) with ``interleaved``; cos and sin are multiplied by ``attn_factor``; the other channels are
+    copied.  None copies k (and q) as they are.  ``k_pages`` / ``v_pages`` [pages, Hkv, page_size, D] are
+    written in place.  Returns the rotated q [T, H, D] (``out``, which may be q itself, or a new tensor), None
+    without q.  The angles are exact for far positions (64 bits), the rotation is fp32, rounded once.
+    """
+    dev, dt = k.device, k.dtype
+    if dt not in _DTYPES:
+        raise TypeError(f"rope_append supports bfloat16 and float16, got {dt}")
+    _check_heads("k", k, dt, dev)
+    _check_heads("v", v, dt, dev)
+    T, Hkv, D = k.shape
+    if v.shape != k.shape:
+        raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} differ in shape")
+    _check_pool(k_pages, v_pages, dt, dev)
+    if k_pages.shape[1] != Hkv or k_pages.shape[3] != D:
+        raise ValueError(f"pages {tuple(k_pages.shape)} do not match k {tuple(k.shape)}")
+    _check_ints("positions", positions, (T,), dev)
+    _check_ints("slot_map", slot_map, (T,), dev)
+    rd = 0
+    if inv_freq is not None:
+        if inv_freq.dim() != 1 or inv_freq.dtype != torch.float32 or not inv_freq.is_contiguous():
+            raise ValueError("inv_freq must be a contiguous 1-D fp32 tensor")
+        if inv_freq.device != dev:
+            raise ValueError(f"inv_freq must be on {dev}, got {inv_freq.device}")
+        rd = 2 * inv_freq.shape[0]
+    if q is not None:
+        _check_heads("q", q, dt, dev)
+        if q.shape[0] != T or q.shape[2] != D:
+            raise ValueError(f"q {tuple(q.shape)} does not match k {tuple(k.shape)}")
+    if out is not None:
+        if q is None:
+            raise ValueError("out without q")
+        _check_heads("out", out, dt, dev)
+        if out.shape != q.shape:
+            raise ValueError(f"out must have q's shape {tuple(q.shape)}, got {tuple(out.shape)}")
+    _check_cuda("k", k)
+    H, q_ptr, o_ptr, qs, os_ = 0, None, None, None, None
+    if q is not None:
+        H = q.shape[1]
+        if out is None:
+            out = torch.empty(T, H, D, dtype=dt, device=dev)
+        q_ptr, o_ptr = q.data_ptr(), out.data_ptr()
+        qs, os_ = _I64x2(q.stride(0), q.stride(1)), _I64x2(out.stride(0), out.stride(1))
+    if T == 0:
+        return out
+    P, _, page_size, _ = k_pages.shape
+    _on_device(dev, _lib.load().ffts_rope_append, q_ptr, qs, k.data_ptr(), _I64x2(k.stride(0), k.stride(1)),
+               v.data_ptr(), _I64x2(v.stride(0), v.stride(1)), _DTYPES[dt], T, H, Hkv, D, positions.data_ptr(),
+               slot_map.data_ptr(), inv_freq.data_ptr() if rd else None, rd, int(bool(interleaved)),
+               float(attn_factor), o_ptr, os_, k_pages.data_ptr(), _I64x3(*k_pages.stride()[:3]), v_pages.data_ptr(),
+               _I64x3(*v_pages.stride()[:3]), P, page_size)
+    return out
+
+
+def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor,
+                    cu_q: torch.Tensor, kv_lens: torch.Tensor, *, scale: Optional[float] = None,
+                    window: Optional[int] = None, sinks: int = 0, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Causal attention of each request's new tokens over its pages (ffts_paged_attn).
+
+    q [T, H, D]: request r's new tokens are rows ``cu_q[r] .. cu_q[r + 1] - 1``, the last of its ``kv_lens[r]``
+    tokens; ``k_pages`` / ``v_pages`` [pages, Hkv, page_size, D] hold all of them (append first), H % Hkv == 0,
+    H / Hkv <= 128, page_size 16 to 256 (a power of two), D 64 or 128, bf16 or fp16.  ``block_table`` int32
+    [R, width], ``cu_q`` int32 [R + 1], ``kv_lens`` int32 [R] (``plan_pages``); requests may have any number of
+    new tokens, also none.  ``scale`` defaults to D ** -0.5.
+
+    With ``window`` W a token at position p sees the keys p - W + 1 .. p and the first ``sinks`` keys of its
+    request (the work does not grow with the rest); pages it does not see may be gone from the table.  Tokens that see
+    nothing (kv_len 0) get zeros.  Returns [T, H, D] (or fills ``out``); rows of no request are not written.
+
+    A bounded wait that runs out in the kernel raises WaitTimeout at a later call or at ``check_status()``.
+    """
+    dev, dt = q.device, q.dtype
+    if dt not in _DTYPES:
+        raise TypeError(f"paged attention supports bfloat16 and float16, got {dt}")
+    _check_heads("q", q, dt, dev)
+    _check_pool(k_pages, v_pages, dt, dev)
+    T, H, D = q.shape
+    P, Hkv, page_size, Dk = k_pages.shape
+    if Dk != D or Hkv == 0 or H % Hkv:
+        raise ValueError(f"pages {tuple(k_pages.shape)} do not match q {tuple(q.shape)}")
+    if kv_lens.dim() != 1:
+        raise ValueError("kv_lens must be 1-D")
+    R = kv_lens.shape[0]
+    _check_ints("kv_lens", kv_lens, (R,), dev)
+    _check_ints("cu_q", cu_q, (R + 1,), dev)
+    _check_table(block_table, R, dev)
+    if window is None:
+        if sinks:
+            raise ValueError("sinks need a window")
+        window = 0
+    elif window < 1:
+        raise ValueError(f"window must be at least 1, got {window}")
+    if sinks < 0:
+        raise ValueError(f"sinks must not be negative, got {sinks}")
+    if out is not None:
+        _check_heads("out", out, dt, dev)
+        if out.shape != q.shape:
+            raise ValueError(f"out must have q's shape {tuple(q.shape)}, got {tuple(out.shape)}")
+    if P == 0:
+        raise ValueError("the pool has no pages")
+    _check_cuda("q", q)
+    if out is None:
+        out = torch.empty(T, H, D, dtype=dt, device=dev)
+    if T == 0 or R == 0:
+        return out
+    lib = _lib.load()
+    status = device_status(dev)
+    status.poll_direct()
+    nbytes = lib.ffts_paged_workspace_bytes(T, R, H, Hkv, D)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    width = block_table.shape[1]
+    _on_device(dev, lib.ffts_paged_attn, q.data_ptr(), _I64x2(q.stride(0), q.stride(1)), k_pages.data_ptr(),
+               _I64x3(*k_pages.stride()[:3]), v_pages.data_ptr(), _I64x3(*v_pages.stride()[:3]), _DTYPES[dt], T, R, H,
+               Hkv, D, P, page_size, block_table.data_ptr(), block_table.stride(0) if R > 1 else width, width,
+               cu_q.data_ptr(), kv_lens.data_ptr(), D ** -0.5 if scale is None else float(scale), window, sinks,
+               out.data_ptr(), _I64x2(out.stride(0), out.stride(1)), ws.data_ptr(), nbytes, status.direct_ptr)
+    return out

@@ -16,6 +16,10 @@ waits are unbounded), so the codes are this library's own:
   7  QKV projection: the MMA issuer's wait timed out
   8  QKV projection: an epilogue warp's wait timed out
   9  QKV projection: dynamic shared memory was not 1024-byte aligned (nothing ran)
+ 10  paged attention: the TMA producer's wait timed out
+ 11  paged attention: the MMA issuer's wait timed out
+ 12  paged attention: a softmax warp's wait timed out
+ 13  paged attention: dynamic shared memory was not 1024-byte aligned (nothing ran)
 
 A ``StatusWord`` owns one such word.  After each launch that may write it,
 ``read_back`` enqueues an asynchronous copy of the word into pinned host memory
@@ -27,6 +31,11 @@ once; call it (``fftsparse_b200.check_status()``) where the result must be
 known to be good, e.g. at the end of a forward pass.  The word is sticky (a
 kernel only ever sets it), so a read that overtakes an earlier one loses
 nothing; raising clears it.
+
+The paged attention, whose calls are short, stores its code straight into a second,
+pinned host word (``direct_ptr``): no copy and no event follow the kernel, and
+``poll_direct`` is a host read, which a stream that is being captured into a graph
+allows.  ``poll`` and ``check`` look at both words.
 """
 from __future__ import annotations
 
@@ -46,6 +55,10 @@ MESSAGES = {
     7: "QKV projection kernel: the MMA issuer's bounded wait timed out",
     8: "QKV projection kernel: an epilogue warp's bounded wait timed out",
     9: "QKV projection kernel: dynamic shared memory was not 1024-byte aligned (nothing ran)",
+    10: "paged attention kernel: the TMA producer's bounded wait timed out",
+    11: "paged attention kernel: the MMA issuer's bounded wait timed out",
+    12: "paged attention kernel: a softmax warp's bounded wait timed out",
+    13: "paged attention kernel: dynamic shared memory was not 1024-byte aligned (nothing ran)",
 }
 
 
@@ -66,6 +79,15 @@ class StatusWord:
         self._cuda = self.device.type == "cuda"
         self._host = torch.zeros(1, dtype=torch.int32, pin_memory=True) if self._cuda else None
         self._event: Optional[torch.cuda.Event] = None
+        self._direct = torch.zeros(1, dtype=torch.int32, pin_memory=self._cuda)
+        self._direct_view = self._direct.numpy()
+        self.direct_ptr = self._direct.data_ptr()  # the device can write here (unified addressing)
+
+    def poll_direct(self) -> None:
+        """Raise WaitTimeout if a kernel has stored a code into the host word (no CUDA call)."""
+        code = int(self._direct_view[0])
+        if code:
+            self._raise(code)
 
     def read_back(self, stream: Optional[torch.cuda.Stream] = None) -> None:
         """Enqueue the copy of the word to the host after the work already on ``stream``."""
@@ -80,6 +102,7 @@ class StatusWord:
 
     def poll(self) -> None:
         """Raise WaitTimeout if a completed read-back holds a nonzero code (never blocks)."""
+        self.poll_direct()
         if not self._cuda:
             code = int(self.word[0])
         elif self._event is None or not self._event.query():
@@ -93,12 +116,13 @@ class StatusWord:
         """Wait for the device and raise WaitTimeout if the word is nonzero."""
         if self._cuda:
             torch.cuda.synchronize(self.device)
-        code = int(self.word[0].item())
+        code = int(self.word[0].item()) or int(self._direct_view[0])
         if code:
             self._raise(code)
 
     def _raise(self, code: int) -> None:
         self.word.zero_()
+        self._direct_view[0] = 0
         if self._host is not None:
             self._host.zero_()
         self._event = None

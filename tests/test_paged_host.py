@@ -1,0 +1,237 @@
+"""Host side of the paged operators without a GPU: refusals, rotary frequencies and
+the share arithmetic of the paged attention's schedule."""
+import math
+import random
+
+import pytest
+import torch
+
+import fftsparse_b200 as F
+
+
+def ints(*v):
+    return torch.tensor(v, dtype=torch.int32)
+
+
+# ------------------------------------------------------------------ refusals
+def plan_args(**kw):
+    a = dict(cached_lens=ints(3, 4), new_lens=ints(1, 1), block_table=torch.zeros(2, 4, dtype=torch.int32),
+             free_pages=ints(5, 6), page_size=16, num_tokens=2)
+    return dict(a, **kw)
+
+
+@pytest.mark.parametrize("kw,err", [
+    (dict(cached_lens=torch.zeros(2)), TypeError),
+    (dict(cached_lens=torch.zeros(2, 1, dtype=torch.int32)), ValueError),
+    (dict(new_lens=ints(1)), ValueError),
+    (dict(new_lens=torch.ones(2, dtype=torch.int64)), TypeError),
+    (dict(new_lens=ints(1, 2, 3, 4)[::2]), ValueError),
+    (dict(block_table=torch.zeros(3, 4, dtype=torch.int32)), ValueError),
+    (dict(block_table=torch.zeros(4, 2, dtype=torch.int32).t()), ValueError),
+    (dict(block_table=torch.zeros(2, 4)), TypeError),
+    (dict(free_pages=torch.zeros(2, 2, dtype=torch.int32)), ValueError),
+    (dict(num_tokens=-1), ValueError),
+    (dict(), ValueError),  # a good call, on CPU tensors
+])
+def test_plan_refusals(kw, err):
+    with pytest.raises(err):
+        F.plan_pages(**plan_args(**kw))
+
+
+def rope_args(**kw):
+    bf = torch.bfloat16
+    a = dict(q=torch.zeros(3, 4, 64, dtype=bf), k=torch.zeros(3, 2, 64, dtype=bf), v=torch.zeros(3, 2, 64, dtype=bf),
+             positions=ints(0, 1, 2), slot_map=ints(0, 1, 2), k_pages=torch.zeros(2, 2, 16, 64, dtype=bf),
+             v_pages=torch.zeros(2, 2, 16, 64, dtype=bf), inv_freq=torch.ones(32))
+    return dict(a, **kw)
+
+
+@pytest.mark.parametrize("kw,err", [
+    (dict(k=torch.zeros(3, 2, 64)), TypeError),
+    (dict(v=torch.zeros(3, 1, 64, dtype=torch.bfloat16)), ValueError),
+    (dict(v=torch.zeros(3, 2, 64, dtype=torch.float16)), TypeError),
+    (dict(q=torch.zeros(2, 4, 64, dtype=torch.bfloat16)), ValueError),
+    (dict(q=torch.zeros(3, 64, 4, dtype=torch.bfloat16).transpose(1, 2)), ValueError),
+    (dict(positions=ints(0, 1)), ValueError),
+    (dict(slot_map=torch.zeros(3, dtype=torch.int64)), TypeError),
+    (dict(k_pages=torch.zeros(2, 3, 16, 64, dtype=torch.bfloat16)), ValueError),
+    (dict(k_pages=torch.zeros(2, 3, 16, 64, dtype=torch.bfloat16),
+          v_pages=torch.zeros(2, 3, 16, 64, dtype=torch.bfloat16)), ValueError),
+    (dict(inv_freq=torch.ones(32, dtype=torch.float64)), ValueError),
+    (dict(q=None, out=torch.zeros(3, 4, 64, dtype=torch.bfloat16)), ValueError),
+    (dict(out=torch.zeros(3, 2, 64, dtype=torch.bfloat16)), ValueError),
+    (dict(), ValueError),
+])
+def test_rope_append_refusals(kw, err):
+    with pytest.raises(err):
+        F.rope_append(**rope_args(**kw))
+
+
+def attn_args(**kw):
+    bf = torch.bfloat16
+    a = dict(q=torch.zeros(3, 4, 64, dtype=bf), k_pages=torch.zeros(2, 2, 16, 64, dtype=bf),
+             v_pages=torch.zeros(2, 2, 16, 64, dtype=bf), block_table=torch.zeros(2, 1, dtype=torch.int32),
+             cu_q=ints(0, 1, 3), kv_lens=ints(4, 4))
+    return dict(a, **kw)
+
+
+@pytest.mark.parametrize("kw,err", [
+    (dict(q=torch.zeros(3, 4, 64)), TypeError),
+    (dict(q=torch.zeros(3, 3, 64, dtype=torch.bfloat16)), ValueError),
+    (dict(q=torch.zeros(3, 4, 128, dtype=torch.bfloat16)), ValueError),
+    (dict(q=torch.zeros(4, 64, dtype=torch.bfloat16)), ValueError),
+    (dict(cu_q=ints(0, 1)), ValueError),
+    (dict(cu_q=torch.zeros(3, dtype=torch.int64)), TypeError),
+    (dict(kv_lens=ints(4, 4, 4)), ValueError),
+    (dict(block_table=torch.zeros(1, 1, dtype=torch.int32)), ValueError),
+    (dict(window=0), ValueError),
+    (dict(sinks=4), ValueError),
+    (dict(window=8, sinks=-1), ValueError),
+    (dict(out=torch.zeros(3, 4, 128, dtype=torch.bfloat16)), ValueError),
+    (dict(k_pages=torch.zeros(0, 2, 16, 64, dtype=torch.bfloat16),
+          v_pages=torch.zeros(0, 2, 16, 64, dtype=torch.bfloat16)), ValueError),
+    (dict(), ValueError),
+])
+def test_paged_attention_refusals(kw, err):
+    with pytest.raises(err):
+        F.paged_attention(**attn_args(**kw))
+
+
+# ------------------------------------------------------------------ rotary frequencies
+def test_rotary_frequencies_of_each_scaling():
+    d, base, L0 = 64, 10000.0, 4096
+    f = [base ** (-2 * i / d) for i in range(d // 2)]
+
+    def got(scaling, **kw):
+        return F.rotary_inv_freq(d, base, scaling, **kw)
+
+    def near(t, want):  # fp32: half a step
+        w = torch.tensor(want, dtype=torch.float64)
+        return bool(((t.double() - w).abs() <= torch.finfo(torch.float32).eps / 2 * w * 1.001).all())
+
+    t, a = got(None)
+    assert t.dtype == torch.float32 and a == 1.0 and near(t, f)
+    t, a = got({"rope_type": "linear", "factor": 4.0})
+    assert a == 1.0 and near(t, [x / 4 for x in f])
+    dyn = {"type": "dynamic", "factor": 2.0, "original_max_position_embeddings": L0}
+    assert near(got(dyn, seq_len=100)[0], f)
+    grown = base * (2.0 * 16384 / L0 - 1.0) ** (d / (d - 2))
+    assert near(got(dyn, seq_len=16384)[0], [grown ** (-2 * i / d) for i in range(d // 2)])
+
+    t, _ = got({"rope_type": "llama3", "factor": 8.0, "low_freq_factor": 1.0, "high_freq_factor": 4.0,
+                "original_max_position_embeddings": L0})
+    want = []
+    for x in f:
+        wl = 2 * math.pi / x
+        if wl > L0 / 1.0:
+            want.append(x / 8)
+        elif wl < L0 / 4.0:
+            want.append(x)
+        else:
+            s = (L0 / wl - 1.0) / 3.0
+            want.append((1 - s) * x / 8 + s * x)
+    assert near(t, want)
+
+    t, a = got({"rope_type": "yarn", "factor": 4.0, "original_max_position_embeddings": L0})
+    lo = math.floor(d * math.log(L0 / (32 * 2 * math.pi)) / (2 * math.log(base)))
+    hi = math.ceil(d * math.log(L0 / (1 * 2 * math.pi)) / (2 * math.log(base)))
+    want = []
+    for i, x in enumerate(f):
+        ramp = min(1.0, max(0.0, (i - lo) / (hi - lo)))
+        want.append(x / 4 * ramp + x * (1 - ramp))
+    assert near(t, want) and abs(a - (0.1 * math.log(4.0) + 1.0)) < 1e-12
+
+
+@pytest.mark.parametrize("args", [(0, 1e4, None), (15, 1e4, None), (64, 1e4, {"rope_type": "bogus"}),
+                                  (64, 1e4, {"rope_type": "linear"}), (2, 1e4, {"rope_type": "dynamic"})])
+def test_rotary_frequency_refusals(args):
+    with pytest.raises(ValueError):
+        F.rotary_inv_freq(*args)
+
+
+# ------------------------------------------------------------------ schedule
+BM, BN, MIN_UNITS = 128, 64, 4
+
+
+def keys_of(pos0, ntok, window, sinks):
+    hi = max(0, pos0 + ntok)
+    lo = max(0, pos0 - window + 1) if window else 0
+    nt, wt0 = -(-hi // BN), lo // BN
+    st = min(-(-min(sinks, hi) // BN), wt0)
+    return hi, lo, st, wt0, max(1, st + nt - wt0)
+
+
+@pytest.mark.parametrize("seed", range(40))
+def test_shares_cover_every_unit_once_and_the_merge_finds_its_partials(seed):
+    """The (q tile, head, key tile) units are cut into shares as the kernel cuts them; every key that a
+    row sees lies in exactly one visited tile, every slot is written once, and the merge of each cut
+    (q tile, head) reads just the slots its shares wrote."""
+    rng = random.Random(seed)
+    G = rng.choice([1, 2, 4, 7, 8, 16, 128])
+    Hkv, ctas = rng.choice([1, 2, 8]), rng.choice([1, 3, 8, 296])
+    window = rng.choice([0, 0, 1, 50, 700])
+    sinks = rng.choice([0, 4, 130]) if window else 0
+    tpt = BM // G
+    tiles, cum = [], [0]
+    for _ in range(rng.randrange(1, 12)):
+        n = rng.choice([0, 1, 1, rng.randrange(1, 300)])
+        kv = rng.choice([0, n, n + rng.randrange(0, 3000), rng.randrange(0, n + 1)])
+        for i in range(0, n, tpt):
+            t = (kv - n + i, min(tpt, n - i))
+            g = keys_of(*t, window, sinks)
+            tiles.append((t, g))
+            cum.append(cum[-1] + g[4])
+            visited = [j if j < g[2] else j - g[2] + g[3] for j in range(g[4])]
+            assert len(set(visited)) == len(visited)
+            for pos in range(max(0, t[0]), t[0] + t[1]):
+                seen = [c for c in range(pos + 1) if not window or c > pos - window or c < sinks]
+                assert {c // BN for c in seen} <= set(visited)
+                assert all(c < g[0] and (c >= g[1] or c < sinks) for c in seen)
+    units = cum[-1] * Hkv
+    per = max(MIN_UNITS, -(-units // ctas))
+    covered, wrote, whole = {}, {}, set()
+    for c in range(ctas):
+        u, u1, first = per * c, min(units, per * (c + 1)), True
+        while u < u1:
+            x = max(i for i in range(len(tiles)) if cum[i] * Hkv <= u)
+            n = tiles[x][1][4]
+            h, j0 = divmod(u - cum[x] * Hkv, n)
+            j1 = min(n, j0 + u1 - u)
+            for j in range(j0, j1):
+                assert (x, h, j) not in covered
+                covered[x, h, j] = c
+            if (j0, j1) == (0, n):
+                whole.add((x, h))
+            else:
+                slot = 2 * c + (0 if first else 1)
+                assert slot not in wrote
+                wrote[slot] = (x, h)
+            u, first = u + j1 - j0, False
+    assert len(covered) == units
+    merged = {}
+    for c in range(1, ctas):
+        u = per * c
+        if u >= units:
+            continue
+        x = max(i for i in range(len(tiles)) if cum[i] * Hkv <= u)
+        n = tiles[x][1][4]
+        h, j0 = divmod(u - cum[x] * Hkv, n)
+        begin = u - j0
+        if j0 == 0 or begin // per != c - 1:
+            continue
+        assert (x, h) not in merged
+        merged[x, h] = [2 * (c - 1) + (0 if begin % per == 0 else 1)] + \
+            [2 * s for s in range(c, (begin + n - 1) // per + 1)]
+    for (x, h), slots in merged.items():
+        assert slots == sorted(s for s, at in wrote.items() if at == (x, h))
+    assert whole | set(merged) == {(x, h) for x in range(len(tiles)) for h in range(Hkv)}
+    assert not whole & set(merged)
+
+
+def test_workspace_query_needs_no_gpu():
+    from fftsparse_b200 import _lib
+    lib = _lib.load()
+    small, large = (lib.ffts_paged_workspace_bytes(t, 4, 32, 8, 128) for t in (4, 100000))
+    assert 0 < small < large
+    assert lib.ffts_paged_workspace_bytes(0, 4, 32, 8, 128) == 0
+    assert lib.ffts_paged_workspace_bytes(4, 4, 30, 8, 128) == 0

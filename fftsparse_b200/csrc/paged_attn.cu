@@ -8,13 +8,15 @@
 // Work.  The G = H / Hkv query heads of a KV head share one 128-row tile with as many tokens as fit
 // (128 / G, row = token * G + head), so a key tile is loaded once for all of them.  A q tile visits the
 // 64-key tiles that any of its rows can see (the sinks' tiles, then the window's), in order.  All (q tile, KV
-// head, key tile) triples form one line of W units, cut into equal shares: CTA c of the persistent grid
-// takes units [c * per, (c + 1) * per).  A share that begins or ends inside a (q tile, head) leaves fp32
-// partial sums that merge_kernel joins.  So one decode request and a batch of ragged chunks alike load
-// every SM equally, and nothing about the lengths is needed on the host.
-//   schedule_kernel  one CTA: q tiles of every request and the running sum of their key tiles
+// head)s form one line, each as long as its key tiles plus kOverhead for loading Q and storing the result, and
+// the line is cut into equal shares: CTA c of the persistent grid takes [c * per, (c + 1) * per).  So one
+// decode request and a batch of ragged chunks alike load every SM equally, and nothing about the lengths is
+// needed on the host.  A share that begins or ends between two key tiles of a (q tile, head) leaves fp32
+// partial sums, which are joined in the order of the shares.
+//   schedule_kernel  one CTA: q tiles of every request and the running sum of their lengths
 //   attn_kernel      two CTAs per SM, each walking its share
-//   merge_kernel     joins the (q tile, head)s that several shares cut
+//   join_kernel      the (q tile, head)s that several shares cut (a kernel of its own: inside attn_kernel
+//                    its registers made the softmax loop spill, 1.15 -> 1.89 ms at 2048 tokens over 32768)
 //
 // attn_kernel's roles (192 threads):
 //   warp 4      producer: page numbers one tile ahead, Q per segment, K tiles into a three-stage ring, V
@@ -50,7 +52,8 @@ constexpr int kKStages = 3, kVStages = 2;
 constexpr int kTmemCols = 256;  // S0, S1 (64 columns each), O (D): two CTAs fill an SM's 512
 constexpr uint32_t kTmemO = 128;
 constexpr int kMaxCtas = 512;   // partial slots in the workspace (two per CTA)
-constexpr int kMinUnits = 4;    // key tiles per share, at least
+constexpr int kMinShare = 4;    // length of a share, at least
+constexpr int kOverhead = 2;    // length of a (q tile, head) besides its key tiles
 constexpr double kWaitSeconds = 2.0, kDrainSeconds = 4.0;
 
 constexpr int kErrProducer = 10, kErrMma = 11, kErrSoftmax = 12, kErrSmemAlign = 13;
@@ -88,6 +91,12 @@ struct Tile {
   int tok0, pos0, ntok, r;
 };
 
+// A (q tile, head) that several shares cut: rows nrows from token tok0 and head head0 on; its partials lie in
+// first_slot and in the first slots of the shares behind it up to s1.  nrows 0: none.
+struct Cut {
+  int tok0, nrows, head0, s1, first_slot;
+};
+
 struct Params {
   int T, R, H, Hkv, G, tpt;   // tpt: tokens per q tile
   const int32_t *table;       // [R, width]
@@ -99,10 +108,11 @@ struct Params {
   int64_t os_t, os_h;
   float scale_log2;
   Tile *tiles;                // [max_tiles]
-  long long *cum;             // [max_tiles + 1]: key tiles (of one head) before q tile x
+  long long *cum;             // [max_tiles + 1]: length (of one head) before q tile x
   int *header;                // [0]: q tiles
-  float *part;                // [2 * ctas][128][D], then m, l: [2 * ctas][128] float2
-  float2 *part_ml;
+  Cut *cuts;                  // [ctas]: the (q tile, head) that share c begins and others go on with
+  float *part;                // [2 * ctas][D / 4][128 rows] float4
+  float2 *part_ml;            // [2 * ctas][128 rows]: m (log2 units) and l
   int max_tiles, ctas;
   int *status;
   long long wait_cycles, drain_cycles;
@@ -127,9 +137,9 @@ __device__ __forceinline__ Keys keys_of(int pos0, int ntok, int window, int sink
 
 __device__ __forceinline__ int key_tile(const Keys &g, int j) { return j < g.st ? j : j - g.st + g.wt0; }
 
-__device__ __forceinline__ long long share_of(const Params &p, long long units) {
-  const long long per = (units + p.ctas - 1) / p.ctas;
-  return per < kMinUnits ? kMinUnits : per;
+__device__ __forceinline__ long long share_of(const Params &p, long long length) {
+  const long long per = (length + p.ctas - 1) / p.ctas;
+  return per < kMinShare ? kMinShare : per;
 }
 
 // ---------------------------------------------------------------- schedule
@@ -164,6 +174,7 @@ __global__ void __launch_bounds__(kSchedThreads) schedule_kernel(const __grid_co
   const long long cap = (long long)p.width << p.ps_shift;  // keys a table row can hold
   long long tile_base = 0, unit_base = 0;
   if (tid == 0) p.cum[0] = 0;
+  if (tid < p.ctas) p.cuts[tid].nrows = 0;
   for (int r0 = 0; r0 < p.R; r0 += kSchedThreads) {
     const int nr = min(kSchedThreads, p.R - r0);
     int q0 = 0, len = 0, kv = 0;
@@ -196,7 +207,7 @@ __global__ void __launch_bounds__(kSchedThreads) schedule_kernel(const __grid_co
         t.pos0 = s_kv[lo] - s_len[lo] + i;
         t.ntok = min(p.tpt, s_len[lo] - i);
         t.r = r0 + lo;
-        n = keys_of(t.pos0, t.ntok, p.window, p.sinks).n;
+        n = keys_of(t.pos0, t.ntok, p.window, p.sinks).n + kOverhead;
         if (FFTS_IN_RANGE(tile_base + x, p.max_tiles)) p.tiles[tile_base + x] = t;
       }
       long long units;
@@ -210,18 +221,19 @@ __global__ void __launch_bounds__(kSchedThreads) schedule_kernel(const __grid_co
   if (tid == 0) p.header[0] = int(tile_base);
 }
 
-// Walks the (q tile, head, key tile) units [u, u1) segment by segment; the same in every lane.
+// Walks the share [u, u1) of the line segment by segment; the same in every lane.
 struct Walk {
   const Params &p;
   long long u, u1;
-  long long base, next;  // units before q tile x and behind it, all heads
+  long long base, next;  // the line before q tile x and behind it, all heads
   int x;
   Tile t;
   Keys g;
-  int h, j0, j1;  // the segment: head and key tiles [j0, j1) of the g.n
+  int h, j0, j1;         // the segment: head and key tiles [j0, j1) of the g.n
+  long long begin;       // where its (q tile, head) begins
   __device__ __forceinline__ Walk(const Params &prm) : p(prm) {}
 
-  // Finds the q tile of unit u0 (whole warp; u0 < units).
+  // Finds the q tile at u0 (whole warp; u0 < length).
   __device__ __forceinline__ void seek(long long u0, long long end, int ntiles) {
     u = u0;
     u1 = end;
@@ -245,19 +257,25 @@ struct Walk {
     next = p.cum[x + 1] * p.Hkv;
     g = keys_of(t.pos0, t.ntok, p.window, p.sinks);
   }
-  // The segment at u; false behind the share's end.
+  // The next segment with key tiles; false behind the share's end.
   __device__ __forceinline__ bool segment() {
-    if (u >= u1) return false;
-    if (u >= next) {
-      ++x;
-      load();
+    while (u < u1) {
+      if (u >= next) {
+        ++x;
+        load();
+      }
+      const int len = g.n + kOverhead;
+      const long long rem = u - base;
+      h = int(rem / len);
+      const int at = int(rem - (long long)h * len);
+      const int to = int(min((long long)len, at + (u1 - u)));
+      begin = u - at;
+      u += to - at;
+      j0 = max(0, at - kOverhead);
+      j1 = max(0, to - kOverhead);
+      if (j1 > j0) return true;
     }
-    const long long rem = u - base;
-    h = int(rem / g.n);
-    j0 = int(rem - (long long)h * g.n);
-    j1 = int(min((long long)g.n, j0 + (u1 - u)));
-    u += j1 - j0;
-    return true;
+    return false;
   }
 };
 
@@ -313,9 +331,9 @@ __global__ void __launch_bounds__(kThreads, 2)
     return;
   }
   const int ntiles = p.header[0];
-  const long long units = p.cum[FFTS_INDEX(ntiles, p.max_tiles + 1)] * p.Hkv;
-  const long long per = share_of(p, units);
-  const long long u0 = per * blockIdx.x, u1 = min(units, u0 + per);
+  const long long length = p.cum[FFTS_INDEX(ntiles, p.max_tiles + 1)] * p.Hkv;
+  const long long per = share_of(p, length);
+  const long long u0 = per * blockIdx.x, u1 = min(length, u0 + per);
   if (u0 >= u1) return;  // uniform in the CTA, before any allocation
   const uint32_t sbase = smem_u32(smem);
   auto bar = [&](int i) { return sbase + Lay::bars + 8u * uint32_t(i); };
@@ -350,7 +368,6 @@ __global__ void __launch_bounds__(kThreads, 2)
   fence_after();
   const uint32_t tmem = *tmem_slot;
   const uint32_t tm_o = tmem + kTmemO;
-  const int total = int(min(u1 - u0, (long long)0x7fffffff));
 
   Walk w(p);
   w.seek(u0, u1, ntiles);
@@ -366,27 +383,23 @@ __global__ void __launch_bounds__(kThreads, 2)
     struct Load {
       int page, row, h;
     };
-    int seg = -1, j = 0, j1 = 0;
+    int j = 0, j1 = 0;
     bool fresh = false;  // the fetched tile is its segment's first
-    auto fetch = [&]() -> Load {
-      if (j >= j1) {
-        w.segment();
+    auto fetch = [&](Load &l) -> bool {
+      fresh = j >= j1;
+      if (fresh) {
+        if (!w.segment()) return false;
         j = w.j0;
         j1 = w.j1;
-        ++seg;
-        fresh = true;
-      } else {
-        fresh = false;
       }
       const int c = key_tile(w.g, j) * kBN + my_box * box;  // first key of the box
       ++j;
-      Load l;
       l.page = -1;
       l.row = c & (ps - 1);
       l.h = w.h;
       if (lane < boxes && c < w.g.hi && (c + box > w.g.lo || c < p.sinks))
         l.page = p.table[int64_t(w.t.r) * p.table_ld + FFTS_INDEX(c >> p.ps_shift, p.width)];
-      return l;
+      return true;
     };
     bool ok = true;
     int nk = 0, nv = 0, nq = 0;  // loads issued
@@ -402,13 +415,13 @@ __global__ void __launch_bounds__(kThreads, 2)
       if (lane < boxes) tma_load_4d(dst, is_k ? &tm_k : &tm_v, bar(full), my_half * 64, l.row, l.h, l.page);
       if (is_k) ++nk; else ++nv;
     };
-    Load cur = fetch(), prev = cur;
-    for (int n = 0; n < total && ok; ++n) {
+    Load cur{}, prev{};
+    bool more = fetch(cur);
+    while (more && ok) {
       const bool cur_fresh = fresh;
       const int tok0 = w.t.tok0, qh = w.h * p.G;
-      Load next = cur;
       // K(n), V(n - 1); a new segment's Q waits for the last S of the one before, so V(n - 1) goes first
-      if (cur_fresh && n > 0) load(prev, false);
+      if (cur_fresh && nk > 0) load(prev, false);
       load(cur, true);
       if (cur_fresh && ok) {
         ok = __all_sync(0xffffffffu, mbar_wait(bar(BQE), (nq & 1) ^ 1, abort_flag, p.wait_cycles));
@@ -419,12 +432,13 @@ __global__ void __launch_bounds__(kThreads, 2)
         }
         if (ok) ++nq;
       }
-      if (n + 1 < total) next = fetch();  // its page numbers arrive while the stages fill
-      if (!cur_fresh && n > 0) load(prev, false);
+      Load next = cur;
+      more = fetch(next);  // its page numbers arrive while the stages fill
+      if (!cur_fresh && nk > 1) load(prev, false);
       prev = cur;
       cur = next;
     }
-    if (ok) load(prev, false);
+    if (ok && nk > 0) load(prev, false);
     if (!ok) {
       if (lane == 0) {
         *abort_flag = 1;
@@ -451,15 +465,15 @@ __global__ void __launch_bounds__(kThreads, 2)
       // needs only to know which tiles begin a segment (bit n % 32 of firsts).
       int s = 0, seg = 0, s_left = 0;
       uint32_t firsts = 0;
-      for (int n = 0; n < total && ok; ++n) {
-        while (s < total && s < n + 2) {
+      bool more = w.segment();
+      for (int n = 0; ok && (more || n < s); ++n) {
+        while (more && s < n + 2) {
           const bool first = s_left == 0;
           if (first) {
             // a new segment's Q is not there yet: PV tiles that are due go first
             if (s > n && !mbar_try(bar(BQF), seg & 1)) break;
             ok = mbar_wait(bar(BQF), seg & 1, abort_flag, p.wait_cycles);
             if (!ok) break;
-            w.segment();
             s_left = w.j1 - w.j0;
             ++seg;
           }
@@ -477,7 +491,10 @@ __global__ void __launch_bounds__(kThreads, 2)
           }
           umma_commit(bar(BSF + (s & 1)));
           umma_commit(bar(BKE + ks));
-          if (--s_left == 0) umma_commit(bar(BQE));
+          if (--s_left == 0) {
+            umma_commit(bar(BQE));
+            more = w.segment();
+          }
           firsts = (firsts & ~(1u << (s & 31))) | (uint32_t(first) << (s & 31));
           ++s;
         }
@@ -650,7 +667,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         const int slot = 2 * int(blockIdx.x) + (first_seg ? 0 : 1);
         const float inv_l = l_run > 0.0f ? 1.0f / l_run : 0.0f;
         uint16_t *dst = p.out + int64_t(w.t.tok0 + tl) * p.os_t + int64_t(w.h * p.G + hg) * p.os_h;
-        float *pd = p.part + (int64_t(slot) * kBM + r) * D;
+        float4 *pd = reinterpret_cast<float4 *>(p.part) + int64_t(slot) * (kBM * D / 4) + r;
 #pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {
           float o[32];
@@ -671,12 +688,21 @@ __global__ void __launch_bounds__(kThreads, 2)
           } else if (FFTS_IN_RANGE(slot, 2 * p.ctas)) {
 #pragma unroll
             for (int q = 0; q < 8; ++q)
-              *reinterpret_cast<float4 *>(pd + c * 32 + q * 4) =
-                  make_float4(o[q * 4], o[q * 4 + 1], o[q * 4 + 2], o[q * 4 + 3]);
+              pd[(c * 8 + q) * kBM] = make_float4(o[q * 4], o[q * 4 + 1], o[q * 4 + 2], o[q * 4 + 3]);
           }
         }
         if (live && !whole && FFTS_IN_RANGE(slot, 2 * p.ctas))
           p.part_ml[int64_t(slot) * kBM + r] = make_float2(m_ref * p.scale_log2, l_run);
+      }
+      // the share that holds the first key tile leaves a note for the join
+      if (w.j0 == 0 && w.j1 < g.n && r == 0 && FFTS_IN_RANGE(blockIdx.x, p.ctas)) {
+        Cut cut;
+        cut.tok0 = w.t.tok0;
+        cut.nrows = nrows;
+        cut.head0 = w.h * p.G;
+        cut.s1 = int((w.begin + kOverhead + g.n - 1) / per);
+        cut.first_slot = 2 * int(blockIdx.x) + (first_seg ? 0 : 1);
+        p.cuts[blockIdx.x] = cut;
       }
       first_seg = false;
     }
@@ -692,70 +718,98 @@ __global__ void __launch_bounds__(kThreads, 2)
   if (warp == 5) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
 }
 
-// ---------------------------------------------------------------- merge
-constexpr int kMergeWarps = 4;
-
-// Block (c, y): the (q tile, head) that share c - 1 begins and share c goes on with, rows y * 4 + warp of
-// every gridDim.y * 4.  Its partials are share c - 1's last segment and the first ones of c, c + 1, ...
-template <typename E, int D>
-__global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const __grid_constant__ Params p) {
-  const int ntiles = p.header[0];
-  const long long units = p.cum[FFTS_INDEX(ntiles, p.max_tiles + 1)] * p.Hkv;
-  const long long per = share_of(p, units);
-  const int c = int(blockIdx.x) + 1;
-  const long long u = per * c;
-  if (u >= units) return;
-  Walk w(p);
-  w.seek(u, u + 1, ntiles);
-  w.segment();
-  if (w.j0 == 0) return;  // the cut lies between two
-  const long long begin = u - w.j0, end = begin + w.g.n;
-  if (begin / per != c - 1) return;  // an earlier block's
-  const int last = int((end - 1) / per);
-  const int first_slot = 2 * (c - 1) + (begin % per == 0 ? 0 : 1);
-  const int lane = threadIdx.x & 31;
-  const int nrows = w.t.ntok * p.G;
-  constexpr int kC = D / 32;  // channels per lane
-  for (int r = int(blockIdx.y) * kMergeWarps + (threadIdx.x >> 5); r < nrows; r += int(gridDim.y) * kMergeWarps) {
-    float m = -INFINITY;
-    for (int s = c - 1 + lane; s <= last; s += 32) {
-      const int slot = s == c - 1 ? first_slot : 2 * s;
-      m = fmaxf(m, p.part_ml[int64_t(FFTS_INDEX(slot, 2 * p.ctas)) * kBM + r].x);
-    }
+// ---------------------------------------------------------------- join
+// For each row o = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s over the shares s, with M taken along as they
+// are read.  A partial is stored 16-byte piece by piece over the rows ([D / 4][128 rows]), so rows that lie
+// side by side in a warp are read and written whole.  A thread has one row and the pieces c0, c0 + step, ...; PB shares x
+// CB pieces are in flight at a time, since the time is that of the rounds through L2.
+template <typename E, int D, int PB, int CB>
+__device__ __forceinline__ void join_rows(const Params &p, uint16_t *dst, int r, int q, int step, int s0,
+                                          int s1, int first_slot) {
+  auto slot = [&](int s) { return int64_t(FFTS_INDEX(s == s0 ? first_slot : 2 * s, 2 * p.ctas)); };
+  for (int c0 = q; c0 < D / 4; c0 += CB * step) {
+    float4 acc[CB];
 #pragma unroll
-    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    float acc[kC], l = 0.0f;
+    for (int i = 0; i < CB; ++i) acc[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float m = -INFINITY, l = 0.0f;
+    for (int sb = s0; sb <= s1; sb += PB) {
+      float2 ml[PB];
+      float4 v[PB][CB];
 #pragma unroll
-    for (int i = 0; i < kC; ++i) acc[i] = 0.0f;
-#pragma unroll 4
-    for (int s = c - 1; s <= last; ++s) {
-      const int slot = FFTS_INDEX(s == c - 1 ? first_slot : 2 * s, 2 * p.ctas);
-      const float2 ml = p.part_ml[int64_t(slot) * kBM + r];
-      const float *src = p.part + (int64_t(slot) * kBM + r) * D + lane * kC;
-      float v[kC];
-      if (kC == 4) {
-        const float4 q = *reinterpret_cast<const float4 *>(src);
-        v[0] = q.x; v[1] = q.y; v[kC - 2] = q.z; v[kC - 1] = q.w;
-      } else {
-        const float2 q = *reinterpret_cast<const float2 *>(src);
-        v[0] = q.x; v[1] = q.y;
+      for (int k = 0; k < PB; ++k) {
+        ml[k] = make_float2(-INFINITY, 0.0f);
+        if (sb + k <= s1) {
+          const int64_t at = slot(sb + k);
+          ml[k] = __ldcg(&p.part_ml[at * kBM + r]);
+          const float4 *src = reinterpret_cast<const float4 *>(p.part) + at * (kBM * D / 4) + r;
+#pragma unroll
+          for (int i = 0; i < CB; ++i)
+            if (c0 + i * step < D / 4) v[k][i] = __ldcg(src + (c0 + i * step) * kBM);
+        }
       }
-      // a share whose keys the row does not see has l = 0 and m = -inf: nothing of it counts
-      const float f = ml.x == -INFINITY ? 0.0f : exp2f(ml.x - m);
-      l = fmaf(f, ml.y, l);
+      float top = m;
 #pragma unroll
-      for (int i = 0; i < kC; ++i) acc[i] = fmaf(f, f > 0.0f ? v[i] : 0.0f, acc[i]);
+      for (int k = 0; k < PB; ++k) top = fmaxf(top, ml[k].x);
+      const float old = m == -INFINITY ? 0.0f : exp2f(m - top);
+      m = top;
+      l *= old;
+#pragma unroll
+      for (int i = 0; i < CB; ++i) {
+        acc[i].x *= old;
+        acc[i].y *= old;
+        acc[i].z *= old;
+        acc[i].w *= old;
+      }
+#pragma unroll
+      for (int k = 0; k < PB; ++k) {
+        if (ml[k].x == -INFINITY) continue;  // no share, or one whose keys the row does not see: o = 0, l = 0
+        const float f = exp2f(ml[k].x - top);
+        l = fmaf(f, ml[k].y, l);
+#pragma unroll
+        for (int i = 0; i < CB; ++i)
+          if (c0 + i * step < D / 4) {
+            acc[i].x = fmaf(f, v[k][i].x, acc[i].x);
+            acc[i].y = fmaf(f, v[k][i].y, acc[i].y);
+            acc[i].z = fmaf(f, v[k][i].z, acc[i].z);
+            acc[i].w = fmaf(f, v[k][i].w, acc[i].w);
+          }
+      }
     }
     const float inv_l = l > 0.0f ? 1.0f / l : 0.0f;
-    const int tl = r / p.G, hg = r - tl * p.G;
-    uint16_t *dst = p.out + int64_t(w.t.tok0 + tl) * p.os_t + int64_t(w.h * p.G + hg) * p.os_h + lane * kC;
-    if (FFTS_IN_RANGE(w.t.tok0 + tl, p.T)) {
 #pragma unroll
-      for (int i = 0; i < kC; i += 2)
-        *reinterpret_cast<uint32_t *>(dst + i) = Num<E>::pack(l > 0.0f ? acc[i] * inv_l : 0.0f,
-                                                              l > 0.0f ? acc[i + 1] * inv_l : 0.0f);
-    }
+    for (int i = 0; i < CB; ++i)
+      if (c0 + i * step < D / 4) {
+        uint2 o = make_uint2(0u, 0u);
+        if (l > 0.0f)
+          o = make_uint2(Num<E>::pack(acc[i].x * inv_l, acc[i].y * inv_l), Num<E>::pack(acc[i].z * inv_l, acc[i].w * inv_l));
+        *reinterpret_cast<uint2 *>(dst + (c0 + i * step) * 4) = o;
+      }
   }
+}
+
+// Block (s0, y): the (q tile, head) that share s0 begins; the pieces of a row go round the blocks of y and
+// the threads that its rows leave.
+constexpr int kJoinThreads = 128;
+constexpr int kJoinBlocks = 4;
+
+template <typename E, int D>
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ Params p) {
+  const int s0 = int(blockIdx.x);
+  const Cut cut = p.cuts[s0];
+  if (cut.nrows == 0) return;
+  int rows = 1;
+  while (rows < cut.nrows) rows <<= 1;
+  const int r = int(threadIdx.x) % rows, per_block = kJoinThreads / rows;
+  const int q = int(blockIdx.y) * per_block + int(threadIdx.x) / rows, step = kJoinBlocks * per_block;
+  if (r >= cut.nrows || q >= D / 4) return;
+  const int tl = r / p.G, hg = r - tl * p.G;
+  if (!FFTS_IN_RANGE(cut.tok0 + tl, p.T)) return;
+  uint16_t *dst = p.out + int64_t(cut.tok0 + tl) * p.os_t + int64_t(cut.head0 + hg) * p.os_h;
+  // few rows: one or two pieces per thread and often many shares; many rows: the other way round
+  if (rows <= 16)
+    join_rows<E, D, 8, 1>(p, dst, r, q, step, s0, cut.s1, cut.first_slot);
+  else
+    join_rows<E, D, 2, 4>(p, dst, r, q, step, s0, cut.s1, cut.first_slot);
 }
 
 // ---------------------------------------------------------------- host side
@@ -791,16 +845,17 @@ static int encode(CUtensorMap *map, CUtensorMapDataType type, int rank, const vo
 
 __device__ int g_status_sink;
 
-// Workspace: cum, tiles, header, partial (m, l), partial O; every part a multiple of 16 bytes.
+// Workspace: cum, tiles, header, cuts, partial (m, l), partial O; every part a multiple of 16 bytes.
 struct Space {
-  int64_t max_tiles, cum, tiles, header, ml, part, bytes;
+  int64_t max_tiles, cum, tiles, header, cuts, ml, part, bytes;
   Space(int64_t T, int64_t R, int64_t G, int64_t D) {
     const int64_t tpt = kBM / G;
     max_tiles = T / tpt + std::min(R, T);  // sum of ceil(len / tpt)
     cum = 0;
     tiles = cum + (max_tiles + 2) / 2 * 16;
     header = tiles + max_tiles * 16;
-    ml = header + 16;
+    cuts = header + 16;
+    ml = cuts + kMaxCtas * int64_t(sizeof(Cut));
     part = ml + int64_t(2 * kMaxCtas) * kBM * 8;
     bytes = part + int64_t(2 * kMaxCtas) * kBM * D * 4;
   }
@@ -830,12 +885,8 @@ static int launch(const Params &p, const void *q, const int64_t *qs, const void 
   FFTS_CUDA(cudaGetLastError());
   attn_kernel<E, D><<<unsigned(p.ctas), kThreads, Layout<D>::bytes, stream>>>(mq, mk, mv, p);
   FFTS_CUDA(cudaGetLastError());
-  if (p.ctas > 1) {
-    // rows of the largest tile, in 8 blocks
-    const dim3 grid(unsigned(p.ctas - 1), unsigned(std::min<int64_t>(8, ceil_div(int64_t(p.tpt) * p.G, kMergeWarps))));
-    merge_kernel<E, D><<<grid, kMergeWarps * 32, 0, stream>>>(p);
-    FFTS_CUDA(cudaGetLastError());
-  }
+  join_kernel<E, D><<<dim3(unsigned(p.ctas), kJoinBlocks), kJoinThreads, 0, stream>>>(p);
+  FFTS_CUDA(cudaGetLastError());
   return FFTS_OK;
 }
 
@@ -901,6 +952,7 @@ int paged_attn(const void *q, const int64_t *qs, const void *k_pages, const int6
   p.cum = reinterpret_cast<long long *>(base + sp.cum);
   p.tiles = reinterpret_cast<Tile *>(base + sp.tiles);
   p.header = reinterpret_cast<int *>(base + sp.header);
+  p.cuts = reinterpret_cast<Cut *>(base + sp.cuts);
   p.part_ml = reinterpret_cast<float2 *>(base + sp.ml);
   p.part = reinterpret_cast<float *>(base + sp.part);
   int sms = 0;

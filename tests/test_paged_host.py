@@ -150,7 +150,7 @@ def test_rotary_frequency_refusals(args):
 
 
 # ------------------------------------------------------------------ schedule
-BM, BN, MIN_UNITS = 128, 64, 4
+BM, BN, MIN_SHARE, OVERHEAD = 128, 64, 4, 2
 
 
 def keys_of(pos0, ntok, window, sinks):
@@ -162,70 +162,69 @@ def keys_of(pos0, ntok, window, sinks):
 
 
 @pytest.mark.parametrize("seed", range(40))
-def test_shares_cover_every_unit_once_and_the_merge_finds_its_partials(seed):
-    """The (q tile, head, key tile) units are cut into shares as the kernel cuts them; every key that a
-    row sees lies in exactly one visited tile, every slot is written once, and the merge of each cut
-    (q tile, head) reads just the slots its shares wrote."""
+def test_shares_cover_every_key_tile_once_and_the_join_finds_its_partials(seed):
+    """The line of (q tile, head)s is cut into shares as the kernel cuts it; every key that a row sees lies
+    in exactly one visited tile, every slot is written once, and the join of each cut (q tile, head)
+    waits for the shares that hold parts of it and reads just the slots they wrote."""
     rng = random.Random(seed)
     G = rng.choice([1, 2, 4, 7, 8, 16, 128])
     Hkv, ctas = rng.choice([1, 2, 8]), rng.choice([1, 3, 8, 296])
     window = rng.choice([0, 0, 1, 50, 700])
     sinks = rng.choice([0, 4, 130]) if window else 0
     tpt = BM // G
-    tiles, cum = [], [0]
+    line, at = [], 0  # (begin, x, head, key tiles)
+    x = 0
     for _ in range(rng.randrange(1, 12)):
         n = rng.choice([0, 1, 1, rng.randrange(1, 300)])
         kv = rng.choice([0, n, n + rng.randrange(0, 3000), rng.randrange(0, n + 1)])
         for i in range(0, n, tpt):
             t = (kv - n + i, min(tpt, n - i))
             g = keys_of(*t, window, sinks)
-            tiles.append((t, g))
-            cum.append(cum[-1] + g[4])
             visited = [j if j < g[2] else j - g[2] + g[3] for j in range(g[4])]
             assert len(set(visited)) == len(visited)
             for pos in range(max(0, t[0]), t[0] + t[1]):
                 seen = [c for c in range(pos + 1) if not window or c > pos - window or c < sinks]
                 assert {c // BN for c in seen} <= set(visited)
                 assert all(c < g[0] and (c >= g[1] or c < sinks) for c in seen)
-    units = cum[-1] * Hkv
-    per = max(MIN_UNITS, -(-units // ctas))
-    covered, wrote, whole = {}, {}, set()
+            for h in range(Hkv):
+                line.append((at, x, h, g[4]))
+                at += g[4] + OVERHEAD
+            x += 1
+    length = at
+    per = max(MIN_SHARE, -(-length // ctas))
+    assert per * ctas >= length
+    covered, wrote, arrived, whole = set(), {}, {}, set()
     for c in range(ctas):
-        u, u1, first = per * c, min(units, per * (c + 1)), True
+        u, u1, first = per * c, min(length, per * (c + 1)), True
         while u < u1:
-            x = max(i for i in range(len(tiles)) if cum[i] * Hkv <= u)
-            n = tiles[x][1][4]
-            h, j0 = divmod(u - cum[x] * Hkv, n)
-            j1 = min(n, j0 + u1 - u)
+            begin, x, h, n = max(s for s in line if s[0] <= u)
+            a, b = u - begin, min(n + OVERHEAD, u1 - begin)
+            u = begin + b
+            j0, j1 = max(0, a - OVERHEAD), max(0, b - OVERHEAD)
+            if j0 == j1:
+                continue
             for j in range(j0, j1):
                 assert (x, h, j) not in covered
-                covered[x, h, j] = c
-            if (j0, j1) == (0, n):
+                covered.add((x, h, j))
+            if j1 - j0 == n:
                 whole.add((x, h))
             else:
                 slot = 2 * c + (0 if first else 1)
                 assert slot not in wrote
                 wrote[slot] = (x, h)
-            u, first = u + j1 - j0, False
-    assert len(covered) == units
-    merged = {}
-    for c in range(1, ctas):
-        u = per * c
-        if u >= units:
-            continue
-        x = max(i for i in range(len(tiles)) if cum[i] * Hkv <= u)
-        n = tiles[x][1][4]
-        h, j0 = divmod(u - cum[x] * Hkv, n)
-        begin = u - j0
-        if j0 == 0 or begin // per != c - 1:
-            continue
-        assert (x, h) not in merged
-        merged[x, h] = [2 * (c - 1) + (0 if begin % per == 0 else 1)] + \
-            [2 * s for s in range(c, (begin + n - 1) // per + 1)]
-    for (x, h), slots in merged.items():
+                s0, s1 = (begin + OVERHEAD) // per, (begin + OVERHEAD + n - 1) // per
+                arrived.setdefault(s0, []).append((x, h, begin, s1))
+            first = False
+    assert len(covered) == sum(n for *_, n in line)
+    cut = set()
+    for s0, parts in arrived.items():
+        assert len(set(parts)) == 1  # a counter belongs to one (q tile, head)
+        x, h, begin, s1 = parts[0]
+        assert len(parts) == s1 - s0 + 1 > 1
+        slots = [2 * s + (0 if per * s >= begin else 1) for s in range(s0, s1 + 1)]
         assert slots == sorted(s for s, at in wrote.items() if at == (x, h))
-    assert whole | set(merged) == {(x, h) for x in range(len(tiles)) for h in range(Hkv)}
-    assert not whole & set(merged)
+        cut.add((x, h))
+    assert whole | cut == {(x, h) for _, x, h, _ in line} and not whole & cut
 
 
 def test_workspace_query_needs_no_gpu():

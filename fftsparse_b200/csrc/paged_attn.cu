@@ -13,7 +13,8 @@
 // decode request and a batch of ragged chunks alike load every SM equally, and nothing about the lengths is
 // needed on the host.  A share that begins or ends between two key tiles of a (q tile, head) leaves fp32
 // partial sums, which are joined in the order of the shares.
-//   schedule_kernel  one CTA: q tiles of every request and the running sum of their lengths
+//   schedule         q tiles of every request and the running sum of their lengths: up to kOwnTiles q
+//                    tiles by every CTA of attn_kernel for itself, beyond by schedule_kernel (one CTA)
 //   attn_kernel      two CTAs per SM, each walking its share
 //   join_kernel      the (q tile, head)s that several shares cut (a kernel of its own: inside attn_kernel
 //                    its registers made the softmax loop spill, 1.15 -> 1.89 ms at 2048 tokens over 32768)
@@ -51,6 +52,8 @@ constexpr int kThreads = 192;
 constexpr int kKStages = 3, kVStages = 2;
 constexpr int kTmemCols = 256;  // S0, S1 (64 columns each), O (D): two CTAs fill an SM's 512
 constexpr uint32_t kTmemO = 128;
+constexpr int kSchedThreads = 1024;
+constexpr int kOwnTiles = 1024;  // up to so many q tiles every CTA builds the schedule itself
 constexpr int kMaxCtas = 512;   // partial slots in the workspace (two per CTA)
 constexpr int kMinShare = 4;    // length of a share, at least
 constexpr int kOverhead = 2;    // length of a (q tile, head) besides its key tiles
@@ -87,7 +90,7 @@ constexpr int BPF = BPV + 2;            // P(n) written (128 arrivals) [2]
 constexpr int BDRAIN = BPF + 2;
 
 // One q tile: tokens [tok0, tok0 + ntok) of request r, the first at position pos0.
-struct Tile {
+struct __align__(16) Tile {
   int tok0, pos0, ntok, r;
 };
 
@@ -107,6 +110,7 @@ struct Params {
   uint16_t *out;
   int64_t os_t, os_h;
   float scale_log2;
+  int own_schedule;           // every CTA has its own copy of tiles and cum
   Tile *tiles;                // [max_tiles]
   long long *cum;             // [max_tiles + 1]: length (of one head) before q tile x
   int *header;                // [0]: q tiles
@@ -143,8 +147,15 @@ __device__ __forceinline__ long long share_of(const Params &p, long long length)
 }
 
 // ---------------------------------------------------------------- schedule
-constexpr int kSchedThreads = 1024;
+// The q tiles of all requests and the line's running sum, by one CTA of NT threads; scratch in its shared memory.
+template <int NT>
+struct SchedScratch {
+  long long warp_sums[32];
+  long long tiles[NT];  // q tiles up to and with the request
+  int q0[NT], len[NT], kv[NT];
+};
 
+template <int NT>
 __device__ __forceinline__ long long sched_scan(long long v, long long *warp_sums, long long *total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
@@ -152,31 +163,29 @@ __device__ __forceinline__ long long sched_scan(long long v, long long *warp_sum
     const long long u = __shfl_up_sync(0xffffffffu, v, o);
     if (lane >= o) v += u;
   }
-  __syncthreads();
+  __syncthreads();  // the previous scan's sums have been read
   if (lane == 31) warp_sums[warp] = v;
   __syncthreads();
-  long long s = warp_sums[lane];
+  long long s = lane < NT / 32 ? warp_sums[lane] : 0;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const long long u = __shfl_up_sync(0xffffffffu, s, o);
     if (lane >= o) s += u;
   }
-  const long long before = warp > 0 ? __shfl_sync(0xffffffffu, s, warp - 1) : 0;
+  const long long before = __shfl_sync(0xffffffffu, s, max(warp - 1, 0));
   *total = __shfl_sync(0xffffffffu, s, 31);
-  return v + before;
+  return v + (warp > 0 ? before : 0);
 }
 
-__global__ void __launch_bounds__(kSchedThreads) schedule_kernel(const __grid_constant__ Params p) {
-  __shared__ long long warp_sums[32];
-  __shared__ long long s_tiles[kSchedThreads];  // q tiles up to and with the request
-  __shared__ int s_q0[kSchedThreads], s_len[kSchedThreads], s_kv[kSchedThreads];
+// tiles [max_tiles], cum [max_tiles + 1]; returns the number of q tiles, *length the line of one head.
+template <int NT>
+__device__ int build_schedule(const Params &p, Tile *tiles, long long *cum, SchedScratch<NT> &sc, long long *length) {
   const int tid = threadIdx.x;
   const long long cap = (long long)p.width << p.ps_shift;  // keys a table row can hold
-  long long tile_base = 0, unit_base = 0;
-  if (tid == 0) p.cum[0] = 0;
-  if (tid < p.ctas) p.cuts[tid].nrows = 0;
-  for (int r0 = 0; r0 < p.R; r0 += kSchedThreads) {
-    const int nr = min(kSchedThreads, p.R - r0);
+  long long tile_base = 0, line = 0;
+  if (tid == 0) cum[0] = 0;
+  for (int r0 = 0; r0 < p.R; r0 += NT) {
+    const int nr = min(NT, p.R - r0);
     int q0 = 0, len = 0, kv = 0;
     if (tid < nr) {
       // lengths are device data: kept inside q and the table whatever they hold
@@ -185,45 +194,55 @@ __global__ void __launch_bounds__(kSchedThreads) schedule_kernel(const __grid_co
       kv = int(min((long long)max(p.kv_lens[r0 + tid], 0), cap));
     }
     long long total;
-    const long long upto = sched_scan((len + p.tpt - 1) / p.tpt, warp_sums, &total);
-    s_tiles[tid] = upto;
-    s_q0[tid] = q0;
-    s_len[tid] = len;
-    s_kv[tid] = kv;
+    const long long upto = sched_scan<NT>((len + p.tpt - 1) / p.tpt, sc.warp_sums, &total);
+    sc.tiles[tid] = upto;
+    sc.q0[tid] = q0;
+    sc.len[tid] = len;
+    sc.kv[tid] = kv;
     __syncthreads();
     const long long fit = min(total, (long long)p.max_tiles - tile_base);
-    for (long long x0 = 0; x0 < fit; x0 += kSchedThreads) {
+    for (long long x0 = 0; x0 < fit; x0 += NT) {
       const long long x = x0 + tid;
       int n = 0;
       if (x < fit) {
         int lo = 0, hi = nr;  // the first request whose tiles reach past x
         while (lo < hi) {
           const int mid = (lo + hi) >> 1;
-          if (s_tiles[mid] > x) hi = mid; else lo = mid + 1;
+          if (sc.tiles[mid] > x) hi = mid; else lo = mid + 1;
         }
-        const int i = int(x - (lo > 0 ? s_tiles[lo - 1] : 0)) * p.tpt;
+        const int i = int(x - (lo > 0 ? sc.tiles[lo - 1] : 0)) * p.tpt;
         Tile t;
-        t.tok0 = s_q0[lo] + i;
-        t.pos0 = s_kv[lo] - s_len[lo] + i;
-        t.ntok = min(p.tpt, s_len[lo] - i);
+        t.tok0 = sc.q0[lo] + i;
+        t.pos0 = sc.kv[lo] - sc.len[lo] + i;
+        t.ntok = min(p.tpt, sc.len[lo] - i);
         t.r = r0 + lo;
         n = keys_of(t.pos0, t.ntok, p.window, p.sinks).n + kOverhead;
-        if (FFTS_IN_RANGE(tile_base + x, p.max_tiles)) p.tiles[tile_base + x] = t;
+        if (FFTS_IN_RANGE(tile_base + x, p.max_tiles)) tiles[tile_base + x] = t;
       }
-      long long units;
-      const long long before = sched_scan(n, warp_sums, &units);
-      if (x < fit && FFTS_IN_RANGE(tile_base + x, p.max_tiles)) p.cum[tile_base + x + 1] = unit_base + before;
-      unit_base += units;
+      long long sum;
+      const long long upto_x = sched_scan<NT>(n, sc.warp_sums, &sum);
+      if (x < fit && FFTS_IN_RANGE(tile_base + x, p.max_tiles)) cum[tile_base + x + 1] = line + upto_x;
+      line += sum;
     }
     tile_base += max(fit, 0ll);
     __syncthreads();  // the chunk's arrays have been read
   }
-  if (tid == 0) p.header[0] = int(tile_base);
+  *length = line;
+  return int(tile_base);
+}
+
+__global__ void __launch_bounds__(kSchedThreads) schedule_kernel(const __grid_constant__ Params p) {
+  __shared__ SchedScratch<kSchedThreads> sc;
+  long long length;
+  const int n = build_schedule<kSchedThreads>(p, p.tiles, p.cum, sc, &length);
+  if (threadIdx.x == 0) p.header[0] = n;
 }
 
 // Walks the share [u, u1) of the line segment by segment; the same in every lane.
 struct Walk {
   const Params &p;
+  const Tile *tiles;
+  const long long *cum;
   long long u, u1;
   long long base, next;  // the line before q tile x and behind it, all heads
   int x;
@@ -231,7 +250,7 @@ struct Walk {
   Keys g;
   int h, j0, j1;         // the segment: head and key tiles [j0, j1) of the g.n
   long long begin;       // where its (q tile, head) begins
-  __device__ __forceinline__ Walk(const Params &prm) : p(prm) {}
+  __device__ __forceinline__ Walk(const Params &prm, const Tile *t_, const long long *c_) : p(prm), tiles(t_), cum(c_) {}
 
   // Finds the q tile at u0 (whole warp; u0 < length).
   __device__ __forceinline__ void seek(long long u0, long long end, int ntiles) {
@@ -242,7 +261,7 @@ struct Walk {
     while (n > 1) {
       const int step = (n + 31) / 32;
       const int i = lane * step;
-      const bool below = i < n && p.cum[lo + i] * p.Hkv <= u0;
+      const bool below = i < n && cum[lo + i] * p.Hkv <= u0;
       const int last = 31 - __clz(__ballot_sync(0xffffffffu, below));
       const int off = last * step;
       lo += off;
@@ -252,9 +271,9 @@ struct Walk {
     load();
   }
   __device__ __forceinline__ void load() {
-    t = p.tiles[FFTS_INDEX(x, p.max_tiles)];
-    base = p.cum[x] * p.Hkv;
-    next = p.cum[x + 1] * p.Hkv;
+    t = tiles[FFTS_INDEX(x, p.max_tiles)];
+    base = cum[x] * p.Hkv;
+    next = cum[x + 1] * p.Hkv;
     g = keys_of(t.pos0, t.ntok, p.window, p.sinks);
   }
   // The next segment with key tiles; false behind the share's end.
@@ -327,14 +346,32 @@ __global__ void __launch_bounds__(kThreads, 2)
   using Lay = Layout<D>;
   extern __shared__ __align__(16) uint8_t smem[];
   if (smem_u32(smem) & 1023u) {  // SWIZZLE_128B tiles need 1024-byte alignment
-    if (threadIdx.x == 0) *reinterpret_cast<volatile int *>(p.status) = kErrSmemAlign;
+    if (threadIdx.x == 0) {
+      *reinterpret_cast<volatile int *>(p.status) = kErrSmemAlign;
+      p.cuts[blockIdx.x].nrows = 0;
+    }
     return;
   }
-  const int ntiles = p.header[0];
-  const long long length = p.cum[FFTS_INDEX(ntiles, p.max_tiles + 1)] * p.Hkv;
+  Tile *tiles = p.tiles;
+  long long *cum = p.cum;
+  int ntiles;
+  long long length;
+  if (p.own_schedule) {
+    tiles += int64_t(blockIdx.x) * p.max_tiles;
+    cum += int64_t(blockIdx.x) * (p.max_tiles + 1);
+    // the scratch lies where the K ring will be
+    ntiles = build_schedule<kThreads>(p, tiles, cum, *reinterpret_cast<SchedScratch<kThreads> *>(smem + Lay::k), &length);
+  } else {
+    ntiles = p.header[0];
+    length = cum[FFTS_INDEX(ntiles, p.max_tiles + 1)];
+  }
+  length *= p.Hkv;
   const long long per = share_of(p, length);
   const long long u0 = per * blockIdx.x, u1 = min(length, u0 + per);
-  if (u0 >= u1) return;  // uniform in the CTA, before any allocation
+  if (u0 >= u1) {  // uniform in the CTA, before any allocation
+    if (threadIdx.x == 0) p.cuts[blockIdx.x].nrows = 0;
+    return;
+  }
   const uint32_t sbase = smem_u32(smem);
   auto bar = [&](int i) { return sbase + Lay::bars + 8u * uint32_t(i); };
   volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + Lay::abort);
@@ -352,7 +389,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     const int row = qrows + (i >> 3) / Lay::halves, hf = (i >> 3) % Lay::halves;
     *reinterpret_cast<uint4 *>(smem + Lay::q + hf * Lay::q_half + row * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
   }
-  if (qrows < kBM) fence_proxy_async();
+  fence_proxy_async();  // TMA writes over the scratch, the MMAs read the zeros
   if (warp == 5) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
                  "r"(kTmemCols));
@@ -369,7 +406,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   const uint32_t tmem = *tmem_slot;
   const uint32_t tm_o = tmem + kTmemO;
 
-  Walk w(p);
+  Walk w(p, tiles, cum);
   w.seek(u0, u1, ntiles);
 
   if (warp == 4) {
@@ -527,7 +564,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     const int tl = r / p.G, hg = r - tl * p.G;  // the row's token in the tile and head in the group
     const uint32_t lane_off = uint32_t(warp * 32) << 16;
     const float2 sc2 = make_float2(p.scale_log2, p.scale_log2);
-    bool ok = true, first_seg = true;
+    bool ok = true, first_seg = true, noted = false;
     int n = 0;
     while (ok && w.segment()) {
       const Keys g = w.g;
@@ -671,11 +708,10 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {
           float o[32];
+          __syncwarp();
           tmem_ld32(tm_o + lane_off + c * 32, o);
           tmem_wait_ld();
-          if (!live) continue;
-          if (whole) {
-            if (!FFTS_IN_RANGE(w.t.tok0 + tl, p.T)) continue;
+          if (live && whole && FFTS_IN_RANGE(w.t.tok0 + tl, p.T)) {
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
               uint32_t v[4];
@@ -685,7 +721,8 @@ __global__ void __launch_bounds__(kThreads, 2)
                                     l_run > 0.0f ? o[q * 8 + 2 * e + 1] * inv_l : 0.0f);
               *reinterpret_cast<uint4 *>(dst + c * 32 + q * 8) = make_uint4(v[0], v[1], v[2], v[3]);
             }
-          } else if (FFTS_IN_RANGE(slot, 2 * p.ctas)) {
+          }
+          if (live && !whole && FFTS_IN_RANGE(slot, 2 * p.ctas)) {
 #pragma unroll
             for (int q = 0; q < 8; ++q)
               pd[(c * 8 + q) * kBM] = make_float4(o[q * 4], o[q * 4 + 1], o[q * 4 + 2], o[q * 4 + 3]);
@@ -703,9 +740,11 @@ __global__ void __launch_bounds__(kThreads, 2)
         cut.s1 = int((w.begin + kOverhead + g.n - 1) / per);
         cut.first_slot = 2 * int(blockIdx.x) + (first_seg ? 0 : 1);
         p.cuts[blockIdx.x] = cut;
+        noted = true;
       }
       first_seg = false;
     }
+    if (r == 0 && !noted) p.cuts[blockIdx.x].nrows = 0;
     if (!ok) {
       *abort_flag = 1;
       *reinterpret_cast<volatile int *>(p.status) = kErrSoftmax;
@@ -794,6 +833,7 @@ constexpr int kJoinBlocks = 4;
 
 template <typename E, int D>
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ Params p) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // launched early: attn_kernel's stores are visible from here
   const int s0 = int(blockIdx.x);
   const Cut cut = p.cuts[s0];
   if (cut.nrows == 0) return;
@@ -851,9 +891,10 @@ struct Space {
   Space(int64_t T, int64_t R, int64_t G, int64_t D) {
     const int64_t tpt = kBM / G;
     max_tiles = T / tpt + std::min(R, T);  // sum of ceil(len / tpt)
+    const int64_t copies = max_tiles <= kOwnTiles ? kMaxCtas : 1;
     cum = 0;
-    tiles = cum + (max_tiles + 2) / 2 * 16;
-    header = tiles + max_tiles * 16;
+    tiles = cum + (copies * (max_tiles + 1) + 1) / 2 * 16;
+    header = tiles + copies * max_tiles * 16;
     cuts = header + 16;
     ml = cuts + kMaxCtas * int64_t(sizeof(Cut));
     part = ml + int64_t(2 * kMaxCtas) * kBM * 8;
@@ -881,12 +922,23 @@ static int launch(const Params &p, const void *q, const int64_t *qs, const void 
     rc = ensure_func_smem(reinterpret_cast<const void *>(&attn_kernel<E, D>), Layout<D>::bytes,
                           int(cudaSharedmemCarveoutMaxShared));
   if (rc) return rc;
-  schedule_kernel<<<1, kSchedThreads, 0, stream>>>(p);
-  FFTS_CUDA(cudaGetLastError());
+  if (!p.own_schedule) {
+    schedule_kernel<<<1, kSchedThreads, 0, stream>>>(p);
+    FFTS_CUDA(cudaGetLastError());
+  }
   attn_kernel<E, D><<<unsigned(p.ctas), kThreads, Layout<D>::bytes, stream>>>(mq, mk, mv, p);
   FFTS_CUDA(cudaGetLastError());
-  join_kernel<E, D><<<dim3(unsigned(p.ctas), kJoinBlocks), kJoinThreads, 0, stream>>>(p);
-  FFTS_CUDA(cudaGetLastError());
+  // launched while attn_kernel drains
+  cudaLaunchAttribute early{};
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(unsigned(p.ctas), kJoinBlocks);
+  cfg.blockDim = dim3(kJoinThreads);
+  cfg.stream = stream;
+  cfg.attrs = &early;
+  cfg.numAttrs = 1;
+  FFTS_CUDA(cudaLaunchKernelEx(&cfg, join_kernel<E, D>, p));
   return FFTS_OK;
 }
 
@@ -949,6 +1001,7 @@ int paged_attn(const void *q, const int64_t *qs, const void *k_pages, const int6
   p.os_h = os[1];
   p.scale_log2 = scale * 1.4426950408889634f;
   p.max_tiles = int(sp.max_tiles);
+  p.own_schedule = sp.max_tiles <= kOwnTiles;
   p.cum = reinterpret_cast<long long *>(base + sp.cum);
   p.tiles = reinterpret_cast<Tile *>(base + sp.tiles);
   p.header = reinterpret_cast<int *>(base + sp.header);

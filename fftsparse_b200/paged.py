@@ -21,8 +21,8 @@ which copies the already rotated k.
 """
 from __future__ import annotations
 
-import ctypes
 import math
+import struct
 from typing import NamedTuple, Optional, Tuple
 
 import torch
@@ -33,58 +33,71 @@ from .status import device_status
 __all__ = ["PagePlan", "plan_pages", "rotary_inv_freq", "rope_append", "paged_attention"]
 
 _DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
-_I64x2 = ctypes.c_int64 * 2
-_I64x3 = ctypes.c_int64 * 3
+_pack2 = struct.Struct("2q").pack  # strides as the C calls take them: int64 arrays
+_pack3 = struct.Struct("3q").pack
+_raw_stream = torch._C._cuda_getCurrentRawStream  # current_stream(device).cuda_stream without the Stream object
 
 
-def _on_device(device: torch.device, fn, *args) -> None:
+def _call(device: torch.device, fn, *args) -> None:
     """One C call with ``device`` current, on its current stream."""
-    if device.index == torch.cuda.current_device():
-        _lib.check(fn(*args, torch.cuda.current_stream(device).cuda_stream))
+    index = device.index
+    if index == torch.cuda.current_device():
+        rc = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(device):
-            _lib.check(fn(*args, torch.cuda.current_stream(device).cuda_stream))
+            rc = fn(*args, _raw_stream(index))
+    if rc:
+        _lib.check(rc)
 
 
-def _check_ints(name: str, t: torch.Tensor, shape, device) -> None:
-    if t.dtype != torch.int32:
+def _check_ints(name: str, t: torch.Tensor, n: int, device) -> None:
+    if t.dtype is not torch.int32:
         raise TypeError(f"{name} must be int32, got {t.dtype}")
-    if t.shape != shape or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous tensor of shape {tuple(shape)}, got {tuple(t.shape)}")
+    if t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous tensor of shape [{n}], got {tuple(t.shape)}")
     if t.device != device:
         raise ValueError(f"{name} must be on {device}, got {t.device}")
 
 
-def _check_table(t: torch.Tensor, rows: int, device) -> None:
-    if t.dtype != torch.int32:
+def _check_table(t: torch.Tensor, rows: int, device) -> int:
+    """The table's row stride (any, of a single row)."""
+    if t.dtype is not torch.int32:
         raise TypeError(f"block_table must be int32, got {t.dtype}")
     if t.dim() != 2 or t.shape[0] != rows or (t.shape[1] > 1 and t.stride(1) != 1):
         raise ValueError(f"block_table must be [{rows}, pages] with unit stride along a row, got {tuple(t.shape)}")
     if t.device != device:
         raise ValueError(f"block_table must be on {device}, got {t.device}")
+    return t.stride(0) if rows > 1 else t.shape[1]
 
 
-def _check_heads(name: str, t: torch.Tensor, dtype, device) -> None:
+def _check_heads(name: str, t: torch.Tensor, dtype, device):
+    """The strides of a [tokens, heads, head_dim] tensor, packed."""
     if t.dim() != 3:
         raise ValueError(f"{name} must be [tokens, heads, head_dim], got shape {tuple(t.shape)}")
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
     if t.device != device:
         raise ValueError(f"{name} must be on {device}, got {t.device}")
-    if t.stride(2) != 1:
+    st, sh, sd = t.stride()
+    if sd != 1:
         raise ValueError(f"{name} must be contiguous in the head dimension")
+    return _pack2(st, sh)
 
 
-def _check_pool(k_pages: torch.Tensor, v_pages: torch.Tensor, dtype, device) -> None:
+def _check_pool(k_pages: torch.Tensor, v_pages: torch.Tensor, dtype, device):
+    """The strides of both pool tensors, packed."""
     if k_pages.dim() != 4 or v_pages.shape != k_pages.shape:
         raise ValueError(f"k_pages and v_pages must both be [pages, Hkv, page_size, D], got "
                          f"{tuple(k_pages.shape)} / {tuple(v_pages.shape)}")
-    if k_pages.dtype != dtype or v_pages.dtype != dtype:
+    if k_pages.dtype is not dtype or v_pages.dtype is not dtype:
         raise TypeError(f"k_pages and v_pages must be {dtype}, got {k_pages.dtype} / {v_pages.dtype}")
     if k_pages.device != device or v_pages.device != device:
         raise ValueError(f"k_pages and v_pages must be on {device}")
-    if k_pages.stride(3) != 1 or v_pages.stride(3) != 1:
+    *ks, kd = k_pages.stride()
+    *vs, vd = v_pages.stride()
+    if kd != 1 or vd != 1:
         raise ValueError("k_pages and v_pages must be contiguous in the head dimension")
+    return _pack3(*ks), _pack3(*vs)
 
 
 def _check_cuda(name: str, t: torch.Tensor) -> None:
@@ -121,20 +134,24 @@ def plan_pages(cached_lens: torch.Tensor, new_lens: torch.Tensor, block_table: t
     dev = cached_lens.device
     if cached_lens.dim() != 1 or free_pages.dim() != 1:
         raise ValueError("cached_lens and free_pages must be 1-D")
-    R = cached_lens.shape[0]
-    _check_ints("cached_lens", cached_lens, (R,), dev)
-    _check_ints("new_lens", new_lens, (R,), dev)
-    _check_table(block_table, R, dev)
-    _check_ints("free_pages", free_pages, free_pages.shape, dev)
+    R, n_free = cached_lens.shape[0], free_pages.shape[0]
+    _check_ints("cached_lens", cached_lens, R, dev)
+    _check_ints("new_lens", new_lens, R, dev)
+    _check_ints("free_pages", free_pages, n_free, dev)
+    table_ld = _check_table(block_table, R, dev)
     if num_tokens < 0:
         raise ValueError(f"num_tokens must not be negative, got {num_tokens}")
     _check_cuda("cached_lens", cached_lens)
-    buf = torch.empty(2 * R + 3 + 2 * num_tokens, dtype=torch.int32, device=dev)
-    plan = PagePlan(*buf.split([R + 1, R, num_tokens, num_tokens, 2]))
-    width = block_table.shape[1]
-    _on_device(dev, _lib.load().ffts_page_plan, cached_lens.data_ptr(), new_lens.data_ptr(), R,
-               block_table.data_ptr(), block_table.stride(0) if R > 1 else width, width, free_pages.data_ptr(),
-               free_pages.shape[0], page_size, num_tokens, *[t.data_ptr() for t in plan])
+    sizes = [R + 1, R, num_tokens, num_tokens, 2]
+    buf = torch.empty(2 * R + 2 * num_tokens + 3, dtype=torch.int32, device=dev)
+    plan = PagePlan(*buf.split_with_sizes(sizes))
+    cu = buf.data_ptr()
+    kv = cu + 4 * (R + 1)
+    pos = kv + 4 * R
+    slot = pos + 4 * num_tokens
+    _call(dev, _lib.load().ffts_page_plan, cached_lens.data_ptr(), new_lens.data_ptr(), R, block_table.data_ptr(),
+          table_ld, block_table.shape[1], free_pages.data_ptr(), n_free, page_size, num_tokens, cu, kv, pos, slot,
+          slot + 4 * num_tokens)
     return plan
 
 
@@ -216,49 +233,47 @@ def rope_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, pos
     dev, dt = k.device, k.dtype
     if dt not in _DTYPES:
         raise TypeError(f"rope_append supports bfloat16 and float16, got {dt}")
-    _check_heads("k", k, dt, dev)
-    _check_heads("v", v, dt, dev)
+    ks = _check_heads("k", k, dt, dev)
+    vs = _check_heads("v", v, dt, dev)
     T, Hkv, D = k.shape
     if v.shape != k.shape:
         raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} differ in shape")
-    _check_pool(k_pages, v_pages, dt, dev)
-    if k_pages.shape[1] != Hkv or k_pages.shape[3] != D:
+    kps, vps = _check_pool(k_pages, v_pages, dt, dev)
+    P, kv_heads, page_size, dim = k_pages.shape
+    if kv_heads != Hkv or dim != D:
         raise ValueError(f"pages {tuple(k_pages.shape)} do not match k {tuple(k.shape)}")
-    _check_ints("positions", positions, (T,), dev)
-    _check_ints("slot_map", slot_map, (T,), dev)
-    rd = 0
+    _check_ints("positions", positions, T, dev)
+    _check_ints("slot_map", slot_map, T, dev)
+    rd, freq = 0, None
     if inv_freq is not None:
-        if inv_freq.dim() != 1 or inv_freq.dtype != torch.float32 or not inv_freq.is_contiguous():
+        if inv_freq.dim() != 1 or inv_freq.dtype is not torch.float32 or not inv_freq.is_contiguous():
             raise ValueError("inv_freq must be a contiguous 1-D fp32 tensor")
         if inv_freq.device != dev:
             raise ValueError(f"inv_freq must be on {dev}, got {inv_freq.device}")
-        rd = 2 * inv_freq.shape[0]
+        rd, freq = 2 * inv_freq.shape[0], inv_freq.data_ptr()
+    H, q_ptr, o_ptr, qs, os_ = 0, None, None, None, None
     if q is not None:
-        _check_heads("q", q, dt, dev)
+        qs = _check_heads("q", q, dt, dev)
+        H = q.shape[1]
         if q.shape[0] != T or q.shape[2] != D:
             raise ValueError(f"q {tuple(q.shape)} does not match k {tuple(k.shape)}")
     if out is not None:
         if q is None:
             raise ValueError("out without q")
-        _check_heads("out", out, dt, dev)
+        os_ = _check_heads("out", out, dt, dev)
         if out.shape != q.shape:
             raise ValueError(f"out must have q's shape {tuple(q.shape)}, got {tuple(out.shape)}")
     _check_cuda("k", k)
-    H, q_ptr, o_ptr, qs, os_ = 0, None, None, None, None
     if q is not None:
-        H = q.shape[1]
         if out is None:
             out = torch.empty(T, H, D, dtype=dt, device=dev)
+            os_ = _pack2(H * D, D)
         q_ptr, o_ptr = q.data_ptr(), out.data_ptr()
-        qs, os_ = _I64x2(q.stride(0), q.stride(1)), _I64x2(out.stride(0), out.stride(1))
     if T == 0:
         return out
-    P, _, page_size, _ = k_pages.shape
-    _on_device(dev, _lib.load().ffts_rope_append, q_ptr, qs, k.data_ptr(), _I64x2(k.stride(0), k.stride(1)),
-               v.data_ptr(), _I64x2(v.stride(0), v.stride(1)), _DTYPES[dt], T, H, Hkv, D, positions.data_ptr(),
-               slot_map.data_ptr(), inv_freq.data_ptr() if rd else None, rd, int(bool(interleaved)),
-               float(attn_factor), o_ptr, os_, k_pages.data_ptr(), _I64x3(*k_pages.stride()[:3]), v_pages.data_ptr(),
-               _I64x3(*v_pages.stride()[:3]), P, page_size)
+    _call(dev, _lib.load().ffts_rope_append, q_ptr, qs, k.data_ptr(), ks, v.data_ptr(), vs, _DTYPES[dt], T, H, Hkv, D,
+          positions.data_ptr(), slot_map.data_ptr(), freq, rd, interleaved, attn_factor, o_ptr, os_,
+          k_pages.data_ptr(), kps, v_pages.data_ptr(), vps, P, page_size)
     return out
 
 
@@ -282,18 +297,18 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     dev, dt = q.device, q.dtype
     if dt not in _DTYPES:
         raise TypeError(f"paged attention supports bfloat16 and float16, got {dt}")
-    _check_heads("q", q, dt, dev)
-    _check_pool(k_pages, v_pages, dt, dev)
+    qs = _check_heads("q", q, dt, dev)
+    kps, vps = _check_pool(k_pages, v_pages, dt, dev)
     T, H, D = q.shape
-    P, Hkv, page_size, Dk = k_pages.shape
-    if Dk != D or Hkv == 0 or H % Hkv:
+    P, Hkv, page_size, dim = k_pages.shape
+    if dim != D or Hkv == 0 or H % Hkv:
         raise ValueError(f"pages {tuple(k_pages.shape)} do not match q {tuple(q.shape)}")
     if kv_lens.dim() != 1:
         raise ValueError("kv_lens must be 1-D")
     R = kv_lens.shape[0]
-    _check_ints("kv_lens", kv_lens, (R,), dev)
-    _check_ints("cu_q", cu_q, (R + 1,), dev)
-    _check_table(block_table, R, dev)
+    _check_ints("kv_lens", kv_lens, R, dev)
+    _check_ints("cu_q", cu_q, R + 1, dev)
+    table_ld = _check_table(block_table, R, dev)
     if window is None:
         if sinks:
             raise ValueError("sinks need a window")
@@ -303,7 +318,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     if sinks < 0:
         raise ValueError(f"sinks must not be negative, got {sinks}")
     if out is not None:
-        _check_heads("out", out, dt, dev)
+        os_ = _check_heads("out", out, dt, dev)
         if out.shape != q.shape:
             raise ValueError(f"out must have q's shape {tuple(q.shape)}, got {tuple(out.shape)}")
     if P == 0:
@@ -311,6 +326,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     _check_cuda("q", q)
     if out is None:
         out = torch.empty(T, H, D, dtype=dt, device=dev)
+        os_ = _pack2(H * D, D)
     if T == 0 or R == 0:
         return out
     lib = _lib.load()
@@ -318,10 +334,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     status.poll_direct()
     nbytes = lib.ffts_paged_workspace_bytes(T, R, H, Hkv, D)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    width = block_table.shape[1]
-    _on_device(dev, lib.ffts_paged_attn, q.data_ptr(), _I64x2(q.stride(0), q.stride(1)), k_pages.data_ptr(),
-               _I64x3(*k_pages.stride()[:3]), v_pages.data_ptr(), _I64x3(*v_pages.stride()[:3]), _DTYPES[dt], T, R, H,
-               Hkv, D, P, page_size, block_table.data_ptr(), block_table.stride(0) if R > 1 else width, width,
-               cu_q.data_ptr(), kv_lens.data_ptr(), D ** -0.5 if scale is None else float(scale), window, sinks,
-               out.data_ptr(), _I64x2(out.stride(0), out.stride(1)), ws.data_ptr(), nbytes, status.direct_ptr)
+    _call(dev, lib.ffts_paged_attn, q.data_ptr(), qs, k_pages.data_ptr(), kps, v_pages.data_ptr(), vps, _DTYPES[dt], T,
+          R, H, Hkv, D, P, page_size, block_table.data_ptr(), table_ld, block_table.shape[1], cu_q.data_ptr(),
+          kv_lens.data_ptr(), D ** -0.5 if scale is None else scale, window, sinks, out.data_ptr(), os_,
+          ws.data_ptr(), nbytes, status.direct_ptr)
     return out

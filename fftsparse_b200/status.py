@@ -134,6 +134,8 @@ _DEVICE_WORDS: Dict[int, StatusWord] = {}
 
 def device_status(device) -> StatusWord:
     """The status word the operators use on ``device`` when the caller passes none."""
+    if isinstance(device, torch.device) and device.index in _DEVICE_WORDS and device.type == "cuda":
+        return _DEVICE_WORDS[device.index]
     device = torch.device(device)
     if device.type != "cuda":  # host-side tests drive the operators' logic with CPU tensors
         idx, dev = -1, torch.device("cpu")

@@ -308,6 +308,14 @@ def test_paged_attention_many_heads_to_a_kv_head(H, Hkv):
     b.check(b.run())
 
 
+@pytest.mark.parametrize("lens", [[(i % 70, 1) for i in range(1300)], [(100, 9003), (7, 1)], [(40, 2)] * 1024])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (90, 5)])
+def test_paged_attention_many_q_tiles(lens, window, sinks):
+    """More q tiles than a CTA schedules by itself, and just as many as it does."""
+    b = Batch(lens, 16, 1, 64, BF, 16, window=window, sinks=sinks, drop=True)
+    b.check(b.run())
+
+
 @pytest.mark.parametrize("dt", [BF, FP])
 def test_paged_attention_scores_that_grow_and_peak(dt):
     """Scores far apart (the running maximum moves by more than its slack) and a scale of its own."""

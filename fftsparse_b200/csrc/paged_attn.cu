@@ -32,19 +32,14 @@
 //               would reach the sum.
 // Every mbarrier wait is bounded (a status code instead of a hang).
 
-#include <cuda.h>
-#include <cuda_fp16.h>
 #include <cudaTypedefs.h>
 
 #include <algorithm>
 
-#include "ffts_common.cuh"
-#include "tc_sm100.cuh"
+#include "paged_common.cuh"
 
 namespace ffts {
 namespace paged {
-
-using namespace ::ffts::tc;
 
 constexpr int kBM = 128;      // rows of a q tile
 constexpr int kBN = 64;       // keys of a key tile
@@ -52,14 +47,7 @@ constexpr int kThreads = 192;
 constexpr int kKStages = 3, kVStages = 2;
 constexpr int kTmemCols = 256;  // S0, S1 (64 columns each), O (D): two CTAs fill an SM's 512
 constexpr uint32_t kTmemO = 128;
-constexpr int kSchedThreads = 1024;
-constexpr int kOwnTiles = 1024;  // up to so many q tiles every CTA builds the schedule itself
-constexpr int kMaxCtas = 512;   // partial slots in the workspace (two per CTA)
-constexpr int kMinShare = 4;    // length of a share, at least
-constexpr int kOverhead = 2;    // length of a (q tile, head) besides its key tiles
 constexpr double kWaitSeconds = 2.0, kDrainSeconds = 4.0;
-
-constexpr int kErrProducer = 10, kErrMma = 11, kErrSoftmax = 12, kErrSmemAlign = 13;
 
 template <int D>
 struct Layout {
@@ -89,256 +77,6 @@ constexpr int BPV = BSF + 2;            // PV(n) complete, frees V stage n % 2 [
 constexpr int BPF = BPV + 2;            // P(n) written (128 arrivals) [2]
 constexpr int BDRAIN = BPF + 2;
 
-// One q tile: tokens [tok0, tok0 + ntok) of request r, the first at position pos0.
-struct __align__(16) Tile {
-  int tok0, pos0, ntok, r;
-};
-
-// A (q tile, head) that several shares cut: rows nrows from token tok0 and head head0 on; its partials lie in
-// first_slot and in the first slots of the shares behind it up to s1.  nrows 0: none.
-struct Cut {
-  int tok0, nrows, head0, s1, first_slot;
-};
-
-struct Params {
-  int T, R, H, Hkv, G, tpt;   // tpt: tokens per q tile
-  const int32_t *table;       // [R, width]
-  int64_t table_ld;
-  int width, n_pages, ps_shift;
-  const int32_t *cu_q, *kv_lens;
-  int window, sinks;          // window 0: none
-  uint16_t *out;
-  int64_t os_t, os_h;
-  float scale_log2;
-  int own_schedule;           // every CTA has its own copy of tiles and cum
-  Tile *tiles;                // [max_tiles]
-  long long *cum;             // [max_tiles + 1]: length (of one head) before q tile x
-  int *header;                // [0]: q tiles
-  Cut *cuts;                  // [ctas]: the (q tile, head) that share c begins and others go on with
-  float *part;                // [2 * ctas][D / 4][128 rows] float4
-  float2 *part_ml;            // [2 * ctas][128 rows]: m (log2 units) and l
-  int max_tiles, ctas;
-  int *status;
-  long long wait_cycles, drain_cycles;
-};
-
-// The key tiles of a q tile: [0, st), then [wt0, ...); n of them in all (at least one, which may be all
-// masked).  Keys >= hi, and keys < lo that are not sinks, are seen by no row.
-struct Keys {
-  int hi, lo, st, wt0, n;
-};
-
-__device__ __forceinline__ Keys keys_of(int pos0, int ntok, int window, int sinks) {
-  Keys g;
-  g.hi = max(0, pos0 + ntok);
-  g.lo = window > 0 ? max(0, pos0 - window + 1) : 0;
-  const int nt = (g.hi + kBN - 1) / kBN;
-  g.wt0 = g.lo / kBN;
-  g.st = min((min(sinks, g.hi) + kBN - 1) / kBN, g.wt0);
-  g.n = max(1, g.st + nt - g.wt0);
-  return g;
-}
-
-__device__ __forceinline__ int key_tile(const Keys &g, int j) { return j < g.st ? j : j - g.st + g.wt0; }
-
-__device__ __forceinline__ long long share_of(const Params &p, long long length) {
-  const long long per = (length + p.ctas - 1) / p.ctas;
-  return per < kMinShare ? kMinShare : per;
-}
-
-// ---------------------------------------------------------------- schedule
-// The q tiles of all requests and the line's running sum, by one CTA of NT threads; scratch in its shared memory.
-template <int NT>
-struct SchedScratch {
-  long long warp_sums[32];
-  long long tiles[NT];  // q tiles up to and with the request
-  int q0[NT], len[NT], kv[NT];
-};
-
-template <int NT>
-__device__ __forceinline__ long long sched_scan(long long v, long long *warp_sums, long long *total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long long u = __shfl_up_sync(0xffffffffu, v, o);
-    if (lane >= o) v += u;
-  }
-  __syncthreads();  // the previous scan's sums have been read
-  if (lane == 31) warp_sums[warp] = v;
-  __syncthreads();
-  long long s = lane < NT / 32 ? warp_sums[lane] : 0;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long long u = __shfl_up_sync(0xffffffffu, s, o);
-    if (lane >= o) s += u;
-  }
-  const long long before = __shfl_sync(0xffffffffu, s, max(warp - 1, 0));
-  *total = __shfl_sync(0xffffffffu, s, 31);
-  return v + (warp > 0 ? before : 0);
-}
-
-// tiles [max_tiles], cum [max_tiles + 1]; returns the number of q tiles, *length the line of one head.
-template <int NT>
-__device__ int build_schedule(const Params &p, Tile *tiles, long long *cum, SchedScratch<NT> &sc, long long *length) {
-  const int tid = threadIdx.x;
-  const long long cap = (long long)p.width << p.ps_shift;  // keys a table row can hold
-  long long tile_base = 0, line = 0;
-  if (tid == 0) cum[0] = 0;
-  for (int r0 = 0; r0 < p.R; r0 += NT) {
-    const int nr = min(NT, p.R - r0);
-    int q0 = 0, len = 0, kv = 0;
-    if (tid < nr) {
-      // lengths are device data: kept inside q and the table whatever they hold
-      q0 = min(max(p.cu_q[r0 + tid], 0), p.T);
-      len = min(max(p.cu_q[r0 + tid + 1], q0), p.T) - q0;
-      kv = int(min((long long)max(p.kv_lens[r0 + tid], 0), cap));
-    }
-    long long total;
-    const long long upto = sched_scan<NT>((len + p.tpt - 1) / p.tpt, sc.warp_sums, &total);
-    sc.tiles[tid] = upto;
-    sc.q0[tid] = q0;
-    sc.len[tid] = len;
-    sc.kv[tid] = kv;
-    __syncthreads();
-    const long long fit = min(total, (long long)p.max_tiles - tile_base);
-    for (long long x0 = 0; x0 < fit; x0 += NT) {
-      const long long x = x0 + tid;
-      int n = 0;
-      if (x < fit) {
-        int lo = 0, hi = nr;  // the first request whose tiles reach past x
-        while (lo < hi) {
-          const int mid = (lo + hi) >> 1;
-          if (sc.tiles[mid] > x) hi = mid; else lo = mid + 1;
-        }
-        const int i = int(x - (lo > 0 ? sc.tiles[lo - 1] : 0)) * p.tpt;
-        Tile t;
-        t.tok0 = sc.q0[lo] + i;
-        t.pos0 = sc.kv[lo] - sc.len[lo] + i;
-        t.ntok = min(p.tpt, sc.len[lo] - i);
-        t.r = r0 + lo;
-        n = keys_of(t.pos0, t.ntok, p.window, p.sinks).n + kOverhead;
-        if (FFTS_IN_RANGE(tile_base + x, p.max_tiles)) tiles[tile_base + x] = t;
-      }
-      long long sum;
-      const long long upto_x = sched_scan<NT>(n, sc.warp_sums, &sum);
-      if (x < fit && FFTS_IN_RANGE(tile_base + x, p.max_tiles)) cum[tile_base + x + 1] = line + upto_x;
-      line += sum;
-    }
-    tile_base += max(fit, 0ll);
-    __syncthreads();  // the chunk's arrays have been read
-  }
-  *length = line;
-  return int(tile_base);
-}
-
-__global__ void __launch_bounds__(kSchedThreads) schedule_kernel(const __grid_constant__ Params p) {
-  __shared__ SchedScratch<kSchedThreads> sc;
-  long long length;
-  const int n = build_schedule<kSchedThreads>(p, p.tiles, p.cum, sc, &length);
-  if (threadIdx.x == 0) p.header[0] = n;
-}
-
-// Walks the share [u, u1) of the line segment by segment; the same in every lane.
-struct Walk {
-  const Params &p;
-  const Tile *tiles;
-  const long long *cum;
-  long long u, u1;
-  long long base, next;  // the line before q tile x and behind it, all heads
-  int x;
-  Tile t;
-  Keys g;
-  int h, j0, j1;         // the segment: head and key tiles [j0, j1) of the g.n
-  long long begin;       // where its (q tile, head) begins
-  __device__ __forceinline__ Walk(const Params &prm, const Tile *t_, const long long *c_) : p(prm), tiles(t_), cum(c_) {}
-
-  // Finds the q tile at u0 (whole warp; u0 < length).
-  __device__ __forceinline__ void seek(long long u0, long long end, int ntiles) {
-    u = u0;
-    u1 = end;
-    int lo = 0, n = ntiles;  // x is in [lo, lo + n): cum[lo] * Hkv <= u0
-    const int lane = threadIdx.x & 31;
-    while (n > 1) {
-      const int step = (n + 31) / 32;
-      const int i = lane * step;
-      const bool below = i < n && cum[lo + i] * p.Hkv <= u0;
-      const int last = 31 - __clz(__ballot_sync(0xffffffffu, below));
-      const int off = last * step;
-      lo += off;
-      n = min(step, n - off);
-    }
-    x = lo;
-    load();
-  }
-  __device__ __forceinline__ void load() {
-    t = tiles[FFTS_INDEX(x, p.max_tiles)];
-    base = cum[x] * p.Hkv;
-    next = cum[x + 1] * p.Hkv;
-    g = keys_of(t.pos0, t.ntok, p.window, p.sinks);
-  }
-  // The next segment with key tiles; false behind the share's end.
-  __device__ __forceinline__ bool segment() {
-    while (u < u1) {
-      if (u >= next) {
-        ++x;
-        load();
-      }
-      const int len = g.n + kOverhead;
-      const long long rem = u - base;
-      h = int(rem / len);
-      const int at = int(rem - (long long)h * len);
-      const int to = int(min((long long)len, at + (u1 - u)));
-      begin = u - at;
-      u += to - at;
-      j0 = max(0, at - kOverhead);
-      j1 = max(0, to - kOverhead);
-      if (j1 > j0) return true;
-    }
-    return false;
-  }
-};
-
-__device__ __forceinline__ uint64_t below(int k) { return k <= 0 ? 0ull : (k >= 64 ? ~0ull : (1ull << k) - 1ull); }
-
-template <typename E>
-struct Num;
-template <>
-struct Num<__nv_bfloat16> {
-  static constexpr uint32_t fmt = 1;
-  static constexpr CUtensorMapDataType map = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  // P <= 2^64 against the reference max: bf16 and the fp32 O have the exponents for it
-  static constexpr float rescale = 64.0f, pmax = 18446744073709551616.0f;
-  static __device__ __forceinline__ uint32_t pack(float a, float b) {
-    const __nv_bfloat162 r = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t *>(&r);
-  }
-};
-template <>
-struct Num<__half> {
-  static constexpr uint32_t fmt = 0;
-  static constexpr CUtensorMapDataType map = CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-  // fp16 ends at 65504: P <= 2^8 after a rescale, 2^14 (a tile's row sum) before the next one; the row's
-  // top has P >= 1, so what is lost below 2^-24 is that far under it
-  static constexpr float rescale = 8.0f, pmax = 16384.0f;
-  static __device__ __forceinline__ uint32_t pack(float a, float b) {
-    const __half2 r = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t *>(&r);
-  }
-};
-
-constexpr uint32_t idesc(uint32_t fmt, bool b_mn_major, int n) {
-  return (1u << 4) | (fmt << 7) | (fmt << 10) | (b_mn_major ? (1u << 16) : 0u) | (uint32_t(n >> 3) << 17) |
-         (uint32_t(kBM >> 4) << 24);
-}
-
-__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *map, uint32_t bar, int c0, int c1, int c2) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
-          dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
-      : "memory");
-}
-
 template <typename E, int D>
 __global__ void __launch_bounds__(kThreads, 2)
     attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
@@ -360,7 +98,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     tiles += int64_t(blockIdx.x) * p.max_tiles;
     cum += int64_t(blockIdx.x) * (p.max_tiles + 1);
     // the scratch lies where the K ring will be
-    ntiles = build_schedule<kThreads>(p, tiles, cum, *reinterpret_cast<SchedScratch<kThreads> *>(smem + Lay::k), &length);
+    ntiles = build_schedule<kBN, kThreads>(p, tiles, cum, *reinterpret_cast<SchedScratch<kThreads> *>(smem + Lay::k), &length);
   } else {
     ntiles = p.header[0];
     length = cum[FFTS_INDEX(ntiles, p.max_tiles + 1)];
@@ -406,7 +144,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   const uint32_t tmem = *tmem_slot;
   const uint32_t tm_o = tmem + kTmemO;
 
-  Walk w(p, tiles, cum);
+  Walk<kBN> w(p, tiles, cum);
   w.seek(u0, u1, ntiles);
 
   if (warp == 4) {
@@ -779,11 +517,11 @@ __device__ __forceinline__ void join_rows(const Params &p, uint16_t *dst, int r,
         ml[k] = make_float2(-INFINITY, 0.0f);
         if (sb + k <= s1) {
           const int64_t at = slot(sb + k);
-          ml[k] = __ldcg(&p.part_ml[at * kBM + r]);
-          const float4 *src = reinterpret_cast<const float4 *>(p.part) + at * (kBM * D / 4) + r;
+          ml[k] = __ldcg(&p.part_ml[at * p.rows + r]);
+          const float4 *src = reinterpret_cast<const float4 *>(p.part) + at * (p.rows * D / 4) + r;
 #pragma unroll
           for (int i = 0; i < CB; ++i)
-            if (c0 + i * step < D / 4) v[k][i] = __ldcg(src + (c0 + i * step) * kBM);
+            if (c0 + i * step < D / 4) v[k][i] = __ldcg(src + (c0 + i * step) * p.rows);
         }
       }
       float top = m;
@@ -837,19 +575,21 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
   const int s0 = int(blockIdx.x);
   const Cut cut = p.cuts[s0];
   if (cut.nrows == 0) return;
-  int rows = 1;
-  while (rows < cut.nrows) rows <<= 1;
-  const int r = int(threadIdx.x) % rows, per_block = kJoinThreads / rows;
+  int rows = 1;  // threads side by side on the rows
+  while (rows < cut.nrows && rows < kJoinThreads) rows <<= 1;
+  const int per_block = kJoinThreads / rows;
   const int q = int(blockIdx.y) * per_block + int(threadIdx.x) / rows, step = kJoinBlocks * per_block;
-  if (r >= cut.nrows || q >= D / 4) return;
-  const int tl = r / p.G, hg = r - tl * p.G;
-  if (!FFTS_IN_RANGE(cut.tok0 + tl, p.T)) return;
-  uint16_t *dst = p.out + int64_t(cut.tok0 + tl) * p.os_t + int64_t(cut.head0 + hg) * p.os_h;
-  // few rows: one or two pieces per thread and often many shares; many rows: the other way round
-  if (rows <= 16)
-    join_rows<E, D, 8, 1>(p, dst, r, q, step, s0, cut.s1, cut.first_slot);
-  else
-    join_rows<E, D, 2, 4>(p, dst, r, q, step, s0, cut.s1, cut.first_slot);
+  if (q >= D / 4) return;
+  for (int r = int(threadIdx.x) % rows; r < cut.nrows; r += rows) {
+    const int tl = r / p.G, hg = r - tl * p.G;
+    if (!FFTS_IN_RANGE(cut.tok0 + tl, p.T)) return;
+    uint16_t *dst = p.out + int64_t(cut.tok0 + tl) * p.os_t + int64_t(cut.head0 + hg) * p.os_h;
+    // few rows: one or two pieces per thread and often many shares; many rows: the other way round
+    if (rows <= 16)
+      join_rows<E, D, 8, 1>(p, dst, r, q, step, s0, cut.s1, cut.first_slot);
+    else
+      join_rows<E, D, 2, 4>(p, dst, r, q, step, s0, cut.s1, cut.first_slot);
+  }
 }
 
 // ---------------------------------------------------------------- host side
@@ -889,7 +629,7 @@ __device__ int g_status_sink;
 struct Space {
   int64_t max_tiles, cum, tiles, header, cuts, ml, part, bytes;
   Space(int64_t T, int64_t R, int64_t G, int64_t D) {
-    const int64_t tpt = kBM / G;
+    const int64_t tpt = kBM / G;  // of the smaller tiles; the larger ones are fewer
     max_tiles = T / tpt + std::min(R, T);  // sum of ceil(len / tpt)
     const int64_t copies = max_tiles <= kOwnTiles ? kMaxCtas : 1;
     cum = 0;
@@ -903,32 +643,37 @@ struct Space {
 };
 
 template <typename E, int D>
-static int launch(const Params &p, const void *q, const int64_t *qs, const void *k, const int64_t *ks, const void *v,
-                  const int64_t *vs, cudaStream_t stream) {
+static int launch(Params &p, bool chunks, const void *q, const int64_t *qs, const void *k, const int64_t *ks,
+                  const void *v, const int64_t *vs, cudaStream_t stream) {
   CUtensorMap mq, mk, mv;
   const cuuint64_t qd[3] = {D, cuuint64_t(p.H), cuuint64_t(p.T)};
   const cuuint64_t qst[2] = {cuuint64_t(qs[1]) * 2, cuuint64_t(qs[0]) * 2};
-  const cuuint32_t qbox[3] = {64, cuuint32_t(p.G), cuuint32_t(p.tpt)};
+  const cuuint32_t qbox[3] = {64, cuuint32_t(p.G), cuuint32_t(kBM / p.G)};
   int rc = encode(&mq, Num<E>::map, 3, q, qd, qst, qbox);
   if (rc) return rc;
   const cuuint64_t ps = 1ull << p.ps_shift;
   const cuuint64_t kd[4] = {D, ps, cuuint64_t(p.Hkv), cuuint64_t(p.n_pages)};
-  const cuuint32_t kbox[4] = {64, cuuint32_t(std::min<cuuint64_t>(ps, kBN)), 1, 1};
+  const cuuint32_t kbox[4] = {64, cuuint32_t(std::min<cuuint64_t>(ps, chunks ? 2 * kBN : kBN)), 1, 1};
   const cuuint64_t kst[3] = {cuuint64_t(ks[2]) * 2, cuuint64_t(ks[1]) * 2, cuuint64_t(ks[0]) * 2};
   const cuuint64_t vst[3] = {cuuint64_t(vs[2]) * 2, cuuint64_t(vs[1]) * 2, cuuint64_t(vs[0]) * 2};
   rc = encode(&mk, Num<E>::map, 4, k, kd, kst, kbox);
   if (!rc) rc = encode(&mv, Num<E>::map, 4, v, kd, vst, kbox);
-  if (!rc)
+  if (rc) return rc;
+  if (chunks) {
+    rc = launch_chunk(p, Num<E>::fmt == 0, D, mq, mk, mv, stream);
+    if (rc) return rc;
+  } else {
     rc = ensure_func_smem(reinterpret_cast<const void *>(&attn_kernel<E, D>), Layout<D>::bytes,
                           int(cudaSharedmemCarveoutMaxShared));
-  if (rc) return rc;
-  if (!p.own_schedule) {
-    schedule_kernel<<<1, kSchedThreads, 0, stream>>>(p);
+    if (rc) return rc;
+    if (!p.own_schedule) {
+      schedule_kernel<kBN><<<1, kSchedThreads, 0, stream>>>(p);
+      FFTS_CUDA(cudaGetLastError());
+    }
+    attn_kernel<E, D><<<unsigned(p.ctas), kThreads, Layout<D>::bytes, stream>>>(mq, mk, mv, p);
     FFTS_CUDA(cudaGetLastError());
   }
-  attn_kernel<E, D><<<unsigned(p.ctas), kThreads, Layout<D>::bytes, stream>>>(mq, mk, mv, p);
-  FFTS_CUDA(cudaGetLastError());
-  // launched while attn_kernel drains
+  // launched while the attention kernel drains
   cudaLaunchAttribute early{};
   early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   early.val.programmaticStreamSerializationAllowed = 1;
@@ -1013,7 +758,11 @@ int paged_attn(const void *q, const int64_t *qs, const void *k_pages, const int6
   if (!rc) rc = device_wait_cycles(kWaitSeconds, &p.wait_cycles);
   if (!rc) rc = device_wait_cycles(kDrainSeconds, &p.drain_cycles);
   if (rc) return rc;
-  p.ctas = std::min(2 * sms, kMaxCtas);
+  // Chunks of at least a 128-row tile on average: the larger tiles of paged_chunk.cu.
+  const bool chunks = T * G >= kBM * R;
+  p.ctas = std::min(chunks ? sms : 2 * sms, kMaxCtas / (chunks ? 2 : 1));
+  p.rows = chunks ? 2 * kBM : kBM;
+  if (chunks) p.tpt *= 2;
   if (status) {
     p.status = status;
   } else {
@@ -1022,10 +771,10 @@ int paged_attn(const void *q, const int64_t *qs, const void *k_pages, const int6
     p.status = static_cast<int *>(sink);
   }
   if (dtype == FFTS_DTYPE_BF16)
-    return D == 128 ? launch<__nv_bfloat16, 128>(p, q, qs, k_pages, ks, v_pages, vs, stream)
-                    : launch<__nv_bfloat16, 64>(p, q, qs, k_pages, ks, v_pages, vs, stream);
-  return D == 128 ? launch<__half, 128>(p, q, qs, k_pages, ks, v_pages, vs, stream)
-                  : launch<__half, 64>(p, q, qs, k_pages, ks, v_pages, vs, stream);
+    return D == 128 ? launch<__nv_bfloat16, 128>(p, chunks, q, qs, k_pages, ks, v_pages, vs, stream)
+                    : launch<__nv_bfloat16, 64>(p, chunks, q, qs, k_pages, ks, v_pages, vs, stream);
+  return D == 128 ? launch<__half, 128>(p, chunks, q, qs, k_pages, ks, v_pages, vs, stream)
+                  : launch<__half, 64>(p, chunks, q, qs, k_pages, ks, v_pages, vs, stream);
 }
 
 }  // namespace ffts

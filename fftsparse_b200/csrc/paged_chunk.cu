@@ -1,0 +1,537 @@
+// paged_chunk.cu -- the paged attention of paged_attn.cu for batches of longer chunks: tiles of 256 rows x 128 keys.
+//
+// Same schedule, shares and partials as paged_attn.cu.  Where a batch brings rows enough, what bounds it is
+// the tensor core, the exponentials and the traffic of K and V, and larger tiles ease all three:
+//   - A 64-key S = Q K^T reads 48 KB of shared memory for 256 clocks of products (the 128-row Q each
+//     time), more than the 128 bytes a clock that it gets; with 128 keys it is 64 KB for 512.
+//   - Two 128-row halves A and B of a q tile share every K and V tile, so half as many bytes are loaded per product.
+//   - The halves take turns: while A's softmax works on its S, the tensor core runs B's products.  With S, P and O of
+//     both halves the SM's 512 TMEM columns are full: one CTA per SM.
+//   - Of every eight exponentials kPoly pairs' worth are computed on the FMA pipe (2^x = 2^round(x) p(x - round(x)), p
+//     fitted to 2^f on [-1/2, 1/2] by least squares of the relative error), since the special function
+//     unit needs as many clocks for a tile as the tensor core.
+//
+// Roles (384 threads; registers are split for the softmax warps, which hold a row's 128 scores):
+//   warps 0-3 / 4-7  softmax of half A / B: thread r owns row r; P goes over the S columns already read.
+//   warp 8           producer: Q of each half, then K(0), V(0), K(1), ... through one five-stage ring.
+//   warps 10, 11     none (registers are split by warpgroup)
+//   warp 9           MMA issuer (one thread): S_A, S_B, then per key tile n: PV_A(n), S_A(n + 1), PV_B(n), S_B(n + 1).
+// A commit tracks all earlier products of the issuing thread, so S_X(n + 1) being there means that PV_X(n) is
+// complete: O may be rescaled then, and only a segment's end waits for its last PV.
+// Every wait is bounded.
+
+#include <algorithm>
+
+#include "paged_common.cuh"
+
+namespace ffts {
+namespace paged {
+
+constexpr int cBM = 128;       // rows of a half
+constexpr int cBN = 128;       // keys of a key tile
+constexpr int cThreads = 384;   // three warpgroups
+constexpr int cRegsSoftmax = 208, cRegsOther = 80;  // after the split; launched with 168 each, 2 * 208 + 80 <= 3 * 168
+constexpr int cStages = 5;
+constexpr int cTmemCols = 512;
+constexpr int kPoly = 1;       // of every 4 pairs of a row's scores, pairs whose exponentials are polynomials
+
+template <int D>
+struct ChunkLayout {
+  static constexpr int halves = D / 64;         // 64-channel swizzle boxes per row
+  static constexpr int box = 128 * 128;         // bytes of one box of 128 rows (or keys)
+  static constexpr int tile = halves * box;     // one half's Q, a K tile or a V tile
+  static constexpr int q = 0;
+  static constexpr int kv = q + 2 * tile;
+  static constexpr int bars = kv + cStages * tile;
+  static constexpr int nbars = 2 * cStages + 2 + 2 + 2 + 2 + 2 + 1;
+  static constexpr int tmem_slot = bars + nbars * 8;
+  static constexpr int abort = tmem_slot + 8;
+  static constexpr int bytes = abort + 8;
+  static_assert(bytes <= 227 * 1024, "one CTA must fit in an SM's shared memory");
+};
+
+constexpr int CKF = 0;              // ring stage loaded [cStages]
+constexpr int CKE = CKF + cStages;  // ring stage free   [cStages]
+constexpr int CQF = CKE + cStages;  // Q of half x loaded
+constexpr int CQE = CQF + 2;        // the segment's S products have read it
+constexpr int CSF = CQE + 2;        // S of half x
+constexpr int CPF = CSF + 2;        // P of half x written (128 arrivals)
+constexpr int COF = CPF + 2;        // O of half x final
+constexpr int CDRAIN = COF + 2;
+
+// 2^x of a pair by range reduction and a polynomial on the FMA pipe; x >= -126 after the clamp, so the
+// exponent field takes round(x) without a wrap.  Relative error 7.5e-5 (degree 3) or 2.6e-6 (degree 4).
+template <int kDegree>
+__device__ __forceinline__ float2 poly_exp2(float2 x) {
+  x.x = fmaxf(x.x, -126.0f);
+  x.y = fmaxf(x.y, -126.0f);
+  const float2 magic = make_float2(12582912.0f, 12582912.0f);  // 1.5 * 2^23: the sum's low bits are round(x)
+  const float2 t = __fadd2_rn(x, magic);
+  const float2 f = __fadd2_rn(x, __fmul2_rn(__fadd2_rn(t, make_float2(-12582912.0f, -12582912.0f)), make_float2(-1.0f, -1.0f)));
+  auto two = [](float c) { return make_float2(c, c); };
+  float2 y;
+  if (kDegree == 3) {
+    y = __ffma2_rn(two(0.05517164617776871f), f, two(0.2426111251115799f));
+    y = __ffma2_rn(y, f, two(0.6932609677314758f));
+    y = __ffma2_rn(y, f, two(0.9999280571937561f));
+  } else {
+    y = __ffma2_rn(two(0.009570099413394928f), f, two(0.05591785907745361f));
+    y = __ffma2_rn(y, f, two(0.240247443318367f));
+    y = __ffma2_rn(y, f, two(0.6931217908859253f));
+    y = __ffma2_rn(y, f, two(0.9999992847442627f));
+  }
+  y.x = __int_as_float(__float_as_int(y.x) + (__float_as_int(t.x) << 23));
+  y.y = __int_as_float(__float_as_int(y.y) + (__float_as_int(t.y) << 23));
+  return y;
+}
+
+template <typename E, int D>
+__global__ void __launch_bounds__(cThreads, 1)
+    chunk_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                 const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ Params p) {
+  using Lay = ChunkLayout<D>;
+  extern __shared__ __align__(16) uint8_t smem[];
+  if (smem_u32(smem) & 1023u) {  // SWIZZLE_128B tiles need 1024-byte alignment
+    if (threadIdx.x == 0) {
+      *reinterpret_cast<volatile int *>(p.status) = kErrSmemAlign;
+      p.cuts[blockIdx.x].nrows = 0;
+    }
+    return;
+  }
+  Tile *tiles = p.tiles;
+  long long *cum = p.cum;
+  int ntiles;
+  long long length;
+  if (p.own_schedule) {
+    tiles += int64_t(blockIdx.x) * p.max_tiles;
+    cum += int64_t(blockIdx.x) * (p.max_tiles + 1);
+    // the scratch lies where the ring will be
+    ntiles = build_schedule<cBN, cThreads>(p, tiles, cum, *reinterpret_cast<SchedScratch<cThreads> *>(smem + Lay::kv), &length);
+  } else {
+    ntiles = p.header[0];
+    length = cum[FFTS_INDEX(ntiles, p.max_tiles + 1)];
+  }
+  length *= p.Hkv;
+  const long long per = share_of(p, length);
+  const long long u0 = per * blockIdx.x, u1 = min(length, u0 + per);
+  if (u0 >= u1) {  // uniform in the CTA, before any allocation
+    if (threadIdx.x == 0) p.cuts[blockIdx.x].nrows = 0;
+    return;
+  }
+  const uint32_t sbase = smem_u32(smem);
+  auto bar = [&](int i) { return sbase + Lay::bars + 8u * uint32_t(i); };
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + Lay::abort);
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + Lay::tmem_slot);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int tph = cBM / p.G;        // tokens of a half
+  const int qrows = tph * p.G;      // rows of it that a Q load fills
+
+  if (threadIdx.x == 0) {
+    *abort_flag = 0;
+    for (int i = 0; i < Lay::nbars; ++i) mbar_init(bar(i), (i == CPF || i == CPF + 1) ? 128u : 1u);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  // rows no Q load fills: zeros, so that they stay finite
+  for (int i = threadIdx.x; i < 2 * (cBM - qrows) * 8 * Lay::halves; i += cThreads) {
+    const int at = i >> 3, hf = at % Lay::halves, row = qrows + (at / Lay::halves) % (cBM - qrows);
+    const int x = at / Lay::halves / (cBM - qrows);
+    *reinterpret_cast<uint4 *>(smem + Lay::q + x * Lay::tile + hf * Lay::box + row * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+  }
+  fence_proxy_async();  // TMA writes over the scratch, the MMAs read the zeros
+  if (warp == 9) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                 "r"(cTmemCols));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  if (warp == 8 && lane == 0) {
+    prefetch_map(&tm_q);
+    prefetch_map(&tm_k);
+    prefetch_map(&tm_v);
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = *tmem_slot;  // S_A, S_B (128 columns each), O_A, O_B
+
+  Walk<cBN> w(p, tiles, cum);
+  w.seek(u0, u1, ntiles);
+
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(cRegsOther));
+    if (warp == 8) {
+      // ============================================================ producer (whole warp)
+      const int ps = 1 << p.ps_shift;
+      const int box = min(ps, cBN);              // keys of one box
+      const int boxes = (cBN / box) * Lay::halves;
+      const int my_box = lane / Lay::halves, my_half = lane % Lay::halves;
+      const uint32_t my_dst = uint32_t(my_half * Lay::box + my_box * box * 128);
+      struct Load {
+        int page, row, h;
+      };
+      int j = 0, j1 = 0;
+      bool fresh = false;  // the fetched tile is its segment's first
+      auto fetch = [&](Load &l) -> bool {
+        fresh = j >= j1;
+        if (fresh) {
+          if (!w.segment()) return false;
+          j = w.j0;
+          j1 = w.j1;
+        }
+        const int c = key_tile(w.g, j) * cBN + my_box * box;  // first key of the box
+        ++j;
+        l.page = -1;
+        l.row = c & (ps - 1);
+        l.h = w.h;
+        if (lane < boxes && c < w.g.hi && (c + box > w.g.lo || c < p.sinks))
+          l.page = p.table[int64_t(w.t.r) * p.table_ld + FFTS_INDEX(c >> p.ps_shift, p.width)];
+        return true;
+      };
+      bool ok = true;
+      int nl = 0, nq[2] = {0, 0};  // loads issued
+      auto load = [&](const Load &l, const CUtensorMap *map) {
+        const int s = nl % cStages;
+        ok = ok && __all_sync(0xffffffffu, mbar_wait(bar(CKE + s), ((nl / cStages) & 1) ^ 1, abort_flag, p.wait_cycles));
+        if (!ok) return;
+        if (lane == 0) mbar_arrive_tx(bar(CKF + s), Lay::tile);
+        __syncwarp();
+        if (lane < boxes)
+          tma_load_4d(sbase + Lay::kv + s * Lay::tile + my_dst, map, bar(CKF + s), my_half * 64, l.row, l.h, l.page);
+        ++nl;
+      };
+      auto load_q = [&](int x, int tok0, int qh) {
+        ok = ok && __all_sync(0xffffffffu, mbar_wait(bar(CQE + x), (nq[x] & 1) ^ 1, abort_flag, p.wait_cycles));
+        if (!ok) return;
+        if (lane == 0) {
+          mbar_arrive_tx(bar(CQF + x), uint32_t(qrows * D * 2));
+          for (int hf = 0; hf < Lay::halves; ++hf)
+            tma_load_3d(sbase + Lay::q + x * Lay::tile + hf * Lay::box, &tm_q, bar(CQF + x), hf * 64, qh, tok0 + x * tph);
+        }
+        ++nq[x];
+      };
+      Load cur{};
+      bool more = fetch(cur);
+      while (more && ok) {
+        // the ring's order is the MMA issuer's: K(n), V(n).  Q waits for the last S of the segment before,
+        // whose K and V are all on their way by then.
+        const int tok0 = w.t.tok0, qh = w.h * p.G;
+        const bool first = fresh, two = w.t.ntok > tph;
+        load(cur, &tm_k);
+        if (first) {
+          load_q(0, tok0, qh);
+          if (two) load_q(1, tok0, qh);
+        }
+        Load next = cur;
+        more = fetch(next);  // its page numbers arrive while the stages fill
+        load(cur, &tm_v);
+        cur = next;
+      }
+      if (!ok) {
+        if (lane == 0) {
+          *abort_flag = 1;
+          *reinterpret_cast<volatile int *>(p.status) = kErrProducer;
+          // wait (bounded, ignoring the abort flag) for the copies in flight
+          volatile int never = 0;
+          for (int x = 0; x < 2; ++x)
+            if (nq[x] > 0) mbar_wait(bar(CQF + x), (nq[x] - 1) & 1, &never, p.drain_cycles);
+          for (int n = max(0, nl - cStages); n < nl; ++n)
+            mbar_wait(bar(CKF + n % cStages), (n / cStages) & 1, &never, p.drain_cycles);
+        }
+        __syncwarp();
+      }
+    } else if (warp == 9) {
+      // ============================================================ MMA issuer (one thread)
+      if (lane == 0) {
+        constexpr uint32_t idS = idesc(Num<E>::fmt, false, cBN), idPV = idesc(Num<E>::fmt, true, D);
+        const uint64_t dq0 = smem_desc(sbase + Lay::q, 16, 1024);
+        const uint64_t dk0 = smem_desc(sbase + Lay::kv, 16, 1024);
+        const uint64_t dv0 = smem_desc(sbase + Lay::kv, Lay::box, 1024);
+        bool ok = true;
+        int nl = 0;                  // ring loads consumed up to the current K
+        int np[2] = {0, 0}, nseg[2] = {0, 0};
+        auto full = [&](int n) { return mbar_wait(bar(CKF + n % cStages), (n / cStages) & 1, abort_flag, p.wait_cycles); };
+        auto issue_s = [&](int x, int stage) {
+          fence_after();
+          const uint64_t dq = dq0 + uint64_t((x * Lay::tile) >> 4), dk = dk0 + uint64_t((stage * Lay::tile) >> 4);
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint32_t off = (kk >> 2) * Lay::box + (kk & 3) * 32;
+            umma_f16(tmem + x * cBN, dq + (off >> 4), dk + (off >> 4), idS, kk > 0 ? 1u : 0u);
+          }
+          umma_commit(bar(CSF + x));
+        };
+        auto issue_pv = [&](int x, int stage, bool first) {
+          fence_after();
+          const uint64_t dv = dv0 + uint64_t((stage * Lay::tile) >> 4);
+#pragma unroll
+          for (int kk = 0; kk < cBN / 16; ++kk)
+            umma_f16_ts(tmem + 256 + x * 128, tmem + x * cBN + kk * 8, dv + uint64_t((kk * 2048) >> 4), idPV,
+                        (!first || kk > 0) ? 1u : 0u);
+        };
+        while (ok && w.segment()) {
+          const int n1 = w.j1 - w.j0;
+          const int halves = w.t.ntok > tph ? 2 : 1;
+          // S of the first key tile: K is load nl, V(n) load nl + 2 n + 1
+          for (int x = 0; x < halves && ok; ++x) {
+            ok = mbar_wait(bar(CQF + x), nseg[x] & 1, abort_flag, p.wait_cycles) && full(nl);
+            if (!ok) break;
+            ++nseg[x];
+            issue_s(x, nl % cStages);
+            if (n1 == 1) umma_commit(bar(CQE + x));
+          }
+          if (ok) umma_commit(bar(CKE + nl % cStages));
+          for (int n = 0; n < n1 && ok; ++n) {
+            const int kv = nl + 2 * n + 1, kn = kv + 1;
+            for (int x = 0; x < halves && ok; ++x) {
+              ok = full(kv) && mbar_wait(bar(CPF + x), np[x] & 1, abort_flag, p.wait_cycles);
+              if (!ok) break;
+              ++np[x];
+              issue_pv(x, kv % cStages, n == 0);
+              if (n + 1 == n1) umma_commit(bar(COF + x));
+              if (n + 1 < n1) {
+                ok = full(kn);
+                if (!ok) break;
+                issue_s(x, kn % cStages);
+                if (n + 2 == n1) umma_commit(bar(CQE + x));
+              }
+            }
+            if (!ok) break;
+            umma_commit(bar(CKE + kv % cStages));
+            if (n + 1 < n1) umma_commit(bar(CKE + kn % cStages));
+          }
+          nl += 2 * n1;
+        }
+        if (!ok) {
+          *abort_flag = 1;
+          *reinterpret_cast<volatile int *>(p.status) = kErrMma;
+        }
+        // wait (bounded) until every MMA this thread issued has completed
+        umma_commit(bar(CDRAIN));
+        volatile int never = 0;
+        mbar_wait(bar(CDRAIN), 0, &never, p.drain_cycles);
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(cRegsSoftmax));
+    // ============================================================ softmax (warps 0-3: half A, 4-7: half B)
+    const int x = warp >> 2;
+    const int r = threadIdx.x & 127;
+    const int tl = x * tph + min(r / p.G, tph - 1), hg = r % p.G;  // the row's token in the tile and head in the group
+    const int row = x * qrows + r;                                 // the tile's rows without the halves' gaps
+    const uint32_t lane_off = uint32_t((warp & 3) * 32) << 16;
+    const uint32_t s_addr = tmem + x * cBN + lane_off, o_addr = tmem + 256 + x * 128 + lane_off;
+    const float2 sc2 = make_float2(p.scale_log2, p.scale_log2);
+    bool ok = true, first_seg = true, noted = false;
+    int n = 0, nseg = 0, kvn = 0;  // S tiles and segments of this half, key tiles of the share so far
+    while (ok && w.segment()) {
+      const Keys g = w.g;
+      const int nrows = w.t.ntok * p.G;
+      const bool mine = w.t.ntok > x * tph;                      // this half has rows
+      const bool active = x * qrows + (warp & 3) * 32 < nrows && mine;  // this warp has
+      // rows of no token take the last token's mask; nobody reads them
+      const int pos = w.t.pos0 + min(tl, w.t.ntok - 1);
+      float m_ref = -INFINITY, l_run = 0.0f;
+      if (!mine) kvn += w.j1 - w.j0;
+      for (int j = w.j0; mine && j < w.j1; ++j, ++n, ++kvn) {
+        if (!__all_sync(0xffffffffu, mbar_wait(bar(CSF + x), n & 1, abort_flag, p.wait_cycles))) { ok = false; break; }
+        fence_after();
+        const int c0 = key_tile(g, j) * cBN;
+        if (x == 0 && (c0 + cBN > g.hi || (c0 < g.lo && c0 + cBN > p.sinks))) {
+          // V rows that no row sees, for both halves (A's product is issued before B's)
+          const int v = 2 * kvn + 1, stage = v % cStages;
+          if (!__all_sync(0xffffffffu, mbar_wait(bar(CKF + stage), (v / cStages) & 1, abort_flag, p.wait_cycles))) { ok = false; break; }
+          const int key = c0 + r;
+          if (key >= g.hi || (key < g.lo && key >= p.sinks)) {
+#pragma unroll
+            for (int hf = 0; hf < Lay::halves; ++hf)
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                *reinterpret_cast<uint4 *>(smem + Lay::kv + stage * Lay::tile + hf * Lay::box + r * 128 + i * 16) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async();
+        }
+        if (active) {
+          // whole: the row sees all keys of the tile
+          const int lim = pos + 1 - c0, from = p.window > 0 ? pos - p.window + 1 - c0 : 0, sink = p.sinks - c0;
+          const bool edge = __any_sync(0xffffffffu, lim < cBN || (from > 0 && sink < cBN));
+          float xs[cBN];
+          auto mask_chunk = [&](int c) {  // 32 columns; from and sink only matter with a window
+            const uint64_t m = (below(lim - 32 * c) & (p.window > 0 ? ~below(from - 32 * c) | below(sink - 32 * c) : ~0ull));
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (!((uint32_t(m) >> e) & 1u)) xs[c * 32 + e] = -INFINITY;
+          };
+          float2 rs2[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+          auto exp_chunk = [&](int c, float2 off2, bool poly) {
+            uint32_t pk[16];
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              const float2 a = __ffma2_rn(make_float2(xs[c * 32 + e], xs[c * 32 + e + 1]), sc2, off2);
+              float2 ex;
+              if (poly && (e >> 1) % 4 < kPoly) {
+                ex = poly_exp2<Num<E>::degree>(a);
+              } else {
+                ex.x = fast_exp2(a.x);
+                ex.y = fast_exp2(a.y);
+              }
+              rs2[(e >> 1) & 1] = __fadd2_rn(rs2[(e >> 1) & 1], ex);
+              pk[e >> 1] = Num<E>::pack(ex.x, ex.y);
+            }
+            tmem_st16u(s_addr + c * 16, pk);
+          };
+          // The common path takes m_ref as it stands and keeps the result when every P of the row is small
+          // enough (by the tile's row sum); a row's first tile with a key, or one that outgrows
+          // m_ref, takes the max path: new m_ref, O and l rescaled, P again.
+          float alpha = 1.0f;
+          bool fast = !__any_sync(0xffffffffu, m_ref == -INFINITY);
+          tmem_ld32(s_addr, xs);
+          tmem_wait_ld();
+          if (fast && !edge) {
+            const float moff = m_ref * p.scale_log2;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              if (c < 3) tmem_ld32(s_addr + 32 * (c + 1), xs + 32 * (c + 1));  // lands while this chunk is worked on
+              exp_chunk(c, make_float2(-moff, -moff), true);
+              if (c < 3) tmem_wait_ld();
+            }
+            const float tsum = (rs2[0].x + rs2[0].y) + (rs2[1].x + rs2[1].y);
+            if (__any_sync(0xffffffffu, !(tsum <= Num<E>::pmax))) {
+              fast = false;
+              tmem_wait_st();  // the max path below rewrites P
+              rs2[0] = rs2[1] = make_float2(0.0f, 0.0f);
+            }
+          } else {
+            fast = false;
+#pragma unroll
+            for (int c = 1; c < 4; ++c) tmem_ld32(s_addr + 32 * c, xs + 32 * c);
+            tmem_wait_ld();
+            if (edge) {
+#pragma unroll
+              for (int c = 0; c < 4; ++c) mask_chunk(c);
+            }
+          }
+          if (!fast) {
+            float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int c = 0; c < cBN; c += 2) mx4[(c >> 1) & 3] = max3f(mx4[(c >> 1) & 3], xs[c], xs[c + 1]);
+            const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+            if (mx > m_ref && (m_ref == -INFINITY || (mx - m_ref) * p.scale_log2 > Num<E>::rescale)) {
+              alpha = m_ref == -INFINITY ? 0.0f : fast_exp2((m_ref - mx) * p.scale_log2);
+              m_ref = mx;
+            }
+            const float moff = (m_ref == -INFINITY ? 0.0f : m_ref) * p.scale_log2;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) exp_chunk(c, make_float2(-moff, -moff), false);
+          }
+          const float2 rsum = __fadd2_rn(rs2[0], rs2[1]);
+          l_run = l_run * alpha + (rsum.x + rsum.y);
+          tmem_wait_st();
+          if (j > w.j0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
+            // O holds PV(n - 1): S(n) was issued after it and is there
+#pragma unroll 1
+            for (int c = 0; c < D / 32; ++c) {
+              float o[32];
+              tmem_ld32(o_addr + c * 32, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; e += 2) {
+                const float2 v = __fmul2_rn(make_float2(o[e], o[e + 1]), make_float2(alpha, alpha));
+                o[e] = v.x;
+                o[e + 1] = v.y;
+              }
+              tmem_st32(o_addr + c * 32, o);
+            }
+            tmem_wait_st();
+          }
+        }
+        fence_before();
+        mbar_arrive(bar(CPF + x));
+      }
+      if (!ok) break;
+      if (mine) {
+        if (!__all_sync(0xffffffffu, mbar_wait(bar(COF + x), nseg & 1, abort_flag, p.wait_cycles))) { ok = false; break; }
+        ++nseg;
+        fence_after();
+      }
+      const int slot = 2 * int(blockIdx.x) + (first_seg ? 0 : 1);
+      if (active) {
+        const bool whole = w.j0 == 0 && w.j1 == g.n;
+        const bool live = r < qrows && row < nrows;
+        const float inv_l = l_run > 0.0f ? 1.0f / l_run : 0.0f;
+        uint16_t *dst = p.out + int64_t(w.t.tok0 + tl) * p.os_t + int64_t(w.h * p.G + hg) * p.os_h;
+        float4 *pd = reinterpret_cast<float4 *>(p.part) + int64_t(slot) * (2 * cBM * D / 4) + row;
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          float o[32];
+          __syncwarp();
+          tmem_ld32(o_addr + c * 32, o);
+          tmem_wait_ld();
+          if (live && whole && FFTS_IN_RANGE(w.t.tok0 + tl, p.T)) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              uint32_t v[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                v[e] = Num<E>::pack(l_run > 0.0f ? o[q * 8 + 2 * e] * inv_l : 0.0f,
+                                    l_run > 0.0f ? o[q * 8 + 2 * e + 1] * inv_l : 0.0f);
+              *reinterpret_cast<uint4 *>(dst + c * 32 + q * 8) = make_uint4(v[0], v[1], v[2], v[3]);
+            }
+          }
+          if (live && !whole && FFTS_IN_RANGE(slot, 2 * p.ctas)) {
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+              pd[(c * 8 + q) * (2 * cBM)] = make_float4(o[q * 4], o[q * 4 + 1], o[q * 4 + 2], o[q * 4 + 3]);
+          }
+        }
+        if (live && !whole && FFTS_IN_RANGE(slot, 2 * p.ctas))
+          p.part_ml[int64_t(slot) * (2 * cBM) + row] = make_float2(m_ref * p.scale_log2, l_run);
+      }
+      // the share that holds the first key tile leaves a note for the join
+      if (w.j0 == 0 && w.j1 < g.n && threadIdx.x == 0 && FFTS_IN_RANGE(blockIdx.x, p.ctas)) {
+        Cut cut;
+        cut.tok0 = w.t.tok0;
+        cut.nrows = nrows;
+        cut.head0 = w.h * p.G;
+        cut.s1 = int((w.begin + kOverhead + g.n - 1) / per);
+        cut.first_slot = slot;
+        p.cuts[blockIdx.x] = cut;
+        noted = true;
+      }
+      first_seg = false;
+    }
+    if (threadIdx.x == 0 && !noted) p.cuts[blockIdx.x].nrows = 0;
+    if (!ok) {
+      *abort_flag = 1;
+      *reinterpret_cast<volatile int *>(p.status) = kErrSoftmax;
+    }
+  }
+
+  fence_before();
+  __syncthreads();
+  fence_after();
+  if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cTmemCols));
+}
+
+template <typename E, int D>
+static int launch(const Params &p, const CUtensorMap &mq, const CUtensorMap &mk, const CUtensorMap &mv,
+                  cudaStream_t stream) {
+  const int rc = ensure_func_smem(reinterpret_cast<const void *>(&chunk_kernel<E, D>), ChunkLayout<D>::bytes,
+                                  int(cudaSharedmemCarveoutMaxShared));
+  if (rc) return rc;
+  if (!p.own_schedule) {
+    schedule_kernel<cBN><<<1, kSchedThreads, 0, stream>>>(p);
+    FFTS_CUDA(cudaGetLastError());
+  }
+  chunk_kernel<E, D><<<unsigned(p.ctas), cThreads, ChunkLayout<D>::bytes, stream>>>(mq, mk, mv, p);
+  FFTS_CUDA(cudaGetLastError());
+  return FFTS_OK;
+}
+
+int launch_chunk(const Params &p, bool half, int D, const CUtensorMap &mq, const CUtensorMap &mk, const CUtensorMap &mv,
+                 cudaStream_t stream) {
+  if (half) return D == 128 ? launch<__half, 128>(p, mq, mk, mv, stream) : launch<__half, 64>(p, mq, mk, mv, stream);
+  return D == 128 ? launch<__nv_bfloat16, 128>(p, mq, mk, mv, stream)
+                  : launch<__nv_bfloat16, 64>(p, mq, mk, mv, stream);
+}
+
+}  // namespace paged
+}  // namespace ffts

@@ -4,9 +4,10 @@ Tolerances, with u = finfo(dtype).eps / 2 the relative size of one rounding:
   rope_append      u |y| for the result's rounding, plus (|a| + |b|) 2^-20 for the fp32 cos and sin (their
                    argument is a fraction of a turn, exact to 2^-25), products and sum, plus the dtype's smallest step
   paged_attention  u |o| for the result's rounding; u A with A = sum p |v| for the rounding of every p (the divisor
-                   sums them unrounded); A e with e = 2 ((D + 2) 2^-23 S + 2^-20) for the scores' fp32
+                   sums them unrounded); A e with e = 2 ((D + 2) 2^-23 S + a) for the scores' fp32
                    products (S the largest sum |q k| scale) through the exponential, both in numerator and
-                   divisor, and its own approximation; keys 2^-24 max |v| for the p that fp16 flushes
+                   divisor, and its approximation a (2^-13 with bf16, 2^-18 with fp16: the larger tiles take part of the exponentials
+                   from a polynomial of relative error 7.5e-5 and 2.6e-6, in p and in the divisor); keys 2^-24 max |v| for the p that fp16 flushes
 """
 import math
 import random
@@ -264,7 +265,7 @@ class Batch:
                     seen &= (j > i - self.window) | (j < self.sinks)
                 p = s.masked_fill(~seen, -math.inf).softmax(-1)
                 want, A = (p @ x for x in (v, v.abs()))
-                e = 2 * ((self.D + 2) * 2.0 ** -23 * S + 2.0 ** -20)
+                e = 2 * ((self.D + 2) * 2.0 ** -23 * S + (2.0 ** -13 if self.dt == BF else 2.0 ** -18))
                 tol = u * want.abs() + (u + e) * A
                 if self.dt == FP:
                     tol = tol + (c + n) * 2.0 ** -24 * float(v.abs().max())

@@ -47,6 +47,8 @@ constexpr int kThreads = 192;
 constexpr int kKStages = 3, kVStages = 2;
 constexpr int kTmemCols = 256;  // S0, S1 (64 columns each), O (D): two CTAs fill an SM's 512
 constexpr uint32_t kTmemO = 128;
+constexpr int kOverhead = 3;    // of 2, 3 and 4: 16 ragged chunks 67, 59, 57 us, 64 decoding requests 155.4, 155.8, 157.4 us
+constexpr int64_t kLongKeys = 16384;
 constexpr double kWaitSeconds = 2.0, kDrainSeconds = 4.0;
 
 template <int D>
@@ -230,11 +232,12 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
   } else if (warp == 5) {
     // ============================================================ MMA issuer (one thread)
-    if (lane == 0) {
+    if (elect_one()) {
       constexpr uint32_t idS = idesc(Num<E>::fmt, false, kBN), idPV = idesc(Num<E>::fmt, true, D);
-      const uint64_t dq = smem_desc(sbase + Lay::q, 16, 1024);
-      const uint64_t dk0 = smem_desc(sbase + Lay::k, 16, 1024);
-      const uint64_t dv0 = smem_desc(sbase + Lay::v, Lay::kv_half, 1024);
+      const uint64_t dk_ = smem_desc(sbase, 16, 1024), dv_ = smem_desc(sbase, Lay::kv_half, 1024);
+      const uint32_t dk_hi = uint32_t(dk_ >> 32), dv_hi = uint32_t(dv_ >> 32);
+      const uint32_t dq = uint32_t(dk_) + (Lay::q >> 4), dk0 = uint32_t(dk_) + (Lay::k >> 4),
+                     dv0 = uint32_t(dv_) + (Lay::v >> 4);
       bool ok = true;
       // S runs up to two tiles ahead of PV.  s_left: S tiles left in the walked segment; the PV side
       // needs only to know which tiles begin a segment (bit n % 32 of firsts).
@@ -256,13 +259,13 @@ __global__ void __launch_bounds__(kThreads, 2)
           ok = mbar_wait(bar(BKF + ks), (s / kKStages) & 1, abort_flag, p.wait_cycles);
           if (!ok) break;
           fence_after();
-          const uint64_t dk = dk0 + uint64_t((ks * Lay::kv_bytes) >> 4);
+          const uint32_t dk = dk0 + ((ks * Lay::kv_bytes) >> 4);
           const uint32_t td = tmem + (s & 1) * kBN;
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk) {
-            const uint32_t qoff = (kk >> 2) * Lay::q_half + (kk & 3) * 32;
-            const uint32_t koff = (kk >> 2) * Lay::kv_half + (kk & 3) * 32;
-            umma_f16(td, dq + (qoff >> 4), dk + (koff >> 4), idS, kk > 0 ? 1u : 0u);
+            const uint32_t qoff = ((kk >> 2) * Lay::q_half + (kk & 3) * 32) >> 4;
+            const uint32_t koff = ((kk >> 2) * Lay::kv_half + (kk & 3) * 32) >> 4;
+            umma_ss(td, dq + qoff, dk_hi, dk + koff, dk_hi, idS, kk > 0);
           }
           umma_commit(bar(BSF + (s & 1)));
           umma_commit(bar(BKE + ks));
@@ -280,11 +283,11 @@ __global__ void __launch_bounds__(kThreads, 2)
         if (!ok) break;
         fence_after();
         const bool first = (firsts >> (n & 31)) & 1u;
-        const uint64_t dv = dv0 + uint64_t((b * Lay::kv_bytes) >> 4);
+        const uint32_t dv = dv0 + ((b * Lay::kv_bytes) >> 4);
         const uint32_t pt = tmem + b * kBN;  // P(n): pairs in the first 32 columns of S buffer n % 2
 #pragma unroll
         for (int kk = 0; kk < kBN / 16; ++kk)
-          umma_f16_ts(tm_o, pt + kk * 8, dv + uint64_t((kk * 2048) >> 4), idPV, (!first || kk > 0) ? 1u : 0u);
+          umma_ts(tm_o, pt + kk * 8, dv + ((kk * 2048) >> 4), dv_hi, idPV, !first || kk > 0);
         umma_commit(bar(BPV + b));
       }
       if (!ok) {
@@ -475,7 +478,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         cut.tok0 = w.t.tok0;
         cut.nrows = nrows;
         cut.head0 = w.h * p.G;
-        cut.s1 = int((w.begin + kOverhead + g.n - 1) / per);
+        cut.s1 = int((u0 + w.begin + p.overhead + g.n - 1) / per);
         cut.first_slot = 2 * int(blockIdx.x) + (first_seg ? 0 : 1);
         p.cuts[blockIdx.x] = cut;
         noted = true;
@@ -503,7 +506,9 @@ __global__ void __launch_bounds__(kThreads, 2)
 template <typename E, int D, int PB, int CB>
 __device__ __forceinline__ void join_rows(const Params &p, uint16_t *dst, int r, int q, int step, int s0,
                                           int s1, int first_slot) {
-  auto slot = [&](int s) { return int64_t(FFTS_INDEX(s == s0 ? first_slot : 2 * s, 2 * p.ctas)); };
+  // in 32 bits: a slot has at most 256 rows of 32 pieces, and there are at most 1024
+  auto slot = [&](int s) { return uint32_t(FFTS_INDEX(s == s0 ? first_slot : 2 * s, 2 * p.ctas)); };
+  const float4 *part = reinterpret_cast<const float4 *>(p.part);
   for (int c0 = q; c0 < D / 4; c0 += CB * step) {
     float4 acc[CB];
 #pragma unroll
@@ -516,12 +521,11 @@ __device__ __forceinline__ void join_rows(const Params &p, uint16_t *dst, int r,
       for (int k = 0; k < PB; ++k) {
         ml[k] = make_float2(-INFINITY, 0.0f);
         if (sb + k <= s1) {
-          const int64_t at = slot(sb + k);
+          const uint32_t at = slot(sb + k);
           ml[k] = __ldcg(&p.part_ml[at * p.rows + r]);
-          const float4 *src = reinterpret_cast<const float4 *>(p.part) + at * (p.rows * D / 4) + r;
 #pragma unroll
           for (int i = 0; i < CB; ++i)
-            if (c0 + i * step < D / 4) v[k][i] = __ldcg(src + (c0 + i * step) * p.rows);
+            if (c0 + i * step < D / 4) v[k][i] = __ldcg(part + ((at * (D / 4) + c0 + i * step) * p.rows + r));
         }
       }
       float top = m;
@@ -567,10 +571,10 @@ __device__ __forceinline__ void join_rows(const Params &p, uint16_t *dst, int r,
 // Block (s0, y): the (q tile, head) that share s0 begins; the pieces of a row go round the blocks of y and
 // the threads that its rows leave.
 constexpr int kJoinThreads = 128;
-constexpr int kJoinBlocks = 4;
+constexpr int kJoinBlocks = 16;
 
 template <typename E, int D>
-__global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(kJoinThreads, 8) join_kernel(const __grid_constant__ Params p) {
   asm volatile("griddepcontrol.wait;" ::: "memory");  // launched early: attn_kernel's stores are visible from here
   const int s0 = int(blockIdx.x);
   const Cut cut = p.cuts[s0];
@@ -586,9 +590,9 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
     uint16_t *dst = p.out + int64_t(cut.tok0 + tl) * p.os_t + int64_t(cut.head0 + hg) * p.os_h;
     // few rows: one or two pieces per thread and often many shares; many rows: the other way round
     if (rows <= 16)
-      join_rows<E, D, 8, 1>(p, dst, r, q, step, s0, cut.s1, cut.first_slot);
+      join_rows<E, D, 4, 1>(p, dst, r, q, step, s0, cut.s1, cut.first_slot);
     else
-      join_rows<E, D, 2, 4>(p, dst, r, q, step, s0, cut.s1, cut.first_slot);
+      join_rows<E, D, 2, 2>(p, dst, r, q, step, s0, cut.s1, cut.first_slot);
   }
 }
 
@@ -710,6 +714,9 @@ int paged_attn(const void *q, const int64_t *qs, const void *k_pages, const int6
   FFTS_REQUIRE(T <= (int64_t(1) << 30) && R <= (int64_t(1) << 30) && H <= 65536 && n_pages < (int64_t(1) << 31) &&
                    width >= 0 && width * page_size <= (int64_t(1) << 30),
                "paged_attn: shape too large (a table row spans at most 2^30 tokens)");
+  FFTS_REQUIRE(Hkv * (ceil_div(width * page_size, kBN) + kOverhead) < (int64_t(1) << 31),
+               "paged_attn: %lld KV heads over a table row of %lld tokens are too many", (long long)Hkv,
+               (long long)(width * page_size));
   FFTS_REQUIRE(window >= 0 && sinks >= 0, "paged_attn: window and sinks must not be negative");
   FFTS_REQUIRE(scale > 0.0f && scale < 3.0e38f, "paged_attn: scale must be positive and finite");
   if (T == 0 || R == 0) return FFTS_OK;
@@ -758,11 +765,16 @@ int paged_attn(const void *q, const int64_t *qs, const void *k_pages, const int6
   if (!rc) rc = device_wait_cycles(kWaitSeconds, &p.wait_cycles);
   if (!rc) rc = device_wait_cycles(kDrainSeconds, &p.drain_cycles);
   if (rc) return rc;
-  // Chunks of at least a 128-row tile on average: the larger tiles of paged_chunk.cu.
-  const bool chunks = T * G >= kBM * R;
+  // The larger tiles of paged_chunk.cu: where requests fill them on average and their key lists, as far as the table and
+  // the window bound them, are long enough to pay for filling and draining one pipeline per SM instead of two.
+  // 2048 tokens of 32 / 8 heads over 32768 cached: 1.19 ms against 1.37 (0.98 and 1.11 before the power cap sets
+  // in); 512 over 16384: 129 us both; 16 ragged chunks over up to 16384: 72 against 59.
+  const int64_t span = window > 0 ? std::min(width * page_size, p.window + p.sinks + T / R) : width * page_size;
+  const bool chunks = T * G >= 2 * kBM * R && span > kLongKeys;
   p.ctas = std::min(chunks ? sms : 2 * sms, kMaxCtas / (chunks ? 2 : 1));
   p.rows = chunks ? 2 * kBM : kBM;
   if (chunks) p.tpt *= 2;
+  p.overhead = kOverhead;
   if (status) {
     p.status = status;
   } else {

@@ -7,15 +7,13 @@
 //   - Two 128-row halves A and B of a q tile share every K and V tile, so half as many bytes are loaded per product.
 //   - The halves take turns: while A's softmax works on its S, the tensor core runs B's products.  With S, P and O of
 //     both halves the SM's 512 TMEM columns are full: one CTA per SM.
-//   - Of every eight exponentials kPoly pairs' worth are computed on the FMA pipe (2^x = 2^round(x) p(x - round(x)), p
-//     fitted to 2^f on [-1/2, 1/2] by least squares of the relative error), since the special function
-//     unit needs as many clocks for a tile as the tensor core.
 //
 // Roles (384 threads; registers are split for the softmax warps, which hold a row's 128 scores):
 //   warps 0-3 / 4-7  softmax of half A / B: thread r owns row r; P goes over the S columns already read.
 //   warp 8           producer: Q of each half, then K(0), V(0), K(1), ... through one five-stage ring.
 //   warps 10, 11     none (registers are split by warpgroup)
 //   warp 9           MMA issuer (one thread): S_A, S_B, then per key tile n: PV_A(n), S_A(n + 1), PV_B(n), S_B(n + 1).
+//                    The product of a half's first 64 keys starts while the exponentials of the others are computed.
 // A commit tracks all earlier products of the issuing thread, so S_X(n + 1) being there means that PV_X(n) is
 // complete: O may be rescaled then, and only a segment's end waits for its last PV.
 // Every wait is bounded.
@@ -33,7 +31,6 @@ constexpr int cThreads = 384;   // three warpgroups
 constexpr int cRegsSoftmax = 208, cRegsOther = 80;  // after the split; launched with 168 each, 2 * 208 + 80 <= 3 * 168
 constexpr int cStages = 5;
 constexpr int cTmemCols = 512;
-constexpr int kPoly = 1;       // of every 4 pairs of a row's scores, pairs whose exponentials are polynomials
 
 template <int D>
 struct ChunkLayout {
@@ -43,7 +40,7 @@ struct ChunkLayout {
   static constexpr int q = 0;
   static constexpr int kv = q + 2 * tile;
   static constexpr int bars = kv + cStages * tile;
-  static constexpr int nbars = 2 * cStages + 2 + 2 + 2 + 2 + 2 + 1;
+  static constexpr int nbars = 2 * cStages + 2 + 2 + 2 + 4 + 2 + 1;
   static constexpr int tmem_slot = bars + nbars * 8;
   static constexpr int abort = tmem_slot + 8;
   static constexpr int bytes = abort + 8;
@@ -55,35 +52,9 @@ constexpr int CKE = CKF + cStages;  // ring stage free   [cStages]
 constexpr int CQF = CKE + cStages;  // Q of half x loaded
 constexpr int CQE = CQF + 2;        // the segment's S products have read it
 constexpr int CSF = CQE + 2;        // S of half x
-constexpr int CPF = CSF + 2;        // P of half x written (128 arrivals)
-constexpr int COF = CPF + 2;        // O of half x final
+constexpr int CPF = CSF + 2;        // P of half x written for the first and last 64 keys (128 arrivals) [2 x + part]
+constexpr int COF = CPF + 4;        // O of half x final
 constexpr int CDRAIN = COF + 2;
-
-// 2^x of a pair by range reduction and a polynomial on the FMA pipe; x >= -126 after the clamp, so the
-// exponent field takes round(x) without a wrap.  Relative error 7.5e-5 (degree 3) or 2.6e-6 (degree 4).
-template <int kDegree>
-__device__ __forceinline__ float2 poly_exp2(float2 x) {
-  x.x = fmaxf(x.x, -126.0f);
-  x.y = fmaxf(x.y, -126.0f);
-  const float2 magic = make_float2(12582912.0f, 12582912.0f);  // 1.5 * 2^23: the sum's low bits are round(x)
-  const float2 t = __fadd2_rn(x, magic);
-  const float2 f = __fadd2_rn(x, __fmul2_rn(__fadd2_rn(t, make_float2(-12582912.0f, -12582912.0f)), make_float2(-1.0f, -1.0f)));
-  auto two = [](float c) { return make_float2(c, c); };
-  float2 y;
-  if (kDegree == 3) {
-    y = __ffma2_rn(two(0.05517164617776871f), f, two(0.2426111251115799f));
-    y = __ffma2_rn(y, f, two(0.6932609677314758f));
-    y = __ffma2_rn(y, f, two(0.9999280571937561f));
-  } else {
-    y = __ffma2_rn(two(0.009570099413394928f), f, two(0.05591785907745361f));
-    y = __ffma2_rn(y, f, two(0.240247443318367f));
-    y = __ffma2_rn(y, f, two(0.6931217908859253f));
-    y = __ffma2_rn(y, f, two(0.9999992847442627f));
-  }
-  y.x = __int_as_float(__float_as_int(y.x) + (__float_as_int(t.x) << 23));
-  y.y = __int_as_float(__float_as_int(y.y) + (__float_as_int(t.y) << 23));
-  return y;
-}
 
 template <typename E, int D>
 __global__ void __launch_bounds__(cThreads, 1)
@@ -128,7 +99,7 @@ __global__ void __launch_bounds__(cThreads, 1)
 
   if (threadIdx.x == 0) {
     *abort_flag = 0;
-    for (int i = 0; i < Lay::nbars; ++i) mbar_init(bar(i), (i == CPF || i == CPF + 1) ? 128u : 1u);
+    for (int i = 0; i < Lay::nbars; ++i) mbar_init(bar(i), (i >= CPF && i < CPF + 4) ? 128u : 1u);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   // rows no Q load fills: zeros, so that they stay finite
@@ -240,65 +211,83 @@ __global__ void __launch_bounds__(cThreads, 1)
       }
     } else if (warp == 9) {
       // ============================================================ MMA issuer (one thread)
-      if (lane == 0) {
+      if (elect_one()) {
         constexpr uint32_t idS = idesc(Num<E>::fmt, false, cBN), idPV = idesc(Num<E>::fmt, true, D);
-        const uint64_t dq0 = smem_desc(sbase + Lay::q, 16, 1024);
-        const uint64_t dk0 = smem_desc(sbase + Lay::kv, 16, 1024);
-        const uint64_t dv0 = smem_desc(sbase + Lay::kv, Lay::box, 1024);
+        const uint64_t dk_ = smem_desc(sbase, 16, 1024), dv_ = smem_desc(sbase, Lay::box, 1024);
+        const uint32_t dk_hi = uint32_t(dk_ >> 32), dv_hi = uint32_t(dv_ >> 32);
+        const uint32_t dq_lo = uint32_t(dk_) + (Lay::q >> 4), dk_lo = uint32_t(dk_) + (Lay::kv >> 4),
+                       dv_lo = uint32_t(dv_) + (Lay::kv >> 4);
         bool ok = true;
         int nl = 0;                  // ring loads consumed up to the current K
         int np[2] = {0, 0}, nseg[2] = {0, 0};
         auto full = [&](int n) { return mbar_wait(bar(CKF + n % cStages), (n / cStages) & 1, abort_flag, p.wait_cycles); };
         auto issue_s = [&](int x, int stage) {
           fence_after();
-          const uint64_t dq = dq0 + uint64_t((x * Lay::tile) >> 4), dk = dk0 + uint64_t((stage * Lay::tile) >> 4);
+          const uint32_t dq = dq_lo + ((x * Lay::tile) >> 4), dk = dk_lo + ((stage * Lay::tile) >> 4);
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk) {
-            const uint32_t off = (kk >> 2) * Lay::box + (kk & 3) * 32;
-            umma_f16(tmem + x * cBN, dq + (off >> 4), dk + (off >> 4), idS, kk > 0 ? 1u : 0u);
+            const uint32_t off = ((kk >> 2) * Lay::box + (kk & 3) * 32) >> 4;
+            umma_ss(tmem + x * cBN, dq + off, dk_hi, dk + off, dk_hi, idS, kk > 0);
           }
           umma_commit(bar(CSF + x));
         };
-        auto issue_pv = [&](int x, int stage, bool first) {
+        auto issue_pv = [&](int x, int stage, int part, bool first) {
           fence_after();
-          const uint64_t dv = dv0 + uint64_t((stage * Lay::tile) >> 4);
+          const uint32_t dv = dv_lo + ((stage * Lay::tile) >> 4) + part * ((4 * 2048) >> 4);
 #pragma unroll
-          for (int kk = 0; kk < cBN / 16; ++kk)
-            umma_f16_ts(tmem + 256 + x * 128, tmem + x * cBN + kk * 8, dv + uint64_t((kk * 2048) >> 4), idPV,
-                        (!first || kk > 0) ? 1u : 0u);
+          for (int kk = 0; kk < cBN / 32; ++kk)
+            umma_ts(tmem + 256 + x * 128, tmem + x * cBN + part * 32 + kk * 8, dv + ((kk * 2048) >> 4), dv_hi, idPV,
+                    !first || kk > 0);
         };
-        while (ok && w.segment()) {
-          const int n1 = w.j1 - w.j0;
-          const int halves = w.t.ntok > tph ? 2 : 1;
-          // S of the first key tile: K is load nl, V(n) load nl + 2 n + 1
-          for (int x = 0; x < halves && ok; ++x) {
-            ok = mbar_wait(bar(CQF + x), nseg[x] & 1, abort_flag, p.wait_cycles) && full(nl);
-            if (!ok) break;
-            ++nseg[x];
-            issue_s(x, nl % cStages);
-            if (n1 == 1) umma_commit(bar(CQE + x));
-          }
-          if (ok) umma_commit(bar(CKE + nl % cStages));
-          for (int n = 0; n < n1 && ok; ++n) {
-            const int kv = nl + 2 * n + 1, kn = kv + 1;
-            for (int x = 0; x < halves && ok; ++x) {
-              ok = full(kv) && mbar_wait(bar(CPF + x), np[x] & 1, abort_flag, p.wait_cycles);
+        // S of half x for the key tile whose K is load kn; a segment's first one needs its Q, its last one frees it
+        auto next_s = [&](int x, int kn, bool first, bool last) {
+          ok = full(kn) && (!first || mbar_wait(bar(CQF + x), nseg[x] & 1, abort_flag, p.wait_cycles));
+          if (!ok) return;
+          nseg[x] += first;
+          issue_s(x, kn % cStages);
+          if (last) umma_commit(bar(CQE + x));
+        };
+        int n1 = 0, halves = 0;  // the segment's key tiles and halves
+        auto segment = [&]() {
+          const bool more = w.segment();
+          n1 = more ? w.j1 - w.j0 : 0;
+          halves = more ? (w.t.ntok > tph ? 2 : 1) : 0;
+        };
+        segment();
+        for (int x = 0; x < halves && ok; ++x) next_s(x, 0, true, n1 == 1);
+        if (ok && halves > 0) umma_commit(bar(CKE));
+        for (int n = 0; halves > 0 && ok;) {
+          // PV of key tile n and S of the one behind it, which may be the next segment's first: then a half's S
+          // goes ahead of the other half's PV only if its Q is there
+          const int now = halves, kv = nl + 1, kn = nl + 2;
+          const bool first = n == 0, end = n + 1 == n1;
+          if (end) segment();
+          n = end ? 0 : n + 1;
+          const bool last = n + 1 == n1;
+          bool due = false;
+          for (int x = 0; x < 2 && ok; ++x) {
+            if (x < now) {
+              ok = full(kv) && mbar_wait(bar(CPF + 2 * x), np[x] & 1, abort_flag, p.wait_cycles);
+              if (!ok) break;
+              issue_pv(x, kv % cStages, 0, first);
+              ok = mbar_wait(bar(CPF + 2 * x + 1), np[x] & 1, abort_flag, p.wait_cycles);
               if (!ok) break;
               ++np[x];
-              issue_pv(x, kv % cStages, n == 0);
-              if (n + 1 == n1) umma_commit(bar(COF + x));
-              if (n + 1 < n1) {
-                ok = full(kn);
-                if (!ok) break;
-                issue_s(x, kn % cStages);
-                if (n + 2 == n1) umma_commit(bar(CQE + x));
-              }
+              issue_pv(x, kv % cStages, 1, false);
+              if (end) umma_commit(bar(COF + x));
             }
-            if (!ok) break;
-            umma_commit(bar(CKE + kv % cStages));
-            if (n + 1 < n1) umma_commit(bar(CKE + kn % cStages));
+            if (x >= halves) continue;
+            if (x == 0 && end && now == 2 &&
+                !(mbar_try(bar(CQF), nseg[0] & 1) && mbar_try(bar(CKF + kn % cStages), (kn / cStages) & 1)))
+              due = true;
+            else
+              next_s(x, kn, end, last);
           }
-          nl += 2 * n1;
+          if (ok && due) next_s(0, kn, end, last);
+          if (!ok) break;
+          umma_commit(bar(CKE + kv % cStages));
+          if (halves > 0) umma_commit(bar(CKE + kn % cStages));
+          nl += 2;
         }
         if (!ok) {
           *abort_flag = 1;
@@ -360,91 +349,70 @@ __global__ void __launch_bounds__(cThreads, 1)
             for (int e = 0; e < 32; ++e)
               if (!((uint32_t(m) >> e) & 1u)) xs[c * 32 + e] = -INFINITY;
           };
+          float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          tmem_ld32(s_addr, xs);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            tmem_wait_ld();
+            if (c < 3) tmem_ld32(s_addr + 32 * (c + 1), xs + 32 * (c + 1));  // lands while this chunk is looked through
+            if (edge) mask_chunk(c);
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) mx4[(e >> 1) & 3] = max3f(mx4[(e >> 1) & 3], xs[c * 32 + e], xs[c * 32 + e + 1]);
+          }
+          const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+          // P and O stay scaled to m_ref until a score outgrows it by 2^rescale
+          float alpha = 1.0f;
+          if (mx > m_ref && (m_ref == -INFINITY || (mx - m_ref) * p.scale_log2 > Num<E>::rescale)) {
+            alpha = m_ref == -INFINITY ? 0.0f : fast_exp2((m_ref - mx) * p.scale_log2);
+            m_ref = mx;
+          }
+          if (j > w.j0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
+            // O holds PV(n - 1): S(n) was issued after it and is there
+#pragma unroll 1
+            for (int c = 0; c < D / 16; ++c) {
+              float o[16];
+              tmem_ld16(o_addr + c * 16, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 16; ++e) o[e] *= alpha;
+              tmem_st16(o_addr + c * 16, o);
+            }
+            tmem_wait_st();
+          }
+          const float moff = (m_ref == -INFINITY ? 0.0f : m_ref) * p.scale_log2;
+          const float2 off2 = make_float2(-moff, -moff);
           float2 rs2[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
-          auto exp_chunk = [&](int c, float2 off2, bool poly) {
+          auto exp_chunk = [&](int c) {
             uint32_t pk[16];
 #pragma unroll
             for (int e = 0; e < 32; e += 2) {
               const float2 a = __ffma2_rn(make_float2(xs[c * 32 + e], xs[c * 32 + e + 1]), sc2, off2);
               float2 ex;
-              if (poly && (e >> 1) % 4 < kPoly) {
-                ex = poly_exp2<Num<E>::degree>(a);
-              } else {
-                ex.x = fast_exp2(a.x);
-                ex.y = fast_exp2(a.y);
-              }
+              ex.x = fast_exp2(a.x);
+              ex.y = fast_exp2(a.y);
               rs2[(e >> 1) & 1] = __fadd2_rn(rs2[(e >> 1) & 1], ex);
               pk[e >> 1] = Num<E>::pack(ex.x, ex.y);
             }
             tmem_st16u(s_addr + c * 16, pk);
           };
-          // The common path takes m_ref as it stands and keeps the result when every P of the row is small
-          // enough (by the tile's row sum); a row's first tile with a key, or one that outgrows
-          // m_ref, takes the max path: new m_ref, O and l rescaled, P again.
-          float alpha = 1.0f;
-          bool fast = !__any_sync(0xffffffffu, m_ref == -INFINITY);
-          tmem_ld32(s_addr, xs);
-          tmem_wait_ld();
-          if (fast && !edge) {
-            const float moff = m_ref * p.scale_log2;
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              if (c < 3) tmem_ld32(s_addr + 32 * (c + 1), xs + 32 * (c + 1));  // lands while this chunk is worked on
-              exp_chunk(c, make_float2(-moff, -moff), true);
-              if (c < 3) tmem_wait_ld();
+          for (int c = 0; c < 4; ++c) {
+            exp_chunk(c);
+            if (c == 1) {  // the first 64 keys' product can start
+              tmem_wait_st();
+              fence_before();
+              mbar_arrive(bar(CPF + 2 * x));
             }
-            const float tsum = (rs2[0].x + rs2[0].y) + (rs2[1].x + rs2[1].y);
-            if (__any_sync(0xffffffffu, !(tsum <= Num<E>::pmax))) {
-              fast = false;
-              tmem_wait_st();  // the max path below rewrites P
-              rs2[0] = rs2[1] = make_float2(0.0f, 0.0f);
-            }
-          } else {
-            fast = false;
-#pragma unroll
-            for (int c = 1; c < 4; ++c) tmem_ld32(s_addr + 32 * c, xs + 32 * c);
-            tmem_wait_ld();
-            if (edge) {
-#pragma unroll
-              for (int c = 0; c < 4; ++c) mask_chunk(c);
-            }
-          }
-          if (!fast) {
-            float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-            for (int c = 0; c < cBN; c += 2) mx4[(c >> 1) & 3] = max3f(mx4[(c >> 1) & 3], xs[c], xs[c + 1]);
-            const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
-            if (mx > m_ref && (m_ref == -INFINITY || (mx - m_ref) * p.scale_log2 > Num<E>::rescale)) {
-              alpha = m_ref == -INFINITY ? 0.0f : fast_exp2((m_ref - mx) * p.scale_log2);
-              m_ref = mx;
-            }
-            const float moff = (m_ref == -INFINITY ? 0.0f : m_ref) * p.scale_log2;
-#pragma unroll
-            for (int c = 0; c < 4; ++c) exp_chunk(c, make_float2(-moff, -moff), false);
           }
           const float2 rsum = __fadd2_rn(rs2[0], rs2[1]);
           l_run = l_run * alpha + (rsum.x + rsum.y);
           tmem_wait_st();
-          if (j > w.j0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
-            // O holds PV(n - 1): S(n) was issued after it and is there
-#pragma unroll 1
-            for (int c = 0; c < D / 32; ++c) {
-              float o[32];
-              tmem_ld32(o_addr + c * 32, o);
-              tmem_wait_ld();
-#pragma unroll
-              for (int e = 0; e < 32; e += 2) {
-                const float2 v = __fmul2_rn(make_float2(o[e], o[e + 1]), make_float2(alpha, alpha));
-                o[e] = v.x;
-                o[e + 1] = v.y;
-              }
-              tmem_st32(o_addr + c * 32, o);
-            }
-            tmem_wait_st();
-          }
+        } else {
+          fence_before();
+          mbar_arrive(bar(CPF + 2 * x));
         }
         fence_before();
-        mbar_arrive(bar(CPF + x));
+        mbar_arrive(bar(CPF + 2 * x + 1));
       }
       if (!ok) break;
       if (mine) {
@@ -491,7 +459,7 @@ __global__ void __launch_bounds__(cThreads, 1)
         cut.tok0 = w.t.tok0;
         cut.nrows = nrows;
         cut.head0 = w.h * p.G;
-        cut.s1 = int((w.begin + kOverhead + g.n - 1) / per);
+        cut.s1 = int((u0 + w.begin + p.overhead + g.n - 1) / per);
         cut.first_slot = slot;
         p.cuts[blockIdx.x] = cut;
         noted = true;

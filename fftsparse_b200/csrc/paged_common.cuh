@@ -14,8 +14,7 @@ namespace paged {
 
 using namespace ::ffts::tc;
 
-constexpr int kMinShare = 4;      // length of a share, at least
-constexpr int kOverhead = 2;      // length of a (q tile, head) besides its key tiles
+constexpr int kMinShare = 4;      // length of a share, at least (2 and 3: the same time for one request's decode step)
 constexpr int kSchedThreads = 1024;
 constexpr int kOwnTiles = 1024;   // up to so many q tiles every CTA builds the schedule itself
 constexpr int kMaxCtas = 512;
@@ -52,6 +51,7 @@ struct Params {
   float2 *part_ml;            // [2 * ctas][rows]: m (log2 units) and l
   int max_tiles, ctas;
   int rows;                   // of a q tile: 128 or 256
+  int overhead;               // length of a (q tile, head) besides its key tiles
   int *status;
   long long wait_cycles, drain_cycles;
 };
@@ -152,7 +152,7 @@ __device__ int build_schedule(const Params &p, Tile *tiles, long long *cum, Sche
         t.pos0 = sc.kv[lo] - sc.len[lo] + i;
         t.ntok = min(p.tpt, sc.len[lo] - i);
         t.r = r0 + lo;
-        n = keys_of<BN>(t.pos0, t.ntok, p.window, p.sinks).n + kOverhead;
+        n = keys_of<BN>(t.pos0, t.ntok, p.window, p.sinks).n + p.overhead;
         if (FFTS_IN_RANGE(tile_base + x, p.max_tiles)) tiles[tile_base + x] = t;
       }
       long long sum;
@@ -175,25 +175,26 @@ __global__ void __launch_bounds__(kSchedThreads) schedule_kernel(const __grid_co
   if (threadIdx.x == 0) p.header[0] = n;
 }
 
-// Walks the share [u, u1) of the line segment by segment; the same in every lane.
+// Walks a share segment by segment; the same in every lane.  Positions are kept relative to the share and to the q tile,
+// in 32 bits: the host refuses a q tile whose heads' line passes 2^31, and a share that did would run for days.
 template <int BN>
 struct Walk {
   const Params &p;
   const Tile *tiles;
   const long long *cum;
-  long long u, u1;
-  long long base, next;  // the line before q tile x and behind it, all heads
+  int left, done;        // of the share: what is ahead, what lies behind
+  int rem, all;          // in q tile x: position and length, all heads
   int x;
   Tile t;
   Keys g;
   int h, j0, j1;         // the segment: head and key tiles [j0, j1) of the g.n
-  long long begin;       // where its (q tile, head) begins
+  int begin;             // where its (q tile, head) begins, relative to the share (may be negative)
   __device__ __forceinline__ Walk(const Params &prm, const Tile *t_, const long long *c_) : p(prm), tiles(t_), cum(c_) {}
 
   // Finds the q tile at u0 (whole warp; u0 < length).
-  __device__ __forceinline__ void seek(long long u0, long long end, int ntiles) {
-    u = u0;
-    u1 = end;
+  __device__ __forceinline__ void seek(long long u0, long long u1, int ntiles) {
+    left = int(u1 - u0);
+    done = 0;
     int lo = 0, n = ntiles;  // x is in [lo, lo + n): cum[lo] * Hkv <= u0
     const int lane = threadIdx.x & 31;
     while (n > 1) {
@@ -206,30 +207,32 @@ struct Walk {
       n = min(step, n - off);
     }
     x = lo;
+    rem = int(u0 - cum[x] * p.Hkv);
     load();
   }
   __device__ __forceinline__ void load() {
     t = tiles[FFTS_INDEX(x, p.max_tiles)];
-    base = cum[x] * p.Hkv;
-    next = cum[x + 1] * p.Hkv;
     g = keys_of<BN>(t.pos0, t.ntok, p.window, p.sinks);
+    all = (g.n + p.overhead) * p.Hkv;
   }
   // The next segment with key tiles; false behind the share's end.
   __device__ __forceinline__ bool segment() {
-    while (u < u1) {
-      if (u >= next) {
+    while (left > 0) {
+      if (rem >= all) {
+        rem = 0;
         ++x;
         load();
       }
-      const int len = g.n + kOverhead;
-      const long long rem = u - base;
-      h = int(rem / len);
-      const int at = int(rem - (long long)h * len);
-      const int to = int(min((long long)len, at + (u1 - u)));
-      begin = u - at;
-      u += to - at;
-      j0 = max(0, at - kOverhead);
-      j1 = max(0, to - kOverhead);
+      const int len = g.n + p.overhead;
+      h = rem / len;
+      const int at = rem - h * len;
+      const int to = min(len, at + left);
+      begin = done - at;
+      rem += to - at;
+      done += to - at;
+      left -= to - at;
+      j0 = max(0, at - p.overhead);
+      j1 = max(0, to - p.overhead);
       if (j1 > j0) return true;
     }
     return false;
@@ -246,7 +249,6 @@ struct Num<__nv_bfloat16> {
   static constexpr CUtensorMapDataType map = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   // P <= 2^64 against the reference max: bf16 and the fp32 O have the exponents for it
   static constexpr float rescale = 64.0f, pmax = 18446744073709551616.0f;
-  static constexpr int degree = 3;  // of paged_chunk.cu's exponential, 2^-13.7 off where P is rounded by 2^-8
   static __device__ __forceinline__ uint32_t pack(float a, float b) {
     const __nv_bfloat162 r = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const uint32_t *>(&r);
@@ -259,7 +261,6 @@ struct Num<__half> {
   // fp16 ends at 65504: P <= 2^8 after a rescale, 2^14 (a tile's row sum) before the next one; the row's
   // top has P >= 1, so what is lost below 2^-24 is that far under it
   static constexpr float rescale = 8.0f, pmax = 16384.0f;
-  static constexpr int degree = 4;  // 2^-18.5, P 2^-11
   static __device__ __forceinline__ uint32_t pack(float a, float b) {
     const __half2 r = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t *>(&r);
@@ -269,6 +270,60 @@ struct Num<__half> {
 constexpr uint32_t idesc(uint32_t fmt, bool b_mn_major, int n) {
   return (1u << 4) | (fmt << 7) | (fmt << 10) | (b_mn_major ? (1u << 16) : 0u) | (uint32_t(n >> 3) << 17) |
          (uint32_t(128 >> 4) << 24);
+}
+
+// True in one thread of the (converged) warp.  The compiler knows that no other thread is in the branch behind it, so
+// the operands of the MMAs there go straight to uniform registers; behind lane == 0 each one takes a
+// loop over the threads that might be active (30 to 40 instructions per MMA).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(one));
+  return one != 0;
+}
+
+// tcgen05.mma with descriptors as their low words (the address and the leading offset, which an advance along the tile
+// leaves alone) and a common high word: one 32-bit addition per operand instead of 64-bit ones.
+__device__ __forceinline__ void umma_ss(uint32_t d, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi,
+                                        uint32_t idesc_, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+      "mov.b64 a, {%1, %2};\n\tmov.b64 b, {%3, %4};\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %5, p;\n\t}" ::"r"(d),
+      "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc_), "r"(uint32_t(accumulate))
+      : "memory");
+}
+// A from TMEM.
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t b_hi, uint32_t idesc_,
+                                        bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
+      "mov.b64 b, {%2, %3};\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b_lo), "r"(b_hi), "r"(idesc_), "r"(uint32_t(accumulate))
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, float *v) {
+  uint32_t r[16];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const float *v) {
+  uint32_t r[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(v[i]);
+  tmem_st16u(taddr, r);
 }
 
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *map, uint32_t bar, int c0, int c1, int c2) {

@@ -4,10 +4,9 @@ Tolerances, with u = finfo(dtype).eps / 2 the relative size of one rounding:
   rope_append      u |y| for the result's rounding, plus (|a| + |b|) 2^-20 for the fp32 cos and sin (their
                    argument is a fraction of a turn, exact to 2^-25), products and sum, plus the dtype's smallest step
   paged_attention  u |o| for the result's rounding; u A with A = sum p |v| for the rounding of every p (the divisor
-                   sums them unrounded); A e with e = 2 ((D + 2) 2^-23 S + a) for the scores' fp32
+                   sums them unrounded); A e with e = 2 ((D + 2) 2^-23 S + 2^-20) for the scores' fp32
                    products (S the largest sum |q k| scale) through the exponential, both in numerator and
-                   divisor, and its approximation a (2^-13 with bf16, 2^-18 with fp16: the larger tiles take part of the exponentials
-                   from a polynomial of relative error 7.5e-5 and 2.6e-6, in p and in the divisor); keys 2^-24 max |v| for the p that fp16 flushes
+                   divisor, and its own approximation; keys 2^-24 max |v| for the p that fp16 flushes
 """
 import math
 import random
@@ -206,7 +205,7 @@ class Batch:
     """Ragged requests over a shuffled pool, NaN wherever nothing may be read."""
 
     def __init__(self, lens, H, Hkv, D, dt, page, layout="heads", seed=0, spread=2.0, window=None, sinks=0, extra=0,
-                 drop=False):
+                 drop=False, width=0):
         g = torch.Generator().manual_seed(seed + 7)
         self.lens, self.dt, self.page, self.window, self.sinks = lens, dt, page, window, sinks
         self.H, self.Hkv, self.D = H, Hkv, D
@@ -220,7 +219,7 @@ class Batch:
         self.vp = torch.full(shape, NAN, dtype=dt, device="cuda")
         if layout == "tokens":
             self.kp, self.vp = self.kp.transpose(1, 2), self.vp.transpose(1, 2)
-        W = max(counts + [1]) + 1
+        W = max(counts + [1, -(-width // page)]) + 1
         table, self.k, self.v, at = [], [], [], 0
         for (c, n), m in zip(lens, counts):
             ids = order[at:at + m]
@@ -265,7 +264,7 @@ class Batch:
                     seen &= (j > i - self.window) | (j < self.sinks)
                 p = s.masked_fill(~seen, -math.inf).softmax(-1)
                 want, A = (p @ x for x in (v, v.abs()))
-                e = 2 * ((self.D + 2) * 2.0 ** -23 * S + (2.0 ** -13 if self.dt == BF else 2.0 ** -18))
+                e = 2 * ((self.D + 2) * 2.0 ** -23 * S + 2.0 ** -20)
                 tol = u * want.abs() + (u + e) * A
                 if self.dt == FP:
                     tol = tol + (c + n) * 2.0 ** -24 * float(v.abs().max())
@@ -303,6 +302,25 @@ def test_paged_attention_window(lens, window, sinks, H, Hkv, D, dt, page):
     b.check(b.run())
 
 
+# Long table rows and requests of 256 rows on average: the kernel with the larger tiles.
+@pytest.mark.parametrize("lens", [[(1000, 37), (0, 200), (129, 1), (0, 129), (3333, 300), (64, 64)], [(9001, 150)], [(0, 256)],
+                                  [(17, 1), (40, 64), (0, 0), (0, 1000), (127, 129), (255, 600)], [(20000, 65)]])
+@pytest.mark.parametrize("H,Hkv,D,dt,page,layout", [
+    (32, 8, 128, BF, 16, "heads"), (28, 4, 128, FP, 32, "heads"), (16, 4, 64, BF, 64, "tokens"), (16, 1, 128, BF, 128, "heads"),
+    (9, 3, 64, FP, 256, "heads"), (5, 1, 128, FP, 16, "tokens"), (4, 4, 128, BF, 128, "heads"), (100, 1, 64, BF, 16, "heads")])
+def test_paged_attention_long_rows(lens, H, Hkv, D, dt, page, layout):
+    b = Batch(lens, H, Hkv, D, dt, page, layout, width=20000)
+    b.check(b.run())
+    F.check_status()
+
+
+@pytest.mark.parametrize("window,sinks", [(16400, 0), (17000, 4), (20000, 130), (10 ** 9, 3)])
+@pytest.mark.parametrize("H,Hkv,D,dt,page", [(8, 2, 128, BF, 16), (14, 2, 64, FP, 128)])
+def test_paged_attention_long_window(window, sinks, H, Hkv, D, dt, page):
+    b = Batch([(20100, 300), (0, 70), (16390, 90)], H, Hkv, D, dt, page, window=window, sinks=sinks, drop=True)
+    b.check(b.run())
+
+
 @pytest.mark.parametrize("H,Hkv", [(128, 1), (64, 1), (66, 2), (100, 1)])
 def test_paged_attention_many_heads_to_a_kv_head(H, Hkv):
     b = Batch(LENS["edges"] + [(500, 5)], H, Hkv, 64, BF, 16)
@@ -310,17 +328,18 @@ def test_paged_attention_many_heads_to_a_kv_head(H, Hkv):
 
 
 @pytest.mark.parametrize("lens", [[(i % 70, 1) for i in range(1300)], [(100, 9003), (7, 1)], [(40, 2)] * 1024])
-@pytest.mark.parametrize("window,sinks", [(None, 0), (90, 5)])
-def test_paged_attention_many_q_tiles(lens, window, sinks):
+@pytest.mark.parametrize("window,sinks,width", [(None, 0, 0), (90, 5, 0), (None, 0, 20000)])
+def test_paged_attention_many_q_tiles(lens, window, sinks, width):
     """More q tiles than a CTA schedules by itself, and just as many as it does."""
-    b = Batch(lens, 16, 1, 64, BF, 16, window=window, sinks=sinks, drop=True)
+    b = Batch(lens, 16, 1, 64, BF, 16, window=window, sinks=sinks, drop=True, width=width)
     b.check(b.run())
 
 
+@pytest.mark.parametrize("width", [0, 20000])
 @pytest.mark.parametrize("dt", [BF, FP])
-def test_paged_attention_scores_that_grow_and_peak(dt):
+def test_paged_attention_scores_that_grow_and_peak(dt, width):
     """Scores far apart (the running maximum moves by more than its slack) and a scale of its own."""
-    b = Batch([(700, 40), (1500, 1)], 8, 2, 64, dt, 16, spread=1.0)
+    b = Batch([(700, 140), (1500, 1)], 8, 2, 64, dt, 16, spread=1.0, width=width)
     ramp = torch.linspace(0.0, 1.0, 1600, device="cuda")
     for r, (c, n) in enumerate(b.lens):
         k = b.k[r].float()
@@ -333,8 +352,9 @@ def test_paged_attention_scores_that_grow_and_peak(dt):
     b.check(b.run(scale=0.5), scale=0.5)
 
 
-def test_rows_of_no_request_stay_and_empty_requests_give_zeros():
-    b = Batch([(30, 3), (0, 5), (100, 2), (40, 0)], 4, 2, 64, BF, 16, extra=4)
+@pytest.mark.parametrize("G,width", [(2, 0), (128, 20000)])
+def test_rows_of_no_request_stay_and_empty_requests_give_zeros(G, width):
+    b = Batch([(30, 3), (0, 5), (100, 2), (40, 0)], 2 * G, 2, 64, BF, 16, extra=4, width=width)
     out = torch.full_like(b.q, 7.0)
     b.kv[1] = 0  # not served: its five tokens see nothing
     got = F.paged_attention(b.q, b.kp, b.vp, b.table, b.cu, b.kv, out=out)
@@ -348,9 +368,10 @@ def test_rows_of_no_request_stay_and_empty_requests_give_zeros():
     b.check(out[8:])
 
 
-def test_more_new_tokens_than_keys():
+@pytest.mark.parametrize("G,width", [(2, 0), (100, 20000)])
+def test_more_new_tokens_than_keys(G, width):
     """kv_len 3 with 5 new tokens: the first two come before the first key and see nothing."""
-    b = Batch([(0, 5)], 2, 1, 64, BF, 16)
+    b = Batch([(0, 5)], G, 1, 64, BF, 16, width=width)
     b.kv[0] = 3
     got = b.run()
     assert bool((got[:2] == 0.0).all())
@@ -358,9 +379,10 @@ def test_more_new_tokens_than_keys():
     b.check(got[2:])
 
 
-def test_lengths_outside_their_tensors_are_kept_inside():
+@pytest.mark.parametrize("G,width", [(2, 0), (128, 20000)])
+def test_lengths_outside_their_tensors_are_kept_inside(G, width):
     """cu_q and kv_lens are device data: whatever they hold, no row outside q and no page outside the table is used."""
-    b = Batch([(30, 3), (50, 4)], 4, 2, 64, BF, 16)
+    b = Batch([(30, 3), (50, 4)], 2 * G, 2, 64, BF, 16, width=width)
     b.kp.nan_to_num_(0.0)
     b.vp.nan_to_num_(0.0)
     out = torch.zeros_like(b.q)
@@ -417,8 +439,9 @@ def test_paged_attention_refusals():
         F.plan_pages(ints([1]), ints([1]), ints([[0]]), ints([1]), 24, 1)
 
 
-def test_two_streams_at_once():
-    one = Batch(LENS["chunks"], 8, 2, 128, BF, 16, seed=1)
+@pytest.mark.parametrize("width", [0, 20000])
+def test_two_streams_at_once(width):
+    one = Batch(LENS["chunks"], 8, 2, 128, BF, 16, seed=1, width=width)
     two = Batch(LENS["decode"], 8, 2, 128, BF, 16, seed=2)
     want = one.run().clone(), two.run().clone()
     streams = torch.cuda.Stream(), torch.cuda.Stream()

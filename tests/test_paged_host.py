@@ -150,7 +150,7 @@ def test_rotary_frequency_refusals(args):
 
 
 # ------------------------------------------------------------------ schedule
-BM, BN, MIN_SHARE, OVERHEAD = 128, 64, 4, 2
+BM, BN, MIN_SHARE, OVERHEAD = 128, 64, 4, 3
 
 
 def keys_of(pos0, ntok, window, sinks):

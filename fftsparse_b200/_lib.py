@@ -30,7 +30,6 @@ DTYPE_F16 = 2
 _P = ctypes.c_void_p
 _I32 = ctypes.c_int32
 _I64 = ctypes.c_int64
-_F32 = ctypes.c_float
 EXPORTS = {
     "ffts_version": (_I32, []),
     "ffts_last_error_string": (ctypes.c_char_p, []),
@@ -52,12 +51,10 @@ EXPORTS = {
     "ffts_decode_workspace_bytes": (_I64, [_I64, _I64, _I64, _I64]),
     "ffts_decode_attn": (_I32, [_P, _I64, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _P, _I64, _P,
                                 _I64, _I64, _P, _I32, _I64, _P]),
-    "ffts_page_plan": (_I32, [_P, _P, _I64, _P, _I64, _I64, _P, _I64, _I64, _I64, _P, _P, _P, _P, _P, _P]),
-    "ffts_rope_append": (_I32, [_P, _P, _P, _P, _P, _P, _I32, _I64, _I64, _I64, _I64, _P, _P, _P, _I64, _I32, _F32,
-                                _P, _P, _P, _P, _P, _P, _I64, _I64, _P]),
+    "ffts_page_plan": (_I32, [_P, _P]),
+    "ffts_rope_append": (_I32, [_P, _P]),
     "ffts_paged_workspace_bytes": (_I64, [_I64, _I64, _I64, _I64, _I64]),
-    "ffts_paged_attn": (_I32, [_P, _P, _P, _P, _P, _P, _I32, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _P, _I64, _I64,
-                               _P, _P, _F32, _I64, _I64, _P, _P, _P, _I64, _P, _P]),
+    "ffts_paged_attn": (_I32, [_P, _P]),
     "ffts_sparse_attn_fwd": (_I32, [_P, _P, _P, _I64, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _I32,
                                     _I32, _P, _P, _P, _P]),
     "ffts_sparse_attn_fwd_rows": (_I32, [_P, _P, _P, _I64, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _I32,

@@ -120,20 +120,10 @@ int decode_attn(const void *q, int64_t qs_b, int64_t qs_h, const void *k, const 
                 const int64_t *vs, int64_t B, int64_t H, int64_t Hkv, int64_t Lk, int64_t D, int64_t splits,
                 void *ws, int64_t ws_bytes, void *out, int64_t os_b, int64_t os_h, const void *bias,
                 int bias_dtype, int64_t bias_sb, cudaStream_t stream);
-int page_plan(const int32_t *cached, const int32_t *fresh, int64_t R, int32_t *table, int64_t table_ld, int64_t width,
-              const int32_t *free_pages, int64_t n_free, int64_t page_size, int64_t T, int32_t *cu_q,
-              int32_t *kv_lens, int32_t *positions, int32_t *slots, int32_t *info, cudaStream_t stream);
-int rope_append(const void *q, const int64_t *qs, const void *k, const int64_t *ks, const void *v, const int64_t *vs,
-                int dtype, int64_t T, int64_t H, int64_t Hkv, int64_t D, const int32_t *positions,
-                const int32_t *slots, const float *inv_freq, int64_t rotary_dim, int interleaved, float amplitude,
-                void *q_out, const int64_t *os, void *k_pages, const int64_t *kps, void *v_pages, const int64_t *vps,
-                int64_t n_pages, int64_t page_size, cudaStream_t stream);
+int page_plan(const ffts_page_plan_args &a, cudaStream_t stream);
+int rope_append(const ffts_rope_append_args &a, cudaStream_t stream);
 int64_t paged_workspace_bytes(int64_t T, int64_t R, int64_t H, int64_t Hkv, int64_t D);
-int paged_attn(const void *q, const int64_t *qs, const void *k_pages, const int64_t *ks, const void *v_pages,
-               const int64_t *vs, int dtype, int64_t T, int64_t R, int64_t H, int64_t Hkv, int64_t D, int64_t n_pages,
-               int64_t page_size, const int32_t *table, int64_t table_ld, int64_t width, const int32_t *cu_q,
-               const int32_t *kv_lens, float scale, int64_t window, int64_t sinks, void *out, const int64_t *os,
-               void *ws, int64_t ws_bytes, int32_t *status, cudaStream_t stream);
+int paged_attn(const ffts_paged_attn_args &a, cudaStream_t stream);
 int64_t mask_workspace_bytes(int64_t B, int64_t H, int64_t N, int64_t D);
 int block_mask(const void *qb, const void *kb, int dtype, int64_t B, int64_t H, int64_t Hkv, int64_t D,
                const ffts_mask_params *params, uint32_t *bits, int32_t *row_count, float *corr,
@@ -250,47 +240,32 @@ int32_t ffts_decode_attn(const void *q, int64_t q_stride_b, int64_t q_stride_h, 
                      static_cast<cudaStream_t>(stream));
 }
 
-int32_t ffts_page_plan(const int32_t *cached_lens, const int32_t *new_lens, int64_t R, int32_t *table,
-                       int64_t table_ld, int64_t width, const int32_t *free_pages, int64_t n_free,
-                       int64_t page_size, int64_t num_tokens, int32_t *cu_q, int32_t *kv_lens, int32_t *positions,
-                       int32_t *slots, int32_t *info, void *stream) {
+int32_t ffts_page_plan(const ffts_page_plan_args *args, void *stream) {
   FFTS_ENTRY("ffts_page_plan");
+  FFTS_REQUIRE(args && args->struct_bytes == int64_t(sizeof(*args)), "page_plan: NULL or foreign argument block");
   int rc = check_device();
   if (rc) return rc;
-  return page_plan(cached_lens, new_lens, R, table, table_ld, width, free_pages, n_free, page_size, num_tokens, cu_q,
-                   kv_lens, positions, slots, info, static_cast<cudaStream_t>(stream));
+  return page_plan(*args, static_cast<cudaStream_t>(stream));
 }
 
-int32_t ffts_rope_append(const void *q, const int64_t *q_strides, const void *k, const int64_t *k_strides,
-                         const void *v, const int64_t *v_strides, int32_t dtype, int64_t T, int64_t H, int64_t Hkv,
-                         int64_t D, const int32_t *positions, const int32_t *slots, const float *inv_freq,
-                         int64_t rotary_dim, int32_t interleaved, float amplitude, void *q_out,
-                         const int64_t *out_strides, void *k_pages, const int64_t *kp_strides, void *v_pages,
-                         const int64_t *vp_strides, int64_t n_pages, int64_t page_size, void *stream) {
+int32_t ffts_rope_append(const ffts_rope_append_args *args, void *stream) {
   FFTS_ENTRY("ffts_rope_append");
+  FFTS_REQUIRE(args && args->struct_bytes == int64_t(sizeof(*args)), "rope_append: NULL or foreign argument block");
   int rc = check_device();
   if (rc) return rc;
-  return rope_append(q, q_strides, k, k_strides, v, v_strides, dtype, T, H, Hkv, D, positions, slots, inv_freq,
-                     rotary_dim, interleaved, amplitude, q_out, out_strides, k_pages, kp_strides, v_pages, vp_strides,
-                     n_pages, page_size, static_cast<cudaStream_t>(stream));
+  return rope_append(*args, static_cast<cudaStream_t>(stream));
 }
 
 int64_t ffts_paged_workspace_bytes(int64_t T, int64_t R, int64_t H, int64_t Hkv, int64_t D) {
   return paged_workspace_bytes(T, R, H, Hkv, D);
 }
 
-int32_t ffts_paged_attn(const void *q, const int64_t *q_strides, const void *k_pages, const int64_t *kp_strides,
-                        const void *v_pages, const int64_t *vp_strides, int32_t dtype, int64_t T, int64_t R,
-                        int64_t H, int64_t Hkv, int64_t D, int64_t n_pages, int64_t page_size, const int32_t *table,
-                        int64_t table_ld, int64_t width, const int32_t *cu_q, const int32_t *kv_lens, float scale,
-                        int64_t window, int64_t sinks, void *out, const int64_t *out_strides, void *workspace,
-                        int64_t workspace_bytes, int32_t *status, void *stream) {
+int32_t ffts_paged_attn(const ffts_paged_attn_args *args, void *stream) {
   FFTS_ENTRY("ffts_paged_attn");
+  FFTS_REQUIRE(args && args->struct_bytes == int64_t(sizeof(*args)), "paged_attn: NULL or foreign argument block");
   int rc = check_device();
   if (rc) return rc;
-  return paged_attn(q, q_strides, k_pages, kp_strides, v_pages, vp_strides, dtype, T, R, H, Hkv, D, n_pages,
-                    page_size, table, table_ld, width, cu_q, kv_lens, scale, window, sinks, out, out_strides,
-                    workspace, workspace_bytes, status, static_cast<cudaStream_t>(stream));
+  return paged_attn(*args, static_cast<cudaStream_t>(stream));
 }
 
 int64_t ffts_mask_workspace_bytes(int64_t B, int64_t H, int64_t N, int64_t D) {

@@ -162,37 +162,36 @@ __global__ void __launch_bounds__(kThreads) page_plan_kernel(const __grid_consta
 
 }  // namespace plan
 
-int page_plan(const int32_t *cached, const int32_t *fresh, int64_t R, int32_t *table, int64_t table_ld, int64_t width,
-              const int32_t *free_pages, int64_t n_free, int64_t page_size, int64_t T, int32_t *cu_q,
-              int32_t *kv_lens, int32_t *positions, int32_t *slots, int32_t *info, cudaStream_t stream) {
+int page_plan(const ffts_page_plan_args &a, cudaStream_t stream) {
   using namespace plan;
-  FFTS_REQUIRE(R >= 0 && T >= 0 && width >= 0 && n_free >= 0, "page_plan: negative size");
-  FFTS_REQUIRE(R < (int64_t(1) << 30) && T <= (int64_t(1) << 30) && n_free < (int64_t(1) << 31),
+  FFTS_REQUIRE(a.R >= 0 && a.num_tokens >= 0 && a.width >= 0 && a.n_free >= 0, "page_plan: negative size");
+  FFTS_REQUIRE(a.R < (int64_t(1) << 30) && a.num_tokens <= (int64_t(1) << 30) && a.n_free < (int64_t(1) << 31),
                "page_plan: more than 2^30 requests or tokens, or 2^31 free pages");
-  FFTS_REQUIRE(page_size >= 1 && page_size <= 4096 && (page_size & (page_size - 1)) == 0,
-               "page_plan: page_size must be a power of two up to 4096 (got %lld)", (long long)page_size);
-  FFTS_REQUIRE(width * page_size <= (int64_t(1) << 30), "page_plan: a table row spans more than 2^30 tokens");
-  FFTS_REQUIRE(table_ld >= width, "page_plan: table rows overlap (row stride %lld, width %lld)", (long long)table_ld,
-               (long long)width);
-  FFTS_REQUIRE(cu_q && info && (R == 0 || (cached && fresh && kv_lens && (width == 0 || table))) &&
-                   (T == 0 || (positions && slots)) && (n_free == 0 || free_pages),
+  FFTS_REQUIRE(a.page_size >= 1 && a.page_size <= 4096 && (a.page_size & (a.page_size - 1)) == 0,
+               "page_plan: page_size must be a power of two up to 4096 (got %lld)", (long long)a.page_size);
+  FFTS_REQUIRE(a.width <= (int64_t(1) << 30) / a.page_size, "page_plan: a table row spans more than 2^30 tokens");
+  FFTS_REQUIRE(a.table_ld >= a.width, "page_plan: table rows overlap (row stride %lld, width %lld)",
+               (long long)a.table_ld, (long long)a.width);
+  FFTS_REQUIRE(a.cu_q && a.info && (a.R == 0 || (a.cached_lens && a.new_lens && a.kv_lens && (a.width == 0 || a.table))) &&
+                   (a.num_tokens == 0 || (a.positions && a.slots)) && (a.n_free == 0 || a.free_pages),
                "page_plan: NULL argument");
+  const int64_t T = a.num_tokens;
   Params p{};
-  p.cached = cached;
-  p.fresh = fresh;
-  p.R = int(R);
-  p.table = table;
-  p.table_ld = table_ld;
-  p.width = int(width);
-  p.free_pages = free_pages;
-  p.n_free = int(n_free);
-  p.ps_shift = ilog2_ceil(page_size);
+  p.cached = a.cached_lens;
+  p.fresh = a.new_lens;
+  p.R = int(a.R);
+  p.table = a.table;
+  p.table_ld = a.table_ld;
+  p.width = int(a.width);
+  p.free_pages = a.free_pages;
+  p.n_free = int(a.n_free);
+  p.ps_shift = ilog2_ceil(a.page_size);
   p.T = int(T);
-  p.cu_q = cu_q;
-  p.kv_lens = kv_lens;
-  p.positions = positions;
-  p.slots = slots;
-  p.info = info;
+  p.cu_q = a.cu_q;
+  p.kv_lens = a.kv_lens;
+  p.positions = a.positions;
+  p.slots = a.slots;
+  p.info = a.info;
   const unsigned grid = unsigned(T > kTokensPerCta ? ceil_div(T, kTokensPerCta) : 1);
   page_plan_kernel<<<grid, kThreads, 0, stream>>>(p);
   FFTS_CUDA(cudaGetLastError());

@@ -647,21 +647,21 @@ struct Space {
 };
 
 template <typename E, int D>
-static int launch(Params &p, bool chunks, const void *q, const int64_t *qs, const void *k, const int64_t *ks,
-                  const void *v, const int64_t *vs, cudaStream_t stream) {
+static int launch(const Params &p, bool chunks, const ffts_paged_attn_args &a, cudaStream_t stream) {
+  const int64_t *qs = a.q_strides, *ks = a.kp_strides, *vs = a.vp_strides;
   CUtensorMap mq, mk, mv;
   const cuuint64_t qd[3] = {D, cuuint64_t(p.H), cuuint64_t(p.T)};
   const cuuint64_t qst[2] = {cuuint64_t(qs[1]) * 2, cuuint64_t(qs[0]) * 2};
   const cuuint32_t qbox[3] = {64, cuuint32_t(p.G), cuuint32_t(kBM / p.G)};
-  int rc = encode(&mq, Num<E>::map, 3, q, qd, qst, qbox);
+  int rc = encode(&mq, Num<E>::map, 3, a.q, qd, qst, qbox);
   if (rc) return rc;
   const cuuint64_t ps = 1ull << p.ps_shift;
   const cuuint64_t kd[4] = {D, ps, cuuint64_t(p.Hkv), cuuint64_t(p.n_pages)};
   const cuuint32_t kbox[4] = {64, cuuint32_t(std::min<cuuint64_t>(ps, chunks ? 2 * kBN : kBN)), 1, 1};
   const cuuint64_t kst[3] = {cuuint64_t(ks[2]) * 2, cuuint64_t(ks[1]) * 2, cuuint64_t(ks[0]) * 2};
   const cuuint64_t vst[3] = {cuuint64_t(vs[2]) * 2, cuuint64_t(vs[1]) * 2, cuuint64_t(vs[0]) * 2};
-  rc = encode(&mk, Num<E>::map, 4, k, kd, kst, kbox);
-  if (!rc) rc = encode(&mv, Num<E>::map, 4, v, kd, vst, kbox);
+  rc = encode(&mk, Num<E>::map, 4, a.k_pages, kd, kst, kbox);
+  if (!rc) rc = encode(&mv, Num<E>::map, 4, a.v_pages, kd, vst, kbox);
   if (rc) return rc;
   if (chunks) {
     rc = launch_chunk(p, Num<E>::fmt == 0, D, mq, mk, mv, stream);
@@ -698,60 +698,57 @@ int64_t paged_workspace_bytes(int64_t T, int64_t R, int64_t H, int64_t Hkv, int6
   return paged::Space(T, R, H / Hkv, D).bytes;
 }
 
-int paged_attn(const void *q, const int64_t *qs, const void *k_pages, const int64_t *ks, const void *v_pages,
-               const int64_t *vs, int dtype, int64_t T, int64_t R, int64_t H, int64_t Hkv, int64_t D, int64_t n_pages,
-               int64_t page_size, const int32_t *table, int64_t table_ld, int64_t width, const int32_t *cu_q,
-               const int32_t *kv_lens, float scale, int64_t window, int64_t sinks, void *out, const int64_t *os,
-               void *ws, int64_t ws_bytes, int32_t *status, cudaStream_t stream) {
+int paged_attn(const ffts_paged_attn_args &a, cudaStream_t stream) {
   using namespace paged;
-  FFTS_REQUIRE(dtype == FFTS_DTYPE_BF16 || dtype == FFTS_DTYPE_F16, "paged_attn: dtype must be bf16 or fp16");
+  const int64_t T = a.T, R = a.R, H = a.H, Hkv = a.Hkv, D = a.D, page_size = a.page_size, width = a.width;
+  FFTS_REQUIRE(a.dtype == FFTS_DTYPE_BF16 || a.dtype == FFTS_DTYPE_F16, "paged_attn: dtype must be bf16 or fp16");
   FFTS_REQUIRE(D == 64 || D == 128, "paged_attn: head_dim must be 64 or 128 (got %lld)", (long long)D);
   FFTS_REQUIRE(T >= 0 && R >= 0 && H >= 1 && Hkv >= 1 && H % Hkv == 0 && H / Hkv <= kBM,
                "paged_attn: bad shape (T %lld, R %lld, H %lld, Hkv %lld; at most %d query heads per KV head)",
                (long long)T, (long long)R, (long long)H, (long long)Hkv, kBM);
   FFTS_REQUIRE(page_size >= 16 && page_size <= 256 && (page_size & (page_size - 1)) == 0,
                "paged_attn: page_size must be 16, 32, 64, 128 or 256 (got %lld)", (long long)page_size);
-  FFTS_REQUIRE(T <= (int64_t(1) << 30) && R <= (int64_t(1) << 30) && H <= 65536 && n_pages < (int64_t(1) << 31) &&
-                   width >= 0 && width * page_size <= (int64_t(1) << 30),
+  FFTS_REQUIRE(T <= (int64_t(1) << 30) && R <= (int64_t(1) << 30) && H <= 65536 && a.n_pages < (int64_t(1) << 31) &&
+                   width >= 0 && width <= (int64_t(1) << 30) / page_size,
                "paged_attn: shape too large (a table row spans at most 2^30 tokens)");
   FFTS_REQUIRE(Hkv * (ceil_div(width * page_size, kBN) + kOverhead) < (int64_t(1) << 31),
                "paged_attn: %lld KV heads over a table row of %lld tokens are too many", (long long)Hkv,
                (long long)(width * page_size));
-  FFTS_REQUIRE(window >= 0 && sinks >= 0, "paged_attn: window and sinks must not be negative");
-  FFTS_REQUIRE(scale > 0.0f && scale < 3.0e38f, "paged_attn: scale must be positive and finite");
+  FFTS_REQUIRE(a.window >= 0 && a.sinks >= 0, "paged_attn: window and sinks must not be negative");
+  FFTS_REQUIRE(a.scale > 0.0f && a.scale < 3.0e38f, "paged_attn: scale must be positive and finite");
   if (T == 0 || R == 0) return FFTS_OK;
-  FFTS_REQUIRE(q && qs && k_pages && ks && v_pages && vs && cu_q && kv_lens && out && os && ws &&
-                   (width == 0 || table) && n_pages >= 1,
+  FFTS_REQUIRE(a.q && a.k_pages && a.v_pages && a.cu_q && a.kv_lens && a.out && a.workspace && (width == 0 || a.table) &&
+                   a.n_pages >= 1,
                "paged_attn: NULL argument or empty pool");
-  FFTS_REQUIRE(table_ld >= width || R == 1, "paged_attn: table rows overlap");
-  auto aligned = [](const void *x) { return (reinterpret_cast<uintptr_t>(x) & 15) == 0; };
-  FFTS_REQUIRE(aligned(q) && aligned(k_pages) && aligned(v_pages) && aligned(out) && aligned(ws),
-               "paged_attn: tensors must be 16-byte aligned");
+  FFTS_REQUIRE(a.table_ld >= width || R == 1, "paged_attn: table rows overlap");
+  for (const void *x : {a.q, a.k_pages, a.v_pages, static_cast<const void *>(a.out), static_cast<const void *>(a.workspace)})
+    FFTS_REQUIRE((reinterpret_cast<uintptr_t>(x) & 15) == 0, "paged_attn: tensors must be 16-byte aligned");
+  const int64_t *qs = a.q_strides, *os = a.out_strides;
   FFTS_REQUIRE(qs[0] > 0 && qs[1] > 0 && qs[0] % 8 == 0 && qs[1] % 8 == 0 && os[0] % 8 == 0 && os[1] % 8 == 0,
                "paged_attn: q and out strides must be positive multiples of 8 elements (16 bytes)");
-  for (const int64_t *st : {ks, vs})
+  for (const int64_t *st : {a.kp_strides, a.vp_strides})
     for (int i = 0; i < 3; ++i)
       FFTS_REQUIRE(st[i] > 0 && st[i] % 8 == 0 && st[i] < (int64_t(1) << 38),
                    "paged_attn: page strides must be positive multiples of 8 elements (16 bytes)");
-  FFTS_REQUIRE(ws_bytes >= paged_workspace_bytes(T, R, H, Hkv, D), "paged_attn: workspace too small");
+  FFTS_REQUIRE(a.workspace_bytes >= paged_workspace_bytes(T, R, H, Hkv, D), "paged_attn: workspace too small");
   const int64_t G = H / Hkv;
   const Space sp(T, R, G, D);
-  uint8_t *base = static_cast<uint8_t *>(ws);
+  uint8_t *base = static_cast<uint8_t *>(a.workspace);
   Params p{};
   p.T = int(T); p.R = int(R); p.H = int(H); p.Hkv = int(Hkv); p.G = int(G); p.tpt = int(kBM / G);
-  p.table = table;
-  p.table_ld = table_ld;
+  p.table = a.table;
+  p.table_ld = a.table_ld;
   p.width = int(width);
-  p.n_pages = int(n_pages);
+  p.n_pages = int(a.n_pages);
   p.ps_shift = ilog2_ceil(page_size);
-  p.cu_q = cu_q;
-  p.kv_lens = kv_lens;
-  p.window = int(std::min<int64_t>(window, int64_t(1) << 30));
-  p.sinks = window > 0 ? int(std::min<int64_t>(sinks, int64_t(1) << 30)) : 0;
-  p.out = static_cast<uint16_t *>(out);
+  p.cu_q = a.cu_q;
+  p.kv_lens = a.kv_lens;
+  p.window = int(std::min<int64_t>(a.window, int64_t(1) << 30));
+  p.sinks = a.window > 0 ? int(std::min<int64_t>(a.sinks, int64_t(1) << 30)) : 0;
+  p.out = static_cast<uint16_t *>(a.out);
   p.os_t = os[0];
   p.os_h = os[1];
-  p.scale_log2 = scale * 1.4426950408889634f;
+  p.scale_log2 = a.scale * 1.4426950408889634f;
   p.max_tiles = int(sp.max_tiles);
   p.own_schedule = sp.max_tiles <= kOwnTiles;
   p.cum = reinterpret_cast<long long *>(base + sp.cum);
@@ -769,24 +766,23 @@ int paged_attn(const void *q, const int64_t *qs, const void *k_pages, const int6
   // the window bound them, are long enough to pay for filling and draining one pipeline per SM instead of two.
   // 2048 tokens of 32 / 8 heads over 32768 cached: 1.19 ms against 1.37 (0.98 and 1.11 before the power cap sets
   // in); 512 over 16384: 129 us both; 16 ragged chunks over up to 16384: 72 against 59.
-  const int64_t span = window > 0 ? std::min(width * page_size, p.window + p.sinks + T / R) : width * page_size;
+  int64_t span = width * page_size;
+  if (p.window > 0) span = std::min(span, int64_t(p.window) + p.sinks + T / R);
   const bool chunks = T * G >= 2 * kBM * R && span > kLongKeys;
   p.ctas = std::min(chunks ? sms : 2 * sms, kMaxCtas / (chunks ? 2 : 1));
   p.rows = chunks ? 2 * kBM : kBM;
   if (chunks) p.tpt *= 2;
   p.overhead = kOverhead;
-  if (status) {
-    p.status = status;
+  if (a.status) {
+    p.status = a.status;
   } else {
     void *sink = nullptr;
     FFTS_CUDA(cudaGetSymbolAddress(&sink, g_status_sink));
     p.status = static_cast<int *>(sink);
   }
-  if (dtype == FFTS_DTYPE_BF16)
-    return D == 128 ? launch<__nv_bfloat16, 128>(p, chunks, q, qs, k_pages, ks, v_pages, vs, stream)
-                    : launch<__nv_bfloat16, 64>(p, chunks, q, qs, k_pages, ks, v_pages, vs, stream);
-  return D == 128 ? launch<__half, 128>(p, chunks, q, qs, k_pages, ks, v_pages, vs, stream)
-                  : launch<__half, 64>(p, chunks, q, qs, k_pages, ks, v_pages, vs, stream);
+  if (a.dtype == FFTS_DTYPE_BF16)
+    return D == 128 ? launch<__nv_bfloat16, 128>(p, chunks, a, stream) : launch<__nv_bfloat16, 64>(p, chunks, a, stream);
+  return D == 128 ? launch<__half, 128>(p, chunks, a, stream) : launch<__half, 64>(p, chunks, a, stream);
 }
 
 }  // namespace ffts

@@ -33,19 +33,21 @@ from .status import device_status
 __all__ = ["PagePlan", "plan_pages", "rotary_inv_freq", "rope_append", "paged_attention"]
 
 _DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
-_pack2 = struct.Struct("2q").pack  # strides as the C calls take them: int64 arrays
-_pack3 = struct.Struct("3q").pack
+# The C calls' argument blocks (ffts_*_args): 64-bit pointers, strides and sizes, then the 32-bit fields.
+_PLAN = struct.Struct("=16q")
+_ROPE = struct.Struct("=31qiifi")
+_ATTN = struct.Struct("=32qif")
 _raw_stream = torch._C._cuda_getCurrentRawStream  # current_stream(device).cuda_stream without the Stream object
 
 
-def _call(device: torch.device, fn, *args) -> None:
+def _call(device: torch.device, fn, block: bytes) -> None:
     """One C call with ``device`` current, on its current stream."""
     index = device.index
     if index == torch.cuda.current_device():
-        rc = fn(*args, _raw_stream(index))
+        rc = fn(block, _raw_stream(index))
     else:
         with torch.cuda.device(device):
-            rc = fn(*args, _raw_stream(index))
+            rc = fn(block, _raw_stream(index))
     if rc:
         _lib.check(rc)
 
@@ -71,7 +73,7 @@ def _check_table(t: torch.Tensor, rows: int, device) -> int:
 
 
 def _check_heads(name: str, t: torch.Tensor, dtype, device):
-    """The strides of a [tokens, heads, head_dim] tensor, packed."""
+    """The token and head strides of a [tokens, heads, head_dim] tensor."""
     if t.dim() != 3:
         raise ValueError(f"{name} must be [tokens, heads, head_dim], got shape {tuple(t.shape)}")
     if t.dtype is not dtype:
@@ -81,11 +83,11 @@ def _check_heads(name: str, t: torch.Tensor, dtype, device):
     st, sh, sd = t.stride()
     if sd != 1:
         raise ValueError(f"{name} must be contiguous in the head dimension")
-    return _pack2(st, sh)
+    return st, sh
 
 
 def _check_pool(k_pages: torch.Tensor, v_pages: torch.Tensor, dtype, device):
-    """The strides of both pool tensors, packed."""
+    """The page, head and row strides of both pool tensors."""
     if k_pages.dim() != 4 or v_pages.shape != k_pages.shape:
         raise ValueError(f"k_pages and v_pages must both be [pages, Hkv, page_size, D], got "
                          f"{tuple(k_pages.shape)} / {tuple(v_pages.shape)}")
@@ -97,7 +99,7 @@ def _check_pool(k_pages: torch.Tensor, v_pages: torch.Tensor, dtype, device):
     *vs, vd = v_pages.stride()
     if kd != 1 or vd != 1:
         raise ValueError("k_pages and v_pages must be contiguous in the head dimension")
-    return _pack3(*ks), _pack3(*vs)
+    return ks, vs
 
 
 def _check_cuda(name: str, t: torch.Tensor) -> None:
@@ -149,9 +151,9 @@ def plan_pages(cached_lens: torch.Tensor, new_lens: torch.Tensor, block_table: t
     kv = cu + 4 * (R + 1)
     pos = kv + 4 * R
     slot = pos + 4 * num_tokens
-    _call(dev, _lib.load().ffts_page_plan, cached_lens.data_ptr(), new_lens.data_ptr(), R, block_table.data_ptr(),
-          table_ld, block_table.shape[1], free_pages.data_ptr(), n_free, page_size, num_tokens, cu, kv, pos, slot,
-          slot + 4 * num_tokens)
+    _call(dev, _lib.load().ffts_page_plan, _PLAN.pack(
+        _PLAN.size, cached_lens.data_ptr(), new_lens.data_ptr(), block_table.data_ptr(), free_pages.data_ptr(), cu, kv,
+        pos, slot, slot + 4 * num_tokens, R, table_ld, block_table.shape[1], n_free, page_size, num_tokens))
     return plan
 
 
@@ -244,14 +246,15 @@ def rope_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, pos
         raise ValueError(f"pages {tuple(k_pages.shape)} do not match k {tuple(k.shape)}")
     _check_ints("positions", positions, T, dev)
     _check_ints("slot_map", slot_map, T, dev)
-    rd, freq = 0, None
+    rd = freq = 0
     if inv_freq is not None:
         if inv_freq.dim() != 1 or inv_freq.dtype is not torch.float32 or not inv_freq.is_contiguous():
             raise ValueError("inv_freq must be a contiguous 1-D fp32 tensor")
         if inv_freq.device != dev:
             raise ValueError(f"inv_freq must be on {dev}, got {inv_freq.device}")
         rd, freq = 2 * inv_freq.shape[0], inv_freq.data_ptr()
-    H, q_ptr, o_ptr, qs, os_ = 0, None, None, None, None
+    H = q_ptr = o_ptr = 0
+    qs = os_ = (0, 0)
     if q is not None:
         qs = _check_heads("q", q, dt, dev)
         H = q.shape[1]
@@ -267,13 +270,14 @@ def rope_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, pos
     if q is not None:
         if out is None:
             out = torch.empty(T, H, D, dtype=dt, device=dev)
-            os_ = _pack2(H * D, D)
+            os_ = (H * D, D)
         q_ptr, o_ptr = q.data_ptr(), out.data_ptr()
     if T == 0:
         return out
-    _call(dev, _lib.load().ffts_rope_append, q_ptr, qs, k.data_ptr(), ks, v.data_ptr(), vs, _DTYPES[dt], T, H, Hkv, D,
-          positions.data_ptr(), slot_map.data_ptr(), freq, rd, interleaved, attn_factor, o_ptr, os_,
-          k_pages.data_ptr(), kps, v_pages.data_ptr(), vps, P, page_size)
+    _call(dev, _lib.load().ffts_rope_append, _ROPE.pack(
+        _ROPE.size, q_ptr, k.data_ptr(), v.data_ptr(), positions.data_ptr(), slot_map.data_ptr(), freq, o_ptr,
+        k_pages.data_ptr(), v_pages.data_ptr(), *qs, *ks, *vs, *os_, *kps, *vps, T, H, Hkv, D, rd, P, page_size,
+        _DTYPES[dt], interleaved, attn_factor, 0))
     return out
 
 
@@ -326,7 +330,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     _check_cuda("q", q)
     if out is None:
         out = torch.empty(T, H, D, dtype=dt, device=dev)
-        os_ = _pack2(H * D, D)
+        os_ = (H * D, D)
     if T == 0 or R == 0:
         return out
     lib = _lib.load()
@@ -334,8 +338,9 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     status.poll_direct()
     nbytes = lib.ffts_paged_workspace_bytes(T, R, H, Hkv, D)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    _call(dev, lib.ffts_paged_attn, q.data_ptr(), qs, k_pages.data_ptr(), kps, v_pages.data_ptr(), vps, _DTYPES[dt], T,
-          R, H, Hkv, D, P, page_size, block_table.data_ptr(), table_ld, block_table.shape[1], cu_q.data_ptr(),
-          kv_lens.data_ptr(), D ** -0.5 if scale is None else scale, window, sinks, out.data_ptr(), os_,
-          ws.data_ptr(), nbytes, status.direct_ptr)
+    _call(dev, lib.ffts_paged_attn, _ATTN.pack(
+        _ATTN.size, q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(), cu_q.data_ptr(),
+        kv_lens.data_ptr(), out.data_ptr(), ws.data_ptr(), status.direct_ptr, *qs, *kps, *vps, *os_, T, R, H, Hkv, D, P,
+        page_size, table_ld, block_table.shape[1], window, sinks, nbytes, _DTYPES[dt],
+        D ** -0.5 if scale is None else scale))
     return out

@@ -201,38 +201,45 @@ FFTS_API int32_t ffts_decode_attn(const void *q, int64_t q_stride_b, int64_t q_s
  * whose callers keep one contiguous cache per prompt.  Per step: ffts_page_plan
  * once, then per layer ffts_rope_append and ffts_paged_attn.  All lengths and
  * tables are device data: the calls can be captured into a graph and replayed
- * with other lengths.
+ * with other lengths.  Each call takes one argument block (struct_bytes is its
+ * sizeof; a foreign function interface then converts one pointer, not thirty
+ * values).
  *
  * ffts_page_plan: the step's bookkeeping from request lengths.
- *   cached_lens, new_lens int32 [R]: tokens in the cache before the step, tokens
- *     of the step (negative counts as 0).
- *   table int32 [R, width], row stride table_ld: page numbers of each request; its
- *     first ceil(cached / page_size) entries are read, the entries of its new pages
- *     are written, taken from free_pages [n_free] in order of the requests.
- *   cu_q int32 [R + 1]: first token of each request (at most num_tokens); kv_lens
- *     int32 [R]: cached + new.
- *   positions, slots int32 [num_tokens]: each token's position in its request, and
+ *   cached_lens, new_lens [R]: tokens in the cache before the step, tokens of the
+ *     step (negative counts as 0).
+ *   table [R, width], row stride table_ld: page numbers of each request; its first
+ *     ceil(cached / page_size) entries are read, the entries of its new pages are
+ *     written, taken from free_pages [n_free] in order of the requests.
+ *   cu_q [R + 1]: first token of each request (at most num_tokens); kv_lens [R]:
+ *     cached + new.
+ *   positions, slots [num_tokens]: each token's position in its request, and
  *     page * page_size + row of its place in the pool.  Rows behind the last
  *     request's tokens get position 0 and slot -1.
- *   info int32 [2]: pages taken from the list, requests not served.
+ *   info [2]: pages taken from the list, requests not served.
  * A request is served if its pages fit its table row, its tokens fit num_tokens and
  * its new pages, counted on from the requests before it, fit the list; one that
  * needs no new page needs no room there.  A request that is not served has kv_len
  * 0 and slots -1.  page_size is a power of two up to 4096.
  */
-FFTS_API int32_t ffts_page_plan(const int32_t *cached_lens, const int32_t *new_lens, int64_t R,
-                  int32_t *table, int64_t table_ld, int64_t width, const int32_t *free_pages,
-                  int64_t n_free, int64_t page_size, int64_t num_tokens, int32_t *cu_q,
-                  int32_t *kv_lens, int32_t *positions, int32_t *slots, int32_t *info, void *stream);
+typedef struct ffts_page_plan_args {
+  int64_t struct_bytes;
+  const int32_t *cached_lens, *new_lens;
+  int32_t *table;
+  const int32_t *free_pages;
+  int32_t *cu_q, *kv_lens, *positions, *slots, *info;
+  int64_t R, table_ld, width, n_free, page_size, num_tokens;
+} ffts_page_plan_args;
+FFTS_API int32_t ffts_page_plan(const ffts_page_plan_args *args, void *stream);
 
 /*
  * ffts_rope_append: rotary positions of q and k and the append of k and v to the
  * pool, one pass.
  *   q [T, H, D] (NULL: none), k, v [T, Hkv, D]: strides (t, h), unit over D; q_out
  *     [T, H, D] with strides (t, h) (may be q).
- *   positions, slots int32 [T]; a token whose slot lies outside the pool is not
- *     appended (its q is rotated all the same).  Slots are distinct.
- *   inv_freq fp32 [rotary_dim / 2]; the first rotary_dim channels are rotated by
+ *   positions, slots [T]; a token whose slot lies outside the pool is not appended
+ *     (its q is rotated all the same).  Slots are distinct.
+ *   inv_freq [rotary_dim / 2]; the first rotary_dim channels are rotated by
  *     position * inv_freq, pairs (i, i + rotary_dim / 2), or (2i, 2i + 1) if
  *     interleaved; cos and sin are multiplied by amplitude; the other channels are
  *     copied.  rotary_dim a multiple of 16 up to D; 0 copies k and v as they are.
@@ -240,15 +247,20 @@ FFTS_API int32_t ffts_page_plan(const int32_t *cached_lens, const int32_t *new_l
  * Angles are reduced in 64 bits, the rest is fp32, rounded once.  bf16 or fp16, D 64
  * or 128; all strides multiples of 8 elements, tensors 16-byte aligned.
  */
-FFTS_API int32_t ffts_rope_append(const void *q, const int64_t *q_strides /* t,h */, const void *k,
-                  const int64_t *k_strides /* t,h */, const void *v,
-                  const int64_t *v_strides /* t,h */, int32_t dtype, int64_t T, int64_t H,
-                  int64_t Hkv, int64_t D, const int32_t *positions, const int32_t *slots,
-                  const float *inv_freq, int64_t rotary_dim, int32_t interleaved, float amplitude,
-                  void *q_out, const int64_t *out_strides /* t,h */, void *k_pages,
-                  const int64_t *kp_strides /* page,head,row */, void *v_pages,
-                  const int64_t *vp_strides /* page,head,row */, int64_t n_pages,
-                  int64_t page_size, void *stream);
+typedef struct ffts_rope_append_args {
+  int64_t struct_bytes;
+  const void *q, *k, *v;
+  const int32_t *positions, *slots;
+  const float *inv_freq;
+  void *q_out, *k_pages, *v_pages;
+  int64_t q_strides[2], k_strides[2], v_strides[2], out_strides[2]; /* t, h */
+  int64_t kp_strides[3], vp_strides[3];                             /* page, head, row */
+  int64_t T, H, Hkv, D, rotary_dim, n_pages, page_size;
+  int32_t dtype, interleaved;
+  float amplitude;
+  int32_t reserved;
+} ffts_rope_append_args;
+FFTS_API int32_t ffts_rope_append(const ffts_rope_append_args *args, void *stream);
 
 /*
  * ffts_paged_attn: causal attention of each request's new tokens over its pages.
@@ -256,9 +268,9 @@ FFTS_API int32_t ffts_rope_append(const void *q, const int64_t *q_strides /* t,h
  *     cu_q[r] .. cu_q[r + 1] - 1, the last of its kv_lens[r] tokens.  Rows of no
  *     request are not written.
  *   k_pages, v_pages [n_pages, Hkv, page_size, D]: strides (page, head, row).
- *   table int32 [R, width], row stride table_ld.  What the pool holds behind a
- *     request's last token, or in pages no token of it sees, does not matter; a page
- *     number outside the pool reads as zeros.
+ *   table [R, width], row stride table_ld.  What the pool holds behind a request's
+ *     last token, or in pages no token of it sees, does not matter; a page number
+ *     outside the pool reads as zeros.
  *   A token at position p sees key c iff c <= p and (window == 0, or c > p - window,
  *   or c < sinks).  Tokens that see nothing get zeros.  window 0: no window.
  *   workspace: ffts_paged_workspace_bytes(T, R, H, Hkv, D) bytes, 16-byte aligned,
@@ -271,15 +283,21 @@ FFTS_API int32_t ffts_rope_append(const void *q, const int64_t *q_strides /* t,h
  * (a power of two); q and page strides multiples of 8 elements, tensors 16-byte
  * aligned.
  */
+typedef struct ffts_paged_attn_args {
+  int64_t struct_bytes;
+  const void *q, *k_pages, *v_pages;
+  const int32_t *table, *cu_q, *kv_lens;
+  void *out, *workspace;
+  int32_t *status;
+  int64_t q_strides[2];                 /* t, h */
+  int64_t kp_strides[3], vp_strides[3]; /* page, head, row */
+  int64_t out_strides[2];               /* t, h */
+  int64_t T, R, H, Hkv, D, n_pages, page_size, table_ld, width, window, sinks, workspace_bytes;
+  int32_t dtype;
+  float scale;
+} ffts_paged_attn_args;
 FFTS_API int64_t ffts_paged_workspace_bytes(int64_t T, int64_t R, int64_t H, int64_t Hkv, int64_t D);
-FFTS_API int32_t ffts_paged_attn(const void *q, const int64_t *q_strides /* t,h */,
-                  const void *k_pages, const int64_t *kp_strides /* page,head,row */,
-                  const void *v_pages, const int64_t *vp_strides /* page,head,row */,
-                  int32_t dtype, int64_t T, int64_t R, int64_t H, int64_t Hkv, int64_t D,
-                  int64_t n_pages, int64_t page_size, const int32_t *table, int64_t table_ld,
-                  int64_t width, const int32_t *cu_q, const int32_t *kv_lens, float scale,
-                  int64_t window, int64_t sinks, void *out, const int64_t *out_strides /* t,h */,
-                  void *workspace, int64_t workspace_bytes, int32_t *status, void *stream);
+FFTS_API int32_t ffts_paged_attn(const ffts_paged_attn_args *args, void *stream);
 
 /* Bytes of device workspace ffts_block_mask / ffts_prefill need. */
 FFTS_API int64_t ffts_mask_workspace_bytes(int64_t B, int64_t H, int64_t N, int64_t D);

@@ -227,6 +227,21 @@ def test_shares_cover_every_key_tile_once_and_the_join_finds_its_partials(seed):
     assert whole | cut == {(x, h) for _, x, h, _ in line} and not whole & cut
 
 
+@pytest.mark.parametrize("name", ["page_plan", "rope_append", "paged_attn"])
+def test_foreign_argument_blocks_are_refused(name):
+    """The blocks that the package packs have the header's sizes; another size is refused before anything else."""
+    from fftsparse_b200 import _lib, paged
+    lib = _lib.load()
+    call = getattr(lib, f"ffts_{name}")
+    size = {"page_plan": paged._PLAN, "rope_append": paged._ROPE, "paged_attn": paged._ATTN}[name].size
+    for wrong in (0, size - 8, size + 8):
+        assert call(wrong.to_bytes(8, "little") + bytes(size), None) == _lib.FFTS_E_INVALID
+        assert b"foreign" in lib.ffts_last_error_string()
+    assert call(None, None) == _lib.FFTS_E_INVALID
+    if not torch.cuda.is_available():  # the right size passes on to the look for a device
+        assert call(size.to_bytes(8, "little") + bytes(size), None) == _lib.FFTS_E_CUDA
+
+
 def test_workspace_query_needs_no_gpu():
     from fftsparse_b200 import _lib
     lib = _lib.load()

@@ -86,12 +86,32 @@ __global__ void __launch_bounds__(kThreads, 2)
   using Lay = Layout<D>;
   extern __shared__ __align__(16) uint8_t smem[];
   if (smem_u32(smem) & 1023u) {  // SWIZZLE_128B tiles need 1024-byte alignment
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     if (threadIdx.x == 0) {
       *reinterpret_cast<volatile int *>(p.status) = kErrSmemAlign;
       p.cuts[blockIdx.x].nrows = 0;
     }
     return;
   }
+  const uint32_t sbase = smem_u32(smem);
+  auto bar = [&](int i) { return sbase + Lay::bars + 8u * uint32_t(i); };
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + Lay::abort);
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + Lay::tmem_slot);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int qrows = p.tpt * p.G;  // rows a Q load fills
+
+  if (threadIdx.x == 0) {
+    *abort_flag = 0;
+    for (int i = 0; i < Lay::nbars; ++i) mbar_init(bar(i), (i == BPF || i == BPF + 1) ? 128u : 1u);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 4 && lane == 0) {
+    prefetch_map(&tm_q);
+    prefetch_map(&tm_k);
+    prefetch_map(&tm_v);
+  }
+  // launched while the kernel before drains: nothing in global memory is touched before this
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   Tile *tiles = p.tiles;
   long long *cum = p.cum;
   int ntiles;
@@ -112,18 +132,6 @@ __global__ void __launch_bounds__(kThreads, 2)
     if (threadIdx.x == 0) p.cuts[blockIdx.x].nrows = 0;
     return;
   }
-  const uint32_t sbase = smem_u32(smem);
-  auto bar = [&](int i) { return sbase + Lay::bars + 8u * uint32_t(i); };
-  volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + Lay::abort);
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + Lay::tmem_slot);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int qrows = p.tpt * p.G;  // rows a Q load fills
-
-  if (threadIdx.x == 0) {
-    *abort_flag = 0;
-    for (int i = 0; i < Lay::nbars; ++i) mbar_init(bar(i), (i == BPF || i == BPF + 1) ? 128u : 1u);
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  }
   // rows no Q load fills: zeros, so that they stay finite
   for (int i = threadIdx.x; i < (kBM - qrows) * 8 * Lay::halves; i += kThreads) {
     const int row = qrows + (i >> 3) / Lay::halves, hf = (i >> 3) % Lay::halves;
@@ -134,11 +142,6 @@ __global__ void __launch_bounds__(kThreads, 2)
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
                  "r"(kTmemCols));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
-  }
-  if (warp == 4 && lane == 0) {
-    prefetch_map(&tm_q);
-    prefetch_map(&tm_k);
-    prefetch_map(&tm_v);
   }
   fence_before();
   __syncthreads();
@@ -674,21 +677,10 @@ static int launch(const Params &p, bool chunks, const ffts_paged_attn_args &a, c
       schedule_kernel<kBN><<<1, kSchedThreads, 0, stream>>>(p);
       FFTS_CUDA(cudaGetLastError());
     }
-    attn_kernel<E, D><<<unsigned(p.ctas), kThreads, Layout<D>::bytes, stream>>>(mq, mk, mv, p);
-    FFTS_CUDA(cudaGetLastError());
+    rc = launch_early(attn_kernel<E, D>, dim3(unsigned(p.ctas)), kThreads, Layout<D>::bytes, stream, mq, mk, mv, p);
+    if (rc) return rc;
   }
-  // launched while the attention kernel drains
-  cudaLaunchAttribute early{};
-  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  early.val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(unsigned(p.ctas), kJoinBlocks);
-  cfg.blockDim = dim3(kJoinThreads);
-  cfg.stream = stream;
-  cfg.attrs = &early;
-  cfg.numAttrs = 1;
-  FFTS_CUDA(cudaLaunchKernelEx(&cfg, join_kernel<E, D>, p));
-  return FFTS_OK;
+  return launch_early(join_kernel<E, D>, dim3(unsigned(p.ctas), kJoinBlocks), kJoinThreads, 0, stream, p);
 }
 
 }  // namespace paged

@@ -63,12 +63,33 @@ __global__ void __launch_bounds__(cThreads, 1)
   using Lay = ChunkLayout<D>;
   extern __shared__ __align__(16) uint8_t smem[];
   if (smem_u32(smem) & 1023u) {  // SWIZZLE_128B tiles need 1024-byte alignment
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     if (threadIdx.x == 0) {
       *reinterpret_cast<volatile int *>(p.status) = kErrSmemAlign;
       p.cuts[blockIdx.x].nrows = 0;
     }
     return;
   }
+  const uint32_t sbase = smem_u32(smem);
+  auto bar = [&](int i) { return sbase + Lay::bars + 8u * uint32_t(i); };
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + Lay::abort);
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + Lay::tmem_slot);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int tph = cBM / p.G;        // tokens of a half
+  const int qrows = tph * p.G;      // rows of it that a Q load fills
+
+  if (threadIdx.x == 0) {
+    *abort_flag = 0;
+    for (int i = 0; i < Lay::nbars; ++i) mbar_init(bar(i), (i >= CPF && i < CPF + 4) ? 128u : 1u);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 8 && lane == 0) {
+    prefetch_map(&tm_q);
+    prefetch_map(&tm_k);
+    prefetch_map(&tm_v);
+  }
+  // launched while the kernel before drains: nothing in global memory is touched before this
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   Tile *tiles = p.tiles;
   long long *cum = p.cum;
   int ntiles;
@@ -89,19 +110,6 @@ __global__ void __launch_bounds__(cThreads, 1)
     if (threadIdx.x == 0) p.cuts[blockIdx.x].nrows = 0;
     return;
   }
-  const uint32_t sbase = smem_u32(smem);
-  auto bar = [&](int i) { return sbase + Lay::bars + 8u * uint32_t(i); };
-  volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + Lay::abort);
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + Lay::tmem_slot);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int tph = cBM / p.G;        // tokens of a half
-  const int qrows = tph * p.G;      // rows of it that a Q load fills
-
-  if (threadIdx.x == 0) {
-    *abort_flag = 0;
-    for (int i = 0; i < Lay::nbars; ++i) mbar_init(bar(i), (i >= CPF && i < CPF + 4) ? 128u : 1u);
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  }
   // rows no Q load fills: zeros, so that they stay finite
   for (int i = threadIdx.x; i < 2 * (cBM - qrows) * 8 * Lay::halves; i += cThreads) {
     const int at = i >> 3, hf = at % Lay::halves, row = qrows + (at / Lay::halves) % (cBM - qrows);
@@ -113,11 +121,6 @@ __global__ void __launch_bounds__(cThreads, 1)
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
                  "r"(cTmemCols));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
-  }
-  if (warp == 8 && lane == 0) {
-    prefetch_map(&tm_q);
-    prefetch_map(&tm_k);
-    prefetch_map(&tm_v);
   }
   fence_before();
   __syncthreads();
@@ -489,9 +492,7 @@ static int launch(const Params &p, const CUtensorMap &mq, const CUtensorMap &mk,
     schedule_kernel<cBN><<<1, kSchedThreads, 0, stream>>>(p);
     FFTS_CUDA(cudaGetLastError());
   }
-  chunk_kernel<E, D><<<unsigned(p.ctas), cThreads, ChunkLayout<D>::bytes, stream>>>(mq, mk, mv, p);
-  FFTS_CUDA(cudaGetLastError());
-  return FFTS_OK;
+  return launch_early(chunk_kernel<E, D>, dim3(unsigned(p.ctas)), cThreads, ChunkLayout<D>::bytes, stream, mq, mk, mv, p);
 }
 
 int launch_chunk(const Params &p, bool half, int D, const CUtensorMap &mq, const CUtensorMap &mk, const CUtensorMap &mv,

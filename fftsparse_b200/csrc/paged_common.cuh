@@ -334,6 +334,24 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *map
       : "memory");
 }
 
+// Launches a kernel that may start while the one before it in the stream drains (it begins with griddepcontrol.wait).
+template <typename... Ts>
+static int launch_early(void (*kernel)(Ts...), dim3 grid, int threads, int smem, cudaStream_t stream,
+                        const std::remove_cv_t<Ts> &...args) {
+  cudaLaunchAttribute early{};
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(unsigned(threads));
+  cfg.dynamicSmemBytes = size_t(smem);
+  cfg.stream = stream;
+  cfg.attrs = &early;
+  cfg.numAttrs = 1;
+  FFTS_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
+  return FFTS_OK;
+}
+
 // The kernel of paged_chunk.cu: p with tiles of 256 rows, K and V maps with boxes of up to 128 keys.
 int launch_chunk(const Params &p, bool half, int D, const CUtensorMap &mq, const CUtensorMap &mk, const CUtensorMap &mv,
                  cudaStream_t stream);

@@ -502,101 +502,127 @@ __global__ void __launch_bounds__(kThreads, 2)
 }
 
 // ---------------------------------------------------------------- join
-// For each row o = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s over the shares s, with M taken along as they
-// are read.  A partial is stored 16-byte piece by piece over the rows ([D / 4][128 rows]), so rows that lie
-// side by side in a warp are read and written whole.  A thread has one row and the pieces c0, c0 + step, ...; PB shares x
-// CB pieces are in flight at a time, since the time is that of the rounds through L2.
-template <typename E, int D, int PB, int CB>
-__device__ __forceinline__ void join_rows(const Params &p, uint16_t *dst, int r, int q, int step, int s0,
-                                          int s1, int first_slot) {
-  // in 32 bits: a slot has at most 256 rows of 32 pieces, and there are at most 1024
-  auto slot = [&](int s) { return uint32_t(FFTS_INDEX(s == s0 ? first_slot : 2 * s, 2 * p.ctas)); };
-  const float4 *part = reinterpret_cast<const float4 *>(p.part);
-  for (int c0 = q; c0 < D / 4; c0 += CB * step) {
-    float4 acc[CB];
-#pragma unroll
-    for (int i = 0; i < CB; ++i) acc[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    float m = -INFINITY, l = 0.0f;
-    for (int sb = s0; sb <= s1; sb += PB) {
-      float2 ml[PB];
-      float4 v[PB][CB];
-#pragma unroll
-      for (int k = 0; k < PB; ++k) {
-        ml[k] = make_float2(-INFINITY, 0.0f);
-        if (sb + k <= s1) {
-          const uint32_t at = slot(sb + k);
-          ml[k] = __ldcg(&p.part_ml[at * p.rows + r]);
-#pragma unroll
-          for (int i = 0; i < CB; ++i)
-            if (c0 + i * step < D / 4) v[k][i] = __ldcg(part + ((at * (D / 4) + c0 + i * step) * p.rows + r));
-        }
-      }
-      float top = m;
-#pragma unroll
-      for (int k = 0; k < PB; ++k) top = fmaxf(top, ml[k].x);
-      const float old = m == -INFINITY ? 0.0f : exp2f(m - top);
-      m = top;
-      l *= old;
-#pragma unroll
-      for (int i = 0; i < CB; ++i) {
-        acc[i].x *= old;
-        acc[i].y *= old;
-        acc[i].z *= old;
-        acc[i].w *= old;
-      }
-#pragma unroll
-      for (int k = 0; k < PB; ++k) {
-        if (ml[k].x == -INFINITY) continue;  // no share, or one whose keys the row does not see: o = 0, l = 0
-        const float f = exp2f(ml[k].x - top);
-        l = fmaf(f, ml[k].y, l);
-#pragma unroll
-        for (int i = 0; i < CB; ++i)
-          if (c0 + i * step < D / 4) {
-            acc[i].x = fmaf(f, v[k][i].x, acc[i].x);
-            acc[i].y = fmaf(f, v[k][i].y, acc[i].y);
-            acc[i].z = fmaf(f, v[k][i].z, acc[i].z);
-            acc[i].w = fmaf(f, v[k][i].w, acc[i].w);
-          }
-      }
-    }
-    const float inv_l = l > 0.0f ? 1.0f / l : 0.0f;
-#pragma unroll
-    for (int i = 0; i < CB; ++i)
-      if (c0 + i * step < D / 4) {
-        uint2 o = make_uint2(0u, 0u);
-        if (l > 0.0f)
-          o = make_uint2(Num<E>::pack(acc[i].x * inv_l, acc[i].y * inv_l), Num<E>::pack(acc[i].z * inv_l, acc[i].w * inv_l));
-        *reinterpret_cast<uint2 *>(dst + (c0 + i * step) * 4) = o;
-      }
-  }
-}
+// Blocks (s0, y): the (q tile, head) that share s0 begins and others go on with, the pieces of many rows by turns.  For each row
+// o = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s over the shares s, with M taken along as they are read.  A
+// partial is stored 16-byte piece by piece over the rows ([D / 4][rows]), so neighbouring threads, on neighbouring
+// rows, read and write whole sectors.  The time is that of the rounds through L2: a thread has four pieces
+// in flight, and where a tile has few rows (decoding), groups of threads take the shares in turn and meet in
+// shared memory, in the order of the groups.
+constexpr int kJoinThreads = 512;
+constexpr int kJoinBlocks = 2;  // 1, 2, 4: 16.5, 11.5, 11.2 us after ragged chunks, 4.5, 4.4, 5.7 us after 64 decoding requests
 
-// Block (s0, y): the (q tile, head) that share s0 begins; the pieces of a row go round the blocks of y and
-// the threads that its rows leave.
-constexpr int kJoinThreads = 128;
-constexpr int kJoinBlocks = 16;
+// (m, l, o) of some shares, o a piece of a row; m = -inf: none of them sees a key.
+struct Part {
+  float m, l;
+  float4 o;
+  // the weight of a part with maximum mm in a sum scaled to top
+  static __device__ __forceinline__ float weight(float mm, float top) { return mm == -INFINITY ? 0.0f : exp2f(mm - top); }
+  __device__ __forceinline__ void scale(float f) {
+    l *= f;
+    o.x *= f;
+    o.y *= f;
+    o.z *= f;
+    o.w *= f;
+  }
+  __device__ __forceinline__ void add(float f, float ll, const float4 &v) {
+    l = fmaf(f, ll, l);
+    o.x = fmaf(f, v.x, o.x);
+    o.y = fmaf(f, v.y, o.y);
+    o.z = fmaf(f, v.z, o.z);
+    o.w = fmaf(f, v.w, o.w);
+  }
+};
 
 template <typename E, int D>
-__global__ void __launch_bounds__(kJoinThreads, 8) join_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(kJoinThreads, 2) join_kernel(const __grid_constant__ Params p) {
+  __shared__ Part met[kJoinThreads];
   asm volatile("griddepcontrol.wait;" ::: "memory");  // launched early: attn_kernel's stores are visible from here
-  const int s0 = int(blockIdx.x);
+  const int s0 = int(blockIdx.x), tid = int(threadIdx.x);
   const Cut cut = p.cuts[s0];
   if (cut.nrows == 0) return;
-  int rows = 1;  // threads side by side on the rows
-  while (rows < cut.nrows && rows < kJoinThreads) rows <<= 1;
-  const int per_block = kJoinThreads / rows;
-  const int q = int(blockIdx.y) * per_block + int(threadIdx.x) / rows, step = kJoinBlocks * per_block;
-  if (q >= D / 4) return;
-  for (int r = int(threadIdx.x) % rows; r < cut.nrows; r += rows) {
+  int rows = 1;
+  while (rows < cut.nrows) rows <<= 1;
+  const int items = rows * (D / 4);  // (piece, row), rows side by side
+  const float4 *part = reinterpret_cast<const float4 *>(p.part);
+  auto store = [&](int r, int piece, const Part &t) {
     const int tl = r / p.G, hg = r - tl * p.G;
     if (!FFTS_IN_RANGE(cut.tok0 + tl, p.T)) return;
-    uint16_t *dst = p.out + int64_t(cut.tok0 + tl) * p.os_t + int64_t(cut.head0 + hg) * p.os_h;
-    // few rows: one or two pieces per thread and often many shares; many rows: the other way round
-    if (rows <= 16)
-      join_rows<E, D, 4, 1>(p, dst, r, q, step, s0, cut.s1, cut.first_slot);
-    else
-      join_rows<E, D, 2, 2>(p, dst, r, q, step, s0, cut.s1, cut.first_slot);
+    const float inv_l = t.l > 0.0f ? 1.0f / t.l : 0.0f;
+    uint2 o = make_uint2(0u, 0u);
+    if (t.l > 0.0f)
+      o = make_uint2(Num<E>::pack(t.o.x * inv_l, t.o.y * inv_l), Num<E>::pack(t.o.z * inv_l, t.o.w * inv_l));
+    *reinterpret_cast<uint2 *>(p.out + int64_t(cut.tok0 + tl) * p.os_t + int64_t(cut.head0 + hg) * p.os_h + piece * 4) = o;
+  };
+  // pieces piece + i * step (i < JP) of row r over shares s, s + by, ..., JS at a time; indices in 32 bits: at
+  // most 1024 slots of 256 rows of 32 pieces
+  auto gather = [&](auto js, auto jp, Part *t, int r, int piece, int step, int s, int by) {
+    constexpr int JS = decltype(js)::value, JP = decltype(jp)::value;
+    for (; s <= cut.s1; s += JS * by) {
+      float2 ml[JS];
+      float4 v[JS][JP];
+#pragma unroll
+      for (int k = 0; k < JS; ++k) {
+        ml[k] = make_float2(-INFINITY, 0.0f);
+        const int sk = s + k * by;
+        if (sk > cut.s1) continue;
+        const uint32_t at = uint32_t(FFTS_INDEX(sk == s0 ? cut.first_slot : 2 * sk, 2 * p.ctas));
+        ml[k] = __ldcg(&p.part_ml[at * p.rows + r]);
+#pragma unroll
+        for (int i = 0; i < JP; ++i)
+          if (piece + i * step < D / 4) v[k][i] = __ldcg(part + ((at * (D / 4) + piece + i * step) * p.rows + r));
+      }
+      float top = t[0].m;
+#pragma unroll
+      for (int k = 0; k < JS; ++k) top = fmaxf(top, ml[k].x);
+      const float old = Part::weight(t[0].m, top);
+#pragma unroll
+      for (int i = 0; i < JP; ++i) {
+        t[i].m = top;
+        t[i].scale(old);
+      }
+#pragma unroll
+      for (int k = 0; k < JS; ++k) {
+        if (ml[k].x == -INFINITY) continue;  // no share, or one whose keys the row does not see
+        const float f = exp2f(ml[k].x - top);
+#pragma unroll
+        for (int i = 0; i < JP; ++i)
+          if (piece + i * step < D / 4) t[i].add(f, ml[k].y, v[k][i]);
+      }
+    }
+  };
+  const Part none{-INFINITY, 0.0f, make_float4(0.0f, 0.0f, 0.0f, 0.0f)};
+  if (items >= kJoinThreads) {
+    const int step = kJoinBlocks * (kJoinThreads / rows);  // pieces the blocks cover at a time
+    const int r = tid % rows;
+    if (r >= cut.nrows) return;
+    constexpr int JP = 2;
+    for (int piece = int(blockIdx.y) + kJoinBlocks * (tid / rows); piece < D / 4; piece += JP * step) {
+      Part t[JP];
+#pragma unroll
+      for (int i = 0; i < JP; ++i) t[i] = none;
+      gather(std::integral_constant<int, 2>{}, std::integral_constant<int, JP>{}, t, r, piece, step, s0, 1);
+#pragma unroll
+      for (int i = 0; i < JP; ++i)
+        if (piece + i * step < D / 4) store(r, piece + i * step, t[i]);
+    }
+    return;
   }
+  if (blockIdx.y > 0) return;
+  const int groups = kJoinThreads / items, g = tid / items, r = tid % rows, piece = tid % items / rows;
+  Part t = none;
+  if (r < cut.nrows)
+    gather(std::integral_constant<int, 4>{}, std::integral_constant<int, 1>{}, &t, r, piece, 1, s0 + g, groups);
+  met[tid] = t;
+  __syncthreads();
+  if (g > 0 || r >= cut.nrows) return;
+  float top = -INFINITY;
+  for (int k = 0; k < groups; ++k) top = fmaxf(top, met[k * items + tid].m);
+  Part sum = none;
+  for (int k = 0; k < groups; ++k) {
+    const Part &q = met[k * items + tid];
+    sum.add(Part::weight(q.m, top), q.l, q.o);
+  }
+  store(r, piece, sum);
 }
 
 // ---------------------------------------------------------------- host side

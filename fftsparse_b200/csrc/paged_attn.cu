@@ -48,6 +48,7 @@ constexpr int kKStages = 3, kVStages = 2;
 constexpr int kTmemCols = 256;  // S0, S1 (64 columns each), O (D): two CTAs fill an SM's 512
 constexpr uint32_t kTmemO = 128;
 constexpr int kOverhead = 3;    // of 2, 3 and 4: 16 ragged chunks 67, 59, 57 us, 64 decoding requests 155.4, 155.8, 157.4 us
+constexpr int kFewRows = 32;    // of a q tile: loaded one by one
 constexpr int64_t kLongKeys = 16384;
 constexpr double kWaitSeconds = 2.0, kDrainSeconds = 4.0;
 
@@ -132,11 +133,9 @@ __global__ void __launch_bounds__(kThreads, 2)
     if (threadIdx.x == 0) p.cuts[blockIdx.x].nrows = 0;
     return;
   }
-  // rows no Q load fills: zeros, so that they stay finite
-  for (int i = threadIdx.x; i < (kBM - qrows) * 8 * Lay::halves; i += kThreads) {
-    const int row = qrows + (i >> 3) / Lay::halves, hf = (i >> 3) % Lay::halves;
-    *reinterpret_cast<uint4 *>(smem + Lay::q + hf * Lay::q_half + row * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
-  }
+  // rows of Q that no load fills stay zeros
+  for (int i = threadIdx.x; i < Lay::q_bytes / 16; i += kThreads)
+    *reinterpret_cast<uint4 *>(smem + Lay::q + i * 16) = make_uint4(0, 0, 0, 0);
   fence_proxy_async();  // TMA writes over the scratch, the MMAs read the zeros
   if (warp == 5) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
@@ -183,6 +182,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     };
     bool ok = true;
     int nk = 0, nv = 0, nq = 0;  // loads issued
+    int filled = 0;              // rows of Q that are not zeros
     auto load = [&](const Load &l, bool is_k) {
       const int n = is_k ? nk : nv;
       const int stages = is_k ? kKStages : kVStages, s = n % stages;
@@ -199,16 +199,37 @@ __global__ void __launch_bounds__(kThreads, 2)
     bool more = fetch(cur);
     while (more && ok) {
       const bool cur_fresh = fresh;
-      const int tok0 = w.t.tok0, qh = w.h * p.G;
+      const int tok0 = w.t.tok0, qh = w.h * p.G, rows = w.t.ntok * p.G;
       // K(n), V(n - 1); a new segment's Q waits for the last S of the one before, so V(n - 1) goes first
       if (cur_fresh && nk > 0) load(prev, false);
       load(cur, true);
       if (cur_fresh && ok) {
         ok = __all_sync(0xffffffffu, mbar_wait(bar(BQE), (nq & 1) ^ 1, abort_flag, p.wait_cycles));
-        if (ok && lane == 0) {
-          mbar_arrive_tx(bar(BQF), uint32_t(qrows * D * 2));
-          for (int hf = 0; hf < Lay::halves; ++hf)
-            tma_load_3d(sbase + Lay::q + hf * Lay::q_half, &tm_q, bar(BQF), hf * 64, qh, tok0);
+        if (ok && rows <= kFewRows) {
+          // Decoding: the few rows themselves, and zeros behind them.  A box would bring the rows of other
+          // requests along, whose products cost power: 64 requests' step ran at 1016 W, 1.43 GHz and 179 us.
+          constexpr int kVecs = D / 8;
+          for (int i = lane; i < rows * kVecs; i += 32) {
+            const int r = i / kVecs, c = i % kVecs;
+            const int tok = FFTS_INDEX(tok0 + r / p.G, p.T);
+            *reinterpret_cast<uint4 *>(smem + Lay::q + (c >> 3) * Lay::q_half + r * 128 + (((c & 7) ^ (r & 7)) << 4)) =
+                *reinterpret_cast<const uint4 *>(p.q + int64_t(tok) * p.qs_t + int64_t(qh + r % p.G) * p.qs_h + c * 8);
+          }
+          for (int i = rows * kVecs + lane; i < filled * kVecs; i += 32) {
+            const int r = i / kVecs, c = i % kVecs;
+            *reinterpret_cast<uint4 *>(smem + Lay::q + (c >> 3) * Lay::q_half + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+          }
+          filled = rows;
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(BQF));
+        } else if (ok) {
+          if (lane == 0) {
+            mbar_arrive_tx(bar(BQF), uint32_t(qrows * D * 2));
+            for (int hf = 0; hf < Lay::halves; ++hf)
+              tma_load_3d(sbase + Lay::q + hf * Lay::q_half, &tm_q, bar(BQF), hf * 64, qh, tok0);
+          }
+          filled = qrows;
         }
         if (ok) ++nq;
       }
@@ -313,10 +334,11 @@ __global__ void __launch_bounds__(kThreads, 2)
     while (ok && w.segment()) {
       const Keys g = w.g;
       const int nrows = w.t.ntok * p.G;
-      const bool active = warp * 32 < nrows;
+      const bool active = warp * 32 < nrows, live = r < nrows;
       // rows of no token take the last token's mask; nobody reads them
       const int pos = w.t.pos0 + min(tl, w.t.ntok - 1);
-      float m_ref = -INFINITY, l_run = 0.0f;
+      // and their P is 0, by an offset of -inf
+      float m_ref = live ? -INFINITY : 0.0f, l_run = 0.0f;
       for (int j = w.j0; j < w.j1; ++j, ++n) {
         const int b = n & 1;
         const uint32_t parity = (n >> 1) & 1;
@@ -377,7 +399,7 @@ __global__ void __launch_bounds__(kThreads, 2)
             }
           };
           if (fast) {
-            const float moff = m_ref * p.scale_log2;
+            const float moff = live ? m_ref * p.scale_log2 : INFINITY;
             exp_half(0, make_float2(-moff, -moff));
             tmem_wait_ld();
             mask_high();
@@ -401,7 +423,7 @@ __global__ void __launch_bounds__(kThreads, 2)
               alpha = m_ref == -INFINITY ? 0.0f : fast_exp2((m_ref - mx) * p.scale_log2);
               m_ref = mx;
             }
-            const float moff = (m_ref == -INFINITY ? 0.0f : m_ref) * p.scale_log2;
+            const float moff = live ? (m_ref == -INFINITY ? 0.0f : m_ref) * p.scale_log2 : INFINITY;
             exp_half(0, make_float2(-moff, -moff));
             exp_half(1, make_float2(-moff, -moff));
           }
@@ -444,7 +466,6 @@ __global__ void __launch_bounds__(kThreads, 2)
       fence_after();
       if (active) {
         const bool whole = w.j0 == 0 && w.j1 == g.n;
-        const bool live = r < nrows;
         const int slot = 2 * int(blockIdx.x) + (first_seg ? 0 : 1);
         const float inv_l = l_run > 0.0f ? 1.0f / l_run : 0.0f;
         uint16_t *dst = p.out + int64_t(w.t.tok0 + tl) * p.os_t + int64_t(w.h * p.G + hg) * p.os_h;
@@ -763,6 +784,9 @@ int paged_attn(const ffts_paged_attn_args &a, cudaStream_t stream) {
   p.kv_lens = a.kv_lens;
   p.window = int(std::min<int64_t>(a.window, int64_t(1) << 30));
   p.sinks = a.window > 0 ? int(std::min<int64_t>(a.sinks, int64_t(1) << 30)) : 0;
+  p.q = static_cast<const uint16_t *>(a.q);
+  p.qs_t = qs[0];
+  p.qs_h = qs[1];
   p.out = static_cast<uint16_t *>(a.out);
   p.os_t = os[0];
   p.os_h = os[1];

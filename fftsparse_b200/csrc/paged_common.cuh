@@ -39,6 +39,8 @@ struct Params {
   int width, n_pages, ps_shift;
   const int32_t *cu_q, *kv_lens;
   int window, sinks;          // window 0: none
+  const uint16_t *q;
+  int64_t qs_t, qs_h;
   uint16_t *out;
   int64_t os_t, os_h;
   float scale_log2;

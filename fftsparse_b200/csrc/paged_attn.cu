@@ -49,6 +49,9 @@ constexpr int kTmemCols = 256;  // S0, S1 (64 columns each), O (D): two CTAs fil
 constexpr uint32_t kTmemO = 128;
 constexpr int kOverhead = 3;    // of 2, 3 and 4: 16 ragged chunks 67, 59, 57 us, 64 decoding requests 155.4, 155.8, 157.4 us
 constexpr int kFewRows = 32;    // of a q tile: loaded one by one
+// With so few rows the products are of 64 rows, whose first 16 lie in the same TMEM lanes 0-15 as those of 128 rows: half the
+// power of products that are mostly of zeros (64 requests' step 169 -> 164 us under the power cap, 2 x 131072 keys 180 -> 172).
+constexpr int kSmallRows = 16;
 constexpr int64_t kLongKeys = 16384;
 constexpr double kWaitSeconds = 2.0, kDrainSeconds = 4.0;
 
@@ -258,15 +261,17 @@ __global__ void __launch_bounds__(kThreads, 2)
     // ============================================================ MMA issuer (one thread)
     if (elect_one()) {
       constexpr uint32_t idS = idesc(Num<E>::fmt, false, kBN), idPV = idesc(Num<E>::fmt, true, D);
+      constexpr uint32_t idS64 = idesc(Num<E>::fmt, false, kBN, 64), idPV64 = idesc(Num<E>::fmt, true, D, 64);
       const uint64_t dk_ = smem_desc(sbase, 16, 1024), dv_ = smem_desc(sbase, Lay::kv_half, 1024);
       const uint32_t dk_hi = uint32_t(dk_ >> 32), dv_hi = uint32_t(dv_ >> 32);
       const uint32_t dq = uint32_t(dk_) + (Lay::q >> 4), dk0 = uint32_t(dk_) + (Lay::k >> 4),
                      dv0 = uint32_t(dv_) + (Lay::v >> 4);
       bool ok = true;
       // S runs up to two tiles ahead of PV.  s_left: S tiles left in the walked segment; the PV side
-      // needs only to know which tiles begin a segment (bit n % 32 of firsts).
+      // needs only to know which tiles begin a segment and which have few rows (bit n % 32 of firsts and smalls).
       int s = 0, seg = 0, s_left = 0;
-      uint32_t firsts = 0;
+      uint32_t firsts = 0, smalls = 0;
+      bool small = false;
       bool more = w.segment();
       for (int n = 0; ok && (more || n < s); ++n) {
         while (more && s < n + 2) {
@@ -277,6 +282,7 @@ __global__ void __launch_bounds__(kThreads, 2)
             ok = mbar_wait(bar(BQF), seg & 1, abort_flag, p.wait_cycles);
             if (!ok) break;
             s_left = w.j1 - w.j0;
+            small = w.t.ntok * p.G <= kSmallRows;
             ++seg;
           }
           const int ks = s % kKStages;
@@ -289,10 +295,11 @@ __global__ void __launch_bounds__(kThreads, 2)
           for (int kk = 0; kk < D / 16; ++kk) {
             const uint32_t qoff = ((kk >> 2) * Lay::q_half + (kk & 3) * 32) >> 4;
             const uint32_t koff = ((kk >> 2) * Lay::kv_half + (kk & 3) * 32) >> 4;
-            umma_ss(td, dq + qoff, dk_hi, dk + koff, dk_hi, idS, kk > 0);
+            umma_ss(td, dq + qoff, dk_hi, dk + koff, dk_hi, small ? idS64 : idS, kk > 0);
           }
           umma_commit(bar(BSF + (s & 1)));
           umma_commit(bar(BKE + ks));
+          smalls = (smalls & ~(1u << (s & 31))) | (uint32_t(small) << (s & 31));
           if (--s_left == 0) {
             umma_commit(bar(BQE));
             more = w.segment();
@@ -311,7 +318,8 @@ __global__ void __launch_bounds__(kThreads, 2)
         const uint32_t pt = tmem + b * kBN;  // P(n): pairs in the first 32 columns of S buffer n % 2
 #pragma unroll
         for (int kk = 0; kk < kBN / 16; ++kk)
-          umma_ts(tm_o, pt + kk * 8, dv + ((kk * 2048) >> 4), dv_hi, idPV, !first || kk > 0);
+          umma_ts(tm_o, pt + kk * 8, dv + ((kk * 2048) >> 4), dv_hi, (smalls >> (n & 31)) & 1u ? idPV64 : idPV,
+                  !first || kk > 0);
         umma_commit(bar(BPV + b));
       }
       if (!ok) {

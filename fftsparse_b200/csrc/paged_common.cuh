@@ -269,9 +269,9 @@ struct Num<__half> {
   }
 };
 
-constexpr uint32_t idesc(uint32_t fmt, bool b_mn_major, int n) {
+constexpr uint32_t idesc(uint32_t fmt, bool b_mn_major, int n, int m = 128) {
   return (1u << 4) | (fmt << 7) | (fmt << 10) | (b_mn_major ? (1u << 16) : 0u) | (uint32_t(n >> 3) << 17) |
-         (uint32_t(128 >> 4) << 24);
+         (uint32_t(m >> 4) << 24);
 }
 
 // True in one thread of the (converged) warp.  The compiler knows that no other thread is in the branch behind it, so

@@ -780,6 +780,7 @@ int paged_attn(const ffts_paged_attn_args &a, cudaStream_t stream) {
   FFTS_REQUIRE(a.workspace_bytes >= paged_workspace_bytes(T, R, H, Hkv, D), "paged_attn: workspace too small");
   const int64_t G = H / Hkv;
   const Space sp(T, R, G, D);
+  FFTS_REQUIRE(sp.max_tiles < (int64_t(1) << 31) - 1, "paged_attn: too many q tiles");
   uint8_t *base = static_cast<uint8_t *>(a.workspace);
   Params p{};
   p.T = int(T); p.R = int(R); p.H = int(H); p.Hkv = int(Hkv); p.G = int(G); p.tpt = int(kBM / G);

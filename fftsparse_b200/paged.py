@@ -83,7 +83,8 @@ def _check_heads(name: str, t: torch.Tensor, dtype, device):
     st, sh, sd = t.stride()
     if sd != 1:
         raise ValueError(f"{name} must be contiguous in the head dimension")
-    return st, sh
+    n, h, d = t.shape
+    return (st if n > 1 else h * d), (sh if h > 1 else d)  # a single row's stride says nothing
 
 
 def _check_pool(k_pages: torch.Tensor, v_pages: torch.Tensor, dtype, device):
@@ -99,6 +100,10 @@ def _check_pool(k_pages: torch.Tensor, v_pages: torch.Tensor, dtype, device):
     *vs, vd = v_pages.stride()
     if kd != 1 or vd != 1:
         raise ValueError("k_pages and v_pages must be contiguous in the head dimension")
+    if 1 in k_pages.shape:  # the stride of a single page, head or row says nothing
+        P, h, n, d = k_pages.shape
+        packed = (h * n * d, n * d, d)
+        ks, vs = ([s if m > 1 else c for s, m, c in zip(st, (P, h, n), packed)] for st in (ks, vs))
     return ks, vs
 
 
@@ -168,8 +173,9 @@ def rotary_inv_freq(rotary_dim: int, base: float = 10000.0, scaling: Optional[di
       dynamic  base grown to base (factor L / L0 - factor + 1)^(d / (d - 2)), L = max(seq_len, L0)
       llama3   f_i / factor for wavelengths above L0 / low_freq_factor, f_i below L0 / high_freq_factor, a linear
                blend between
-      yarn     f_i / factor and f_i blended over the channels that turn beta_slow to beta_fast times within L0;
-               attn_factor = attention_factor or 0.1 ln(factor) + 1
+      yarn     f_i / factor and f_i blended over the channels that turn beta_slow to beta_fast times within L0
+               (whole channels unless truncate is false); attn_factor = attention_factor, or m(mscale) / m(mscale_all_dim)
+               where both are given, or m(1), with m(x) = 0.1 x ln(factor) + 1
 
     with L0 = ``original_max_position_embeddings``.  Computed in 64 bits, rounded once.
     """
@@ -206,12 +212,18 @@ def rotary_inv_freq(rotary_dim: int, base: float = 10000.0, scaling: Optional[di
         def channel(turns):  # the pair that turns so often within L0
             return d * math.log(L0 / (turns * 2.0 * math.pi)) / (2.0 * math.log(base))
 
-        lo = max(math.floor(channel(float(scaling.get("beta_fast", 32.0)))), 0)
-        hi = min(math.ceil(channel(float(scaling.get("beta_slow", 1.0)))), d - 1)
+        lo, hi = (channel(float(scaling.get(k) or v)) for k, v in (("beta_fast", 32.0), ("beta_slow", 1.0)))
+        if scaling.get("truncate", True):
+            lo, hi = math.floor(lo), math.ceil(hi)
+        lo, hi = max(lo, 0), min(hi, d - 1)
         slow = ((i / 2 - lo) / max(hi - lo, 1e-3)).clamp(0.0, 1.0)
         f = slow * f / s + (1.0 - slow) * f
-        given = scaling.get("attention_factor")
-        attn = float(given) if given is not None else (0.1 * math.log(s) + 1.0 if s > 1.0 else 1.0)
+
+        def m(x):
+            return 0.1 * x * math.log(s) + 1.0 if s > 1.0 else 1.0
+
+        given, ms, ms_all = (scaling.get(k) for k in ("attention_factor", "mscale", "mscale_all_dim"))
+        attn = float(given) if given is not None else (m(float(ms)) / m(float(ms_all)) if ms and ms_all else m(1.0))
     elif kind not in ("default", "dynamic"):
         raise ValueError(f"unknown rope scaling '{kind}'")
     return f.to(torch.float32).to(device), attn
@@ -296,7 +308,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     request (the work does not grow with the rest); pages it does not see may be gone from the table.  Tokens that see
     nothing (kv_len 0) get zeros.  Returns [T, H, D] (or fills ``out``); rows of no request are not written.
 
-    A bounded wait that runs out in the kernel raises WaitTimeout at a later call or at ``check_status()``.
+    A bounded wait that runs out in the kernel raises WaitTimeout at a later call or at ``check_status()``.  Before a
+    capture into a CUDA graph make one call outside of it (it sets up the device's status word).
     """
     dev, dt = q.device, q.dtype
     if dt not in _DTYPES:

@@ -405,6 +405,48 @@ def test_strided_q_and_out():
     assert bool((out[..., :16] == 5.0).all()) and bool((out[..., 144:] == 5.0).all())
 
 
+def test_requests_that_share_pages():
+    """Two requests with a common prefix in the same pages, and one listed twice in the batch."""
+    b = Batch([(128, 5), (128, 1), (130, 70)], 8, 2, 128, BF, 16)
+    b.table[1, :8] = b.table[0, :8]
+    b.k[1] = torch.cat([b.k[0][:, :128], b.k[1][:, 128:]], 1)
+    b.v[1] = torch.cat([b.v[0][:, :128], b.v[1][:, 128:]], 1)
+    b.check(b.run())
+    twice = torch.cat([b.table, b.table[2:]])
+    got = F.paged_attention(torch.cat([b.q, b.q[6:]]), b.kp, b.vp, twice, ints([0, 5, 6, 76, 146]), ints([133, 129, 200, 200]))
+    b.check(got)
+    b.q, b.lens, b.k, b.v = b.q[6:], b.lens[2:], b.k[2:], b.v[2:]
+    b.check(got[76:])
+
+
+@pytest.mark.parametrize("width", [0, 20000])
+def test_infinities_and_nan_stay_in_their_rows(width):
+    """A request whose values are broken, and a broken row of q, leave every other row as it was."""
+    lens = [(300, 40), (90, 200), (700, 100)]
+    b = Batch(lens, 8, 2, 128, BF, 16, width=width)
+    want = b.run().clone()
+    b.vp[b.table[1, :19].long()] = math.inf
+    b.kp[b.table[1, :19].long()] = NAN
+    b.q[5, 3] = NAN
+    b.q[250] = math.inf
+    got = b.run()
+    same = torch.ones(340, 8, dtype=torch.bool, device="cuda")
+    same[40:240] = False
+    same[5, 3] = False
+    same[250] = False
+    assert torch.equal(got[same], want[same])
+
+
+def test_strides_of_single_rows_do_not_matter():
+    b = Batch([(40, 1)], 1, 1, 64, BF, 64)
+    q = torch.zeros(3, 1, 67, dtype=BF, device="cuda")
+    q = q.as_strided((1, 1, 64), (67, 5, 1))
+    q.copy_(b.q)
+    page = int(b.table[0, 0])
+    kp, vp = (x[page:page + 1].as_strided((1, 1, 64, 64), (3, 1, 64, 1), x[page].storage_offset()) for x in (b.kp, b.vp))
+    b.check(F.paged_attention(q, kp, vp, ints([[0]]), b.cu, b.kv))
+
+
 def test_pool_offsets_beyond_32_bits():
     """A pool of more than 2^32 bytes and 2^31 elements, its pages in use at both ends."""
     P, Hkv, page, D = 33000, 8, 64, 128

@@ -140,6 +140,10 @@ def test_rotary_frequencies_of_each_scaling():
         ramp = min(1.0, max(0.0, (i - lo) / (hi - lo)))
         want.append(x / 4 * ramp + x * (1 - ramp))
     assert near(t, want) and abs(a - (0.1 * math.log(4.0) + 1.0)) < 1e-12
+    yarn = {"rope_type": "yarn", "factor": 4.0, "original_max_position_embeddings": L0}
+    assert got(dict(yarn, attention_factor=1.5))[1] == 1.5
+    m = [0.1 * x * math.log(4.0) + 1.0 for x in (0.7, 0.4)]
+    assert abs(got(dict(yarn, mscale=0.7, mscale_all_dim=0.4))[1] - m[0] / m[1]) < 1e-12
 
 
 @pytest.mark.parametrize("args", [(0, 1e4, None), (15, 1e4, None), (64, 1e4, {"rope_type": "bogus"}),

@@ -17,6 +17,12 @@
 // A commit tracks all earlier products of the issuing thread, so S_X(n + 1) being there means that PV_X(n) is
 // complete: O may be rescaled then, and only a segment's end waits for its last PV.
 // Every wait is bounded.
+//
+// 2048 tokens of 32 / 8 heads over 32768 cached: 0.98 ms, 1.15 PFLOP/s (0.70 of the measured bf16 burst), 1.16 ms
+// once the
+// power cap holds the clock at 1.5 GHz.  A key tile of both halves takes about 3000 clocks, 2048 of them products: a
+// half's softmax (about 1850 clocks: scores read and looked through 450, exponentials 1400) and its two products
+// follow one another, and the other half's fill the gap only in part.
 
 #include <algorithm>
 

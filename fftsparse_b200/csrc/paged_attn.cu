@@ -514,8 +514,8 @@ __global__ void __launch_bounds__(kThreads, 2)
         if (live && !whole && FFTS_IN_RANGE(slot, 2 * p.ctas))
           p.part_ml[int64_t(slot) * kBM + r] = make_float2(m_ref * p.scale_log2, l_run);
       }
-      // the share that holds the first key tile leaves a note for the join
-      if (w.j0 == 0 && w.j1 < g.n && r == 0 && FFTS_IN_RANGE(blockIdx.x, p.ctas)) {
+      // the share that opens a (q tile, head) and does not end it leaves a note for the join
+      if (w.opens && w.j1 - w.j0 < g.n && r == 0 && FFTS_IN_RANGE(blockIdx.x, p.ctas)) {
         Cut cut;
         cut.tok0 = w.t.tok0;
         cut.nrows = nrows;
@@ -827,7 +827,7 @@ int paged_attn(const ffts_paged_attn_args &a, cudaStream_t stream) {
   // The larger tiles of paged_chunk.cu: where requests fill them on average and their key lists, as far as the table
   // and
   // the window bound them, are long enough to pay for filling and draining one pipeline per SM instead of two.
-  // 2048 tokens of 32 / 8 heads over 32768 cached: 1.19 ms against 1.37 (0.98 and 1.11 before the power cap sets
+  // 2048 tokens of 32 / 8 heads over 32768 cached: 1.09 ms against 1.37 (0.98 and 1.11 before the power cap sets
   // in); 512 over 16384: 129 us both; 16 ragged chunks over up to 16384: 72 against 59.
   int64_t span = width * page_size;
   if (p.window > 0) span = std::min(span, int64_t(p.window) + p.sinks + T / R);

@@ -462,8 +462,8 @@ __global__ void __launch_bounds__(cThreads, 1)
         if (live && !whole && FFTS_IN_RANGE(slot, 2 * p.ctas))
           p.part_ml[int64_t(slot) * (2 * cBM) + row] = make_float2(m_ref * p.scale_log2, l_run);
       }
-      // the share that holds the first key tile leaves a note for the join
-      if (w.j0 == 0 && w.j1 < g.n && threadIdx.x == 0 && FFTS_IN_RANGE(blockIdx.x, p.ctas)) {
+      // the share that opens a (q tile, head) and does not end it leaves a note for the join
+      if (w.opens && w.j1 - w.j0 < g.n && threadIdx.x == 0 && FFTS_IN_RANGE(blockIdx.x, p.ctas)) {
         Cut cut;
         cut.tok0 = w.t.tok0;
         cut.nrows = nrows;

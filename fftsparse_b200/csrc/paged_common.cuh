@@ -190,7 +190,12 @@ struct Walk {
   int x;
   Tile t;
   Keys g;
-  int h, j0, j1;         // the segment: head and key tiles [j0, j1) of the g.n
+  // The segment: head and key tiles [j0, j1) of the g.n.  The line runs through a (q tile, head)'s key tiles from
+  // the last ones to the first: a share that begins inside one takes keys from the start on, a share that
+  // ends inside one ends with the last.  So the shares, which run side by side, are at the same keys at their
+  // beginnings and at their ends, and find each other's tiles in L2.
+  int h, j0, j1;
+  bool opens;            // the (q tile, head) begins in this share
   int begin;             // where its (q tile, head) begins, relative to the share (may be negative)
   __device__ __forceinline__ Walk(const Params &prm, const Tile *t_, const long long *c_) : p(prm), tiles(t_), cum(c_) {}
 
@@ -234,9 +239,12 @@ struct Walk {
       rem += to - at;
       done += to - at;
       left -= to - at;
-      j0 = max(0, at - p.overhead);
-      j1 = max(0, to - p.overhead);
-      if (j1 > j0) return true;
+      const int o0 = max(0, at - p.overhead), o1 = max(0, to - p.overhead);
+      if (o1 == o0) continue;
+      opens = o0 == 0;
+      j0 = g.n - o1;
+      j1 = g.n - o0;
+      return true;
     }
     return false;
   }

@@ -204,9 +204,10 @@ def test_shares_cover_every_key_tile_once_and_the_join_finds_its_partials(seed):
             begin, x, h, n = max(s for s in line if s[0] <= u)
             a, b = u - begin, min(n + OVERHEAD, u1 - begin)
             u = begin + b
-            j0, j1 = max(0, a - OVERHEAD), max(0, b - OVERHEAD)
-            if j0 == j1:
+            o0, o1 = max(0, a - OVERHEAD), max(0, b - OVERHEAD)
+            if o0 == o1:
                 continue
+            j0, j1 = n - o1, n - o0  # a share that opens a (q tile, head) takes the last keys
             for j in range(j0, j1):
                 assert (x, h, j) not in covered
                 covered.add((x, h, j))

@@ -32,13 +32,11 @@
 //               would reach the sum.
 // Every mbarrier wait is bounded (a status code instead of a hang).
 //
-// Decoding is bound by HBM, or by the power cap before it: 64 requests of 512 to 16384 keys, 32 / 8 heads, pages of
-// 16: 155 us
-// at 1.9 GHz (6.3 TB/s, 0.96 of the measured copy), 161 to 165 us a step in a long loop; 2 x 131072 keys 162 us (1.0)
-// and
-// 170.  Chunks are bound by the tensor core and the softmax around it: a key tile takes about 1600 clocks in each of
-// an SM's
-// two CTAs, 640 of them its products (a 64-key S reads 48 KB of shared memory, 384 clocks for 256 of products).
+// Decoding is bound by HBM, or by the power cap before it: 64 requests of 512 to 16384 keys, 32 / 8 heads, pages
+// of 16: 155 us at 1.9 GHz (6.3 TB/s, 0.96 of the measured copy), 161 to 165 us a step in a long loop; 2 x 131072
+// keys 162 us (1.0) and 170.  Chunks are bound by the tensor core and the softmax around it: a key tile takes
+// about 1600 clocks in each of an SM's two CTAs, 640 of them its products (a 64-key S reads 48 KB of shared
+// memory, 384 clocks for 256 of products).
 
 #include <cudaTypedefs.h>
 
@@ -55,12 +53,12 @@ constexpr int kThreads = 192;
 constexpr int kKStages = 3, kVStages = 2;
 constexpr int kTmemCols = 256;  // S0, S1 (64 columns each), O (D): two CTAs fill an SM's 512
 constexpr uint32_t kTmemO = 128;
-constexpr int kOverhead = 3;    // of 2, 3 and 4: 16 ragged chunks 67, 59, 57 us, 64 decoding requests 155.4, 155.8, 157.4 us
+// 2, 3 and 4: 16 ragged chunks 67, 59, 57 us, 64 decoding requests 155.4, 155.8, 157.4 us
+constexpr int kOverhead = 3;
 constexpr int kFewRows = 32;    // of a q tile: loaded one by one
-// With so few rows the products are of 64 rows, whose first 16 lie in the same TMEM lanes 0-15 as those of 128 rows:
-// half the
-// power of products that are mostly of zeros (64 requests' step 169 -> 164 us under the power cap, 2 x 131072 keys
-// 180 -> 172).
+// With so few rows the products are of 64 rows, whose first 16 lie in the same TMEM lanes 0-15 as those of 128
+// rows: half the power of products that are mostly of zeros (64 requests' step 169 -> 164 us under the power cap,
+// 2 x 131072 keys 180 -> 172).
 constexpr int kSmallRows = 16;
 constexpr int64_t kLongKeys = 16384;
 constexpr double kWaitSeconds = 2.0, kDrainSeconds = 4.0;
@@ -541,15 +539,15 @@ __global__ void __launch_bounds__(kThreads, 2)
 }
 
 // ---------------------------------------------------------------- join
-// Blocks (s0, y): the (q tile, head) that share s0 begins and others go on with, the pieces of many rows by turns. 
-// For each row
-// o = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s over the shares s, with M taken along as they are read.  A
-// partial is stored 16-byte piece by piece over the rows ([D / 4][rows]), so neighbouring threads, on neighbouring
-// rows, read and write whole sectors.  The time is that of the rounds through L2: a thread has four pieces
-// in flight, and where a tile has few rows (decoding), groups of threads take the shares in turn and meet in
-// shared memory, in the order of the groups.
+// Blocks (s0, y): the (q tile, head) that share s0 begins and others go on with, the pieces of many rows by turns.
+// For each row o = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s over the shares s, with M taken along as they are
+// read.  A partial is stored 16-byte piece by piece over the rows ([D / 4][rows]), so neighbouring threads, on
+// neighbouring rows, read and write whole sectors.  The time is that of the rounds through L2: a thread has four
+// pieces in flight, and where a tile has few rows (decoding), groups of threads take the shares in turn and meet
+// in shared memory, in the order of the groups.
 constexpr int kJoinThreads = 512;
-constexpr int kJoinBlocks = 2;  // 1, 2, 4: 16.5, 11.5, 11.2 us after ragged chunks, 4.5, 4.4, 5.7 us after 64 decoding requests
+// 1, 2 and 4 blocks: 16.5, 11.5, 11.2 us after ragged chunks, 4.5, 4.4, 5.7 us after 64 decoding requests
+constexpr int kJoinBlocks = 2;
 
 // (m, l, o) of some shares, o a piece of a row; m = -inf: none of them sees a key.
 struct Part {
@@ -824,11 +822,10 @@ int paged_attn(const ffts_paged_attn_args &a, cudaStream_t stream) {
   if (!rc) rc = device_wait_cycles(kWaitSeconds, &p.wait_cycles);
   if (!rc) rc = device_wait_cycles(kDrainSeconds, &p.drain_cycles);
   if (rc) return rc;
-  // The larger tiles of paged_chunk.cu: where requests fill them on average and their key lists, as far as the table
-  // and
-  // the window bound them, are long enough to pay for filling and draining one pipeline per SM instead of two.
-  // 2048 tokens of 32 / 8 heads over 32768 cached: 1.09 ms against 1.37 (0.98 and 1.11 before the power cap sets
-  // in); 512 over 16384: 129 us both; 16 ragged chunks over up to 16384: 72 against 59.
+  // The larger tiles of paged_chunk.cu: where requests fill them on average and their key lists, as far as the
+  // table and the window bound them, are long enough to pay for filling and draining one pipeline per SM instead
+  // of two. 2048 tokens of 32 / 8 heads over 32768 cached: 1.09 ms against 1.37 (0.98 and 1.11 before the power
+  // cap sets in); 512 over 16384: 129 us both; 16 ragged chunks over up to 16384: 72 against 59.
   int64_t span = width * page_size;
   if (p.window > 0) span = std::min(span, int64_t(p.window) + p.sinks + T / R);
   const bool chunks = T * G >= 2 * kBM * R && span > kLongKeys;

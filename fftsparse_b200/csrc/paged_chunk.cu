@@ -19,10 +19,9 @@
 // Every wait is bounded.
 //
 // 2048 tokens of 32 / 8 heads over 32768 cached: 0.98 ms, 1.15 PFLOP/s (0.70 of the measured bf16 burst), 1.16 ms
-// once the
-// power cap holds the clock at 1.5 GHz.  A key tile of both halves takes about 3000 clocks, 2048 of them products: a
-// half's softmax (about 1850 clocks: scores read and looked through 450, exponentials 1400) and its two products
-// follow one another, and the other half's fill the gap only in part.
+// once the power cap holds the clock at 1.5 GHz.  A key tile of both halves takes about 3000 clocks, 2048 of them
+// products: a half's softmax (about 1850 clocks: scores read and looked through 450, exponentials 1400) and its
+// two products follow one another, and the other half's fill the gap only in part.
 
 #include <algorithm>
 

@@ -178,8 +178,8 @@ __global__ void __launch_bounds__(kSchedThreads) schedule_kernel(const __grid_co
 }
 
 // Walks a share segment by segment; the same in every lane.  Positions are kept relative to the share and to the q
-// tile,
-// in 32 bits: the host refuses a q tile whose heads' line passes 2^31, and a share that did would run for days.
+// tile, in 32 bits: the host refuses a q tile whose heads' line passes 2^31, and a share that did would run for
+// days.
 template <int BN>
 struct Walk {
   const Params &p;

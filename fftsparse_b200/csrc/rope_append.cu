@@ -20,7 +20,8 @@
 namespace ffts {
 namespace ropeapp {
 
-constexpr int kThreads = 128;   // 256: 141.8 us where 128 take 135.8 (32768 tokens, 32 / 8 heads), 19.5 and 17.8 (5001, 28 / 4)
+// 256: 141.8 us where 128 take 135.8 (32768 tokens, 32 / 8 heads), 19.5 and 17.8 (5001 tokens, 28 / 4)
+constexpr int kThreads = 128;
 constexpr int kMaxTokens = 8;   // tokens per CTA (4 and 16: 160 and 135 us, 22.0 and 19.1)
 constexpr int kMaxPairs = 64;   // rd / 2, D <= 128
 

@@ -1,5 +1,6 @@
 """Host side of the paged operators without a GPU: refusals, rotary frequencies and
 the share arithmetic of the paged attention's schedule."""
+import ctypes
 import math
 import random
 
@@ -230,6 +231,18 @@ def test_shares_cover_every_key_tile_once_and_the_join_finds_its_partials(seed):
         assert slots == sorted(s for s, at in wrote.items() if at == (x, h))
         cut.add((x, h))
     assert whole | cut == {(x, h) for _, x, h, _ in line} and not whole & cut
+
+
+def test_codes_stored_into_the_host_word_are_raised_once():
+    from fftsparse_b200 import status as S
+    w = S.StatusWord("cpu")
+    for look in (w.poll_direct, w.poll, w.check):
+        look()  # zero: nothing to report
+        ctypes.c_int32.from_address(w.direct_ptr).value = 11
+        with pytest.raises(S.WaitTimeout, match="paged attention") as exc:
+            look()
+        assert exc.value.code == 11
+        look()  # cleared by the raise
 
 
 @pytest.mark.parametrize("name", ["page_plan", "rope_append", "paged_attn"])

@@ -182,7 +182,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         j = w.j0;
         j1 = w.j1;
       }
-      const int c = key_tile(w.g, j) * kBN + my_box * box;  // first key of the box
+      const int c = w.key(j) * kBN + my_box * box;  // first key of the box
       ++j;
       l.page = -1;
       l.row = c & (ps - 1);
@@ -360,7 +360,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         const uint32_t parity = (n >> 1) & 1;
         if (!__all_sync(0xffffffffu, mbar_wait(bar(BSF + b), parity, abort_flag, p.wait_cycles))) { ok = false; break; }
         fence_after();
-        const int c0 = key_tile(g, j) * kBN;
+        const int c0 = w.key(j) * kBN;
         if (c0 + kBN > g.hi || (c0 < g.lo && c0 + kBN > p.sinks)) {
           // V rows that no row sees
           if (!__all_sync(0xffffffffu, mbar_wait(bar(BVF + b), parity, abort_flag, p.wait_cycles))) { ok = false; break; }

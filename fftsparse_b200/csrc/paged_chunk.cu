@@ -156,7 +156,7 @@ __global__ void __launch_bounds__(cThreads, 1)
           j = w.j0;
           j1 = w.j1;
         }
-        const int c = key_tile(w.g, j) * cBN + my_box * box;  // first key of the box
+        const int c = w.key(j) * cBN + my_box * box;  // first key of the box
         ++j;
         l.page = -1;
         l.row = c & (ps - 1);
@@ -331,7 +331,7 @@ __global__ void __launch_bounds__(cThreads, 1)
       for (int j = w.j0; mine && j < w.j1; ++j, ++n, ++kvn) {
         if (!__all_sync(0xffffffffu, mbar_wait(bar(CSF + x), n & 1, abort_flag, p.wait_cycles))) { ok = false; break; }
         fence_after();
-        const int c0 = key_tile(g, j) * cBN;
+        const int c0 = w.key(j) * cBN;
         if (x == 0 && (c0 + cBN > g.hi || (c0 < g.lo && c0 + cBN > p.sinks))) {
           // V rows that no row sees, for both halves (A's product is issued before B's)
           const int v = 2 * kvn + 1, stage = v % cStages;

@@ -196,13 +196,15 @@ struct Walk {
   // beginnings and at their ends, and find each other's tiles in L2.
   int h, j0, j1;
   bool opens;            // the (q tile, head) begins in this share
+  // A whole one begins where the share would be after so many key tiles, for the same reason, and goes round.
+  int turn, seen;
   int begin;             // where its (q tile, head) begins, relative to the share (may be negative)
   __device__ __forceinline__ Walk(const Params &prm, const Tile *t_, const long long *c_) : p(prm), tiles(t_), cum(c_) {}
 
   // Finds the q tile at u0 (whole warp; u0 < length).
   __device__ __forceinline__ void seek(long long u0, long long u1, int ntiles) {
     left = int(u1 - u0);
-    done = 0;
+    done = seen = 0;
     int lo = 0, n = ntiles;  // x is in [lo, lo + n): cum[lo] * Hkv <= u0
     const int lane = threadIdx.x & 31;
     while (n > 1) {
@@ -223,6 +225,8 @@ struct Walk {
     g = keys_of<BN>(t.pos0, t.ntok, p.window, p.sinks);
     all = (g.n + p.overhead) * p.Hkv;
   }
+  // The key tile at step j of [j0, j1).
+  __device__ __forceinline__ int key(int j) const { return key_tile(g, j + turn < j1 ? j + turn : j + turn - g.n); }
   // The next segment with key tiles; false behind the share's end.
   __device__ __forceinline__ bool segment() {
     while (left > 0) {
@@ -244,6 +248,8 @@ struct Walk {
       opens = o0 == 0;
       j0 = g.n - o1;
       j1 = g.n - o0;
+      turn = j1 - j0 == g.n ? seen % g.n : 0;
+      seen += j1 - j0;
       return true;
     }
     return false;

@@ -60,7 +60,7 @@ constexpr int kFewRows = 32;    // of a q tile: loaded one by one
 // rows: half the power of products that are mostly of zeros (64 requests' step 169 -> 164 us under the power cap,
 // 2 x 131072 keys 180 -> 172).
 constexpr int kSmallRows = 16;
-constexpr int64_t kLongKeys = 16384;
+constexpr int64_t kLongRows = 1024, kLongKeys = 4096;  // of a request on average, of a tile
 constexpr double kWaitSeconds = 2.0, kDrainSeconds = 4.0;
 
 template <int D>
@@ -822,13 +822,14 @@ int paged_attn(const ffts_paged_attn_args &a, cudaStream_t stream) {
   if (!rc) rc = device_wait_cycles(kWaitSeconds, &p.wait_cycles);
   if (!rc) rc = device_wait_cycles(kDrainSeconds, &p.drain_cycles);
   if (rc) return rc;
-  // The larger tiles of paged_chunk.cu: where requests fill them on average and their key lists, as far as the
-  // table and the window bound them, are long enough to pay for filling and draining one pipeline per SM instead
-  // of two. 2048 tokens of 32 / 8 heads over 32768 cached: 1.09 ms against 1.37 (0.98 and 1.11 before the power
-  // cap sets in); 512 over 16384: 129 us both; 16 ragged chunks over up to 16384: 72 against 59.
+  // The larger tiles of paged_chunk.cu: where requests fill several of them on average and the keys that a tile sees,
+  // as far as the table and the window bound them, are enough to pay for filling and draining one pipeline per SM
+  // instead of two. In long loops under the power cap, against the tiles of paged_attn.cu (32 / 8 heads): 2048
+  // tokens over nothing 61 us both, over 4096 190 and 207, over 32768 1.09 and 1.37 ms; 512 over 8192 91 and 94; 16
+  // ragged chunks of 650 rows on average 85 and 75; window 1024 61 and 54.
   int64_t span = width * page_size;
-  if (p.window > 0) span = std::min(span, int64_t(p.window) + p.sinks + T / R);
-  const bool chunks = T * G >= 2 * kBM * R && span > kLongKeys;
+  if (p.window > 0) span = std::min(span, int64_t(p.window) + p.sinks);
+  const bool chunks = T * G >= kLongRows * R && span >= kLongKeys;
   p.ctas = std::min(chunks ? sms : 2 * sms, kMaxCtas / (chunks ? 2 : 1));
   p.rows = chunks ? 2 * kBM : kBM;
   if (chunks) p.tpt *= 2;

@@ -302,22 +302,30 @@ def test_paged_attention_window(lens, window, sinks, H, Hkv, D, dt, page):
     b.check(b.run())
 
 
-# Long table rows and requests of 256 rows on average: the kernel with the larger tiles.
-@pytest.mark.parametrize("lens", [[(1000, 37), (0, 200), (129, 1), (0, 129), (3333, 300), (64, 64)], [(9001, 150)], [(0, 256)],
-                                  [(17, 1), (40, 64), (0, 0), (0, 1000), (127, 129), (255, 600)], [(20000, 65)]])
+# Long table rows and requests of 1024 rows on average: the kernel with the larger tiles.
+@pytest.mark.parametrize("lens", [
+    [(1000, 37), (0, 200), (129, 1), (0, 129), (3333, 300), (64, 64), (10, 1400)], [(9001, 300)], [(0, 1024)],
+    [(17, 1), (40, 64), (0, 0), (0, 1000), (127, 129), (255, 600)], [(20000, 260)]])
 @pytest.mark.parametrize("H,Hkv,D,dt,page,layout", [
     (32, 8, 128, BF, 16, "heads"), (28, 4, 128, FP, 32, "heads"), (16, 4, 64, BF, 64, "tokens"), (16, 1, 128, BF, 128, "heads"),
-    (9, 3, 64, FP, 256, "heads"), (5, 1, 128, FP, 16, "tokens"), (4, 4, 128, BF, 128, "heads"), (100, 1, 64, BF, 16, "heads")])
+    (15, 3, 64, FP, 256, "heads"), (5, 1, 128, FP, 16, "tokens"), (100, 1, 64, BF, 16, "heads")])
 def test_paged_attention_long_rows(lens, H, Hkv, D, dt, page, layout):
+    assert sum(n for _, n in lens) * (H // Hkv) >= 1024 * len(lens)
     b = Batch(lens, H, Hkv, D, dt, page, layout, width=20000)
     b.check(b.run())
     F.check_status()
 
 
-@pytest.mark.parametrize("window,sinks", [(16400, 0), (17000, 4), (20000, 130), (10 ** 9, 3)])
+@pytest.mark.parametrize("D,dt,page", [(64, BF, 16), (128, FP, 128)])
+def test_paged_attention_long_rows_without_sharing(D, dt, page):
+    b = Batch([(50, 1100)], 3, 3, D, dt, page, width=20000)
+    b.check(b.run())
+
+
+@pytest.mark.parametrize("window,sinks", [(4100, 0), (5000, 4), (20000, 130), (10 ** 9, 3)])
 @pytest.mark.parametrize("H,Hkv,D,dt,page", [(8, 2, 128, BF, 16), (14, 2, 64, FP, 128)])
 def test_paged_attention_long_window(window, sinks, H, Hkv, D, dt, page):
-    b = Batch([(20100, 300), (0, 70), (16390, 90)], H, Hkv, D, dt, page, window=window, sinks=sinks, drop=True)
+    b = Batch([(20100, 600), (0, 70), (16390, 290)], H, Hkv, D, dt, page, window=window, sinks=sinks, drop=True)
     b.check(b.run())
 
 
@@ -339,7 +347,7 @@ def test_paged_attention_many_q_tiles(lens, window, sinks, width):
 @pytest.mark.parametrize("dt", [BF, FP])
 def test_paged_attention_scores_that_grow_and_peak(dt, width):
     """Scores far apart (the running maximum moves by more than its slack) and a scale of its own."""
-    b = Batch([(700, 140), (1500, 1)], 8, 2, 64, dt, 16, spread=1.0, width=width)
+    b = Batch([(700, 640), (1500, 1)], 8, 2, 64, dt, 16, spread=1.0, width=width)
     ramp = torch.linspace(0.0, 1.0, 1600, device="cuda")
     for r, (c, n) in enumerate(b.lens):
         k = b.k[r].float()
@@ -352,9 +360,9 @@ def test_paged_attention_scores_that_grow_and_peak(dt, width):
     b.check(b.run(scale=0.5), scale=0.5)
 
 
-@pytest.mark.parametrize("G,width", [(2, 0), (128, 20000)])
-def test_rows_of_no_request_stay_and_empty_requests_give_zeros(G, width):
-    b = Batch([(30, 3), (0, 5), (100, 2), (40, 0)], 2 * G, 2, 64, BF, 16, extra=4, width=width)
+@pytest.mark.parametrize("G,width,extra", [(2, 0, 4), (128, 20000, 40)])
+def test_rows_of_no_request_stay_and_empty_requests_give_zeros(G, width, extra):
+    b = Batch([(30, 3), (0, 5), (100, 2), (40, 0)], 2 * G, 2, 64, BF, 16, extra=extra, width=width)
     out = torch.full_like(b.q, 7.0)
     b.kv[1] = 0  # not served: its five tokens see nothing
     got = F.paged_attention(b.q, b.kp, b.vp, b.table, b.cu, b.kv, out=out)
@@ -368,26 +376,26 @@ def test_rows_of_no_request_stay_and_empty_requests_give_zeros(G, width):
     b.check(out[8:])
 
 
-@pytest.mark.parametrize("G,width", [(2, 0), (100, 20000)])
-def test_more_new_tokens_than_keys(G, width):
-    """kv_len 3 with 5 new tokens: the first two come before the first key and see nothing."""
-    b = Batch([(0, 5)], G, 1, 64, BF, 16, width=width)
-    b.kv[0] = 3
+@pytest.mark.parametrize("n,G,width", [(5, 2, 0), (15, 100, 20000)])
+def test_more_new_tokens_than_keys(n, G, width):
+    """Two keys fewer than new tokens: the first two come before the first key and see nothing."""
+    b = Batch([(0, n)], G, 1, 64, BF, 16, width=width)
+    b.kv[0] = n - 2
     got = b.run()
     assert bool((got[:2] == 0.0).all())
-    b.lens, b.q, b.k, b.v = [(0, 3)], b.q[2:], [b.k[0][:, :3]], [b.v[0][:, :3]]
+    b.lens, b.q, b.k, b.v = [(0, n - 2)], b.q[2:], [b.k[0][:, :n - 2]], [b.v[0][:, :n - 2]]
     b.check(got[2:])
 
 
 @pytest.mark.parametrize("G,width", [(2, 0), (128, 20000)])
 def test_lengths_outside_their_tensors_are_kept_inside(G, width):
     """cu_q and kv_lens are device data: whatever they hold, no row outside q and no page outside the table is used."""
-    b = Batch([(30, 3), (50, 4)], 2 * G, 2, 64, BF, 16, width=width)
+    b = Batch([(30, 13), (50, 14)], 2 * G, 2, 64, BF, 16, width=width)
     b.kp.nan_to_num_(0.0)
     b.vp.nan_to_num_(0.0)
     out = torch.zeros_like(b.q)
-    for cu, kv in (([0, 3, 10 ** 6], [33, 54]), ([-5, 3, 7], [2 ** 31 - 1, 54]), ([7, 3, 0], [-1, 54]),
-                   ([0, 7, 7], [10 ** 6, 0]), ([2 ** 31 - 1, -2 ** 31, 5], [33, 54])):
+    for cu, kv in (([0, 13, 10 ** 6], [43, 64]), ([-5, 13, 27], [2 ** 31 - 1, 64]), ([27, 13, 0], [-1, 64]),
+                   ([0, 27, 27], [10 ** 6, 0]), ([2 ** 31 - 1, -2 ** 31, 5], [43, 64])):
         F.paged_attention(b.q, b.kp, b.vp, b.table, ints(cu), ints(kv), out=out)
     torch.cuda.synchronize()
     F.check_status()
@@ -422,7 +430,7 @@ def test_requests_that_share_pages():
 @pytest.mark.parametrize("width", [0, 20000])
 def test_infinities_and_nan_stay_in_their_rows(width):
     """A request whose values are broken, and a broken row of q, leave every other row as it was."""
-    lens = [(300, 40), (90, 200), (700, 100)]
+    lens = [(300, 40), (90, 200), (700, 600)]
     b = Batch(lens, 8, 2, 128, BF, 16, width=width)
     want = b.run().clone()
     b.vp[b.table[1, :19].long()] = math.inf
@@ -430,7 +438,7 @@ def test_infinities_and_nan_stay_in_their_rows(width):
     b.q[5, 3] = NAN
     b.q[250] = math.inf
     got = b.run()
-    same = torch.ones(340, 8, dtype=torch.bool, device="cuda")
+    same = torch.ones(840, 8, dtype=torch.bool, device="cuda")
     same[40:240] = False
     same[5, 3] = False
     same[250] = False
@@ -483,7 +491,7 @@ def test_paged_attention_refusals():
 
 @pytest.mark.parametrize("width", [0, 20000])
 def test_two_streams_at_once(width):
-    one = Batch(LENS["chunks"], 8, 2, 128, BF, 16, seed=1, width=width)
+    one = Batch(LENS["chunks"] + [(10, 1400)], 8, 2, 128, BF, 16, seed=1, width=width)
     two = Batch(LENS["decode"], 8, 2, 128, BF, 16, seed=2)
     want = one.run().clone(), two.run().clone()
     streams = torch.cuda.Stream(), torch.cuda.Stream()

@@ -40,71 +40,81 @@ _ATTN = struct.Struct("=32qif")
 _raw_stream = torch._C._cuda_getCurrentRawStream  # current_stream(device).cuda_stream without the Stream object
 
 
-def _call(device: torch.device, fn, block: bytes) -> None:
-    """One C call with ``device`` current, on its current stream."""
-    index = device.index
-    if index == torch.cuda.current_device():
+_I32 = torch.int32
+_get_device = torch._C._cuda_getDevice
+
+# The checks below run in every call of a decoding step: a device is compared by its index (-1 on the CPU).
+
+
+def _call(index: int, fn, block: bytes) -> None:
+    """One C call with device ``index`` current, on its current stream."""
+    if index == _get_device():
         rc = fn(block, _raw_stream(index))
     else:
-        with torch.cuda.device(device):
+        with torch.cuda.device(index):
             rc = fn(block, _raw_stream(index))
     if rc:
         _lib.check(rc)
 
 
-def _check_ints(name: str, t: torch.Tensor, n: int, device) -> None:
-    if t.dtype is not torch.int32:
+def _check_ints(name: str, t: torch.Tensor, n: int, index: int) -> None:
+    if t.dtype is not _I32:
         raise TypeError(f"{name} must be int32, got {t.dtype}")
-    if t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+    if t.shape != (n,) or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous tensor of shape [{n}], got {tuple(t.shape)}")
-    if t.device != device:
-        raise ValueError(f"{name} must be on {device}, got {t.device}")
+    if t.get_device() != index:
+        raise ValueError(f"{name} must be on the other tensors' device, got {t.device}")
 
 
-def _check_table(t: torch.Tensor, rows: int, device) -> int:
-    """The table's row stride (any, of a single row)."""
-    if t.dtype is not torch.int32:
+def _check_table(t: torch.Tensor, rows: int, index: int):
+    """The table's row stride (its width for a single row) and width."""
+    if t.dtype is not _I32:
         raise TypeError(f"block_table must be int32, got {t.dtype}")
-    if t.dim() != 2 or t.shape[0] != rows or (t.shape[1] > 1 and t.stride(1) != 1):
-        raise ValueError(f"block_table must be [{rows}, pages] with unit stride along a row, got {tuple(t.shape)}")
-    if t.device != device:
-        raise ValueError(f"block_table must be on {device}, got {t.device}")
-    return t.stride(0) if rows > 1 else t.shape[1]
+    if t.dim() == 2:
+        n, width = t.shape
+        ld, unit = t.stride()
+        if n == rows and (unit == 1 or width <= 1):
+            if t.get_device() != index:
+                raise ValueError(f"block_table must be on the other tensors' device, got {t.device}")
+            return (ld if rows > 1 else width), width
+    raise ValueError(f"block_table must be [{rows}, pages] with unit stride along a row, got {tuple(t.shape)}")
 
 
-def _check_heads(name: str, t: torch.Tensor, dtype, device):
-    """The token and head strides of a [tokens, heads, head_dim] tensor."""
-    if t.dim() != 3:
-        raise ValueError(f"{name} must be [tokens, heads, head_dim], got shape {tuple(t.shape)}")
+def _check_heads(name: str, t: torch.Tensor, dtype, index: int):
+    """The token and head strides and the shape of a [tokens, heads, head_dim] tensor."""
+    shape = t.shape
+    if len(shape) != 3:
+        raise ValueError(f"{name} must be [tokens, heads, head_dim], got shape {tuple(shape)}")
     if t.dtype is not dtype:
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
-    if t.device != device:
-        raise ValueError(f"{name} must be on {device}, got {t.device}")
+    if t.get_device() != index:
+        raise ValueError(f"{name} must be on the other tensors' device, got {t.device}")
     st, sh, sd = t.stride()
     if sd != 1:
         raise ValueError(f"{name} must be contiguous in the head dimension")
-    n, h, d = t.shape
-    return (st if n > 1 else h * d), (sh if h > 1 else d)  # a single row's stride says nothing
+    n, h, d = shape
+    return ((st if n > 1 else h * d), (sh if h > 1 else d)), shape  # a single row's stride says nothing
 
 
-def _check_pool(k_pages: torch.Tensor, v_pages: torch.Tensor, dtype, device):
-    """The page, head and row strides of both pool tensors."""
-    if k_pages.dim() != 4 or v_pages.shape != k_pages.shape:
+def _check_pool(k_pages: torch.Tensor, v_pages: torch.Tensor, dtype, index: int):
+    """The page, head and row strides of both pool tensors, and their shape."""
+    shape = k_pages.shape
+    if len(shape) != 4 or v_pages.shape != shape:
         raise ValueError(f"k_pages and v_pages must both be [pages, Hkv, page_size, D], got "
-                         f"{tuple(k_pages.shape)} / {tuple(v_pages.shape)}")
+                         f"{tuple(shape)} / {tuple(v_pages.shape)}")
     if k_pages.dtype is not dtype or v_pages.dtype is not dtype:
         raise TypeError(f"k_pages and v_pages must be {dtype}, got {k_pages.dtype} / {v_pages.dtype}")
-    if k_pages.device != device or v_pages.device != device:
-        raise ValueError(f"k_pages and v_pages must be on {device}")
+    if k_pages.get_device() != index or v_pages.get_device() != index:
+        raise ValueError("k_pages and v_pages must be on the other tensors' device")
     *ks, kd = k_pages.stride()
     *vs, vd = v_pages.stride()
     if kd != 1 or vd != 1:
         raise ValueError("k_pages and v_pages must be contiguous in the head dimension")
-    if 1 in k_pages.shape:  # the stride of a single page, head or row says nothing
-        P, h, n, d = k_pages.shape
+    P, h, n, d = shape
+    if P == 1 or h == 1 or n == 1:  # the stride of a single page, head or row says nothing
         packed = (h * n * d, n * d, d)
-        ks, vs = ([s if m > 1 else c for s, m, c in zip(st, (P, h, n), packed)] for st in (ks, vs))
-    return ks, vs
+        ks, vs = ([s if m > 1 else c for s, m, c in zip(st, shape, packed)] for st in (ks, vs))
+    return ks, vs, shape
 
 
 def _check_cuda(name: str, t: torch.Tensor) -> None:
@@ -138,27 +148,26 @@ def plan_pages(cached_lens: torch.Tensor, new_lens: torch.Tensor, block_table: t
     its tokens are not appended and attend to nothing.  ``info`` holds the pages taken and the requests
     not served; the caller drops that many entries from the front of its list.  Nothing is read back.
     """
-    dev = cached_lens.device
+    index = cached_lens.get_device()
     if cached_lens.dim() != 1 or free_pages.dim() != 1:
         raise ValueError("cached_lens and free_pages must be 1-D")
     R, n_free = cached_lens.shape[0], free_pages.shape[0]
-    _check_ints("cached_lens", cached_lens, R, dev)
-    _check_ints("new_lens", new_lens, R, dev)
-    _check_ints("free_pages", free_pages, n_free, dev)
-    table_ld = _check_table(block_table, R, dev)
+    _check_ints("cached_lens", cached_lens, R, index)
+    _check_ints("new_lens", new_lens, R, index)
+    _check_ints("free_pages", free_pages, n_free, index)
+    table_ld, width = _check_table(block_table, R, index)
     if num_tokens < 0:
         raise ValueError(f"num_tokens must not be negative, got {num_tokens}")
     _check_cuda("cached_lens", cached_lens)
-    sizes = [R + 1, R, num_tokens, num_tokens, 2]
-    buf = torch.empty(2 * R + 2 * num_tokens + 3, dtype=torch.int32, device=dev)
-    plan = PagePlan(*buf.split_with_sizes(sizes))
+    buf = cached_lens.new_empty(2 * R + 2 * num_tokens + 3)
+    plan = PagePlan(*buf.split_with_sizes([R + 1, R, num_tokens, num_tokens, 2]))
     cu = buf.data_ptr()
     kv = cu + 4 * (R + 1)
     pos = kv + 4 * R
     slot = pos + 4 * num_tokens
-    _call(dev, _lib.load().ffts_page_plan, _PLAN.pack(
+    _call(index, _lib.load().ffts_page_plan, _PLAN.pack(
         _PLAN.size, cached_lens.data_ptr(), new_lens.data_ptr(), block_table.data_ptr(), free_pages.data_ptr(), cu, kv,
-        pos, slot, slot + 4 * num_tokens, R, table_ld, block_table.shape[1], n_free, page_size, num_tokens))
+        pos, slot, slot + 4 * num_tokens, R, table_ld, width, n_free, page_size, num_tokens))
     return plan
 
 
@@ -244,49 +253,47 @@ def rope_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, pos
     written in place.  Returns the rotated q [T, H, D] (``out``, which may be q itself, or a new tensor), None
     without q.  The angles are exact for far positions (64 bits), the rotation is fp32, rounded once.
     """
-    dev, dt = k.device, k.dtype
+    index, dt = k.get_device(), k.dtype
     if dt not in _DTYPES:
         raise TypeError(f"rope_append supports bfloat16 and float16, got {dt}")
-    ks = _check_heads("k", k, dt, dev)
-    vs = _check_heads("v", v, dt, dev)
-    T, Hkv, D = k.shape
-    if v.shape != k.shape:
-        raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} differ in shape")
-    kps, vps = _check_pool(k_pages, v_pages, dt, dev)
-    P, kv_heads, page_size, dim = k_pages.shape
+    ks, shape = _check_heads("k", k, dt, index)
+    vs, v_shape = _check_heads("v", v, dt, index)
+    T, Hkv, D = shape
+    if v_shape != shape:
+        raise ValueError(f"k {tuple(shape)} and v {tuple(v_shape)} differ in shape")
+    kps, vps, (P, kv_heads, page_size, dim) = _check_pool(k_pages, v_pages, dt, index)
     if kv_heads != Hkv or dim != D:
-        raise ValueError(f"pages {tuple(k_pages.shape)} do not match k {tuple(k.shape)}")
-    _check_ints("positions", positions, T, dev)
-    _check_ints("slot_map", slot_map, T, dev)
+        raise ValueError(f"pages {tuple(k_pages.shape)} do not match k {tuple(shape)}")
+    _check_ints("positions", positions, T, index)
+    _check_ints("slot_map", slot_map, T, index)
     rd = freq = 0
     if inv_freq is not None:
         if inv_freq.dim() != 1 or inv_freq.dtype is not torch.float32 or not inv_freq.is_contiguous():
             raise ValueError("inv_freq must be a contiguous 1-D fp32 tensor")
-        if inv_freq.device != dev:
-            raise ValueError(f"inv_freq must be on {dev}, got {inv_freq.device}")
+        if inv_freq.get_device() != index:
+            raise ValueError(f"inv_freq must be on the other tensors' device, got {inv_freq.device}")
         rd, freq = 2 * inv_freq.shape[0], inv_freq.data_ptr()
     H = q_ptr = o_ptr = 0
     qs = os_ = (0, 0)
     if q is not None:
-        qs = _check_heads("q", q, dt, dev)
-        H = q.shape[1]
-        if q.shape[0] != T or q.shape[2] != D:
-            raise ValueError(f"q {tuple(q.shape)} does not match k {tuple(k.shape)}")
+        qs, (n, H, dim) = _check_heads("q", q, dt, index)
+        if n != T or dim != D:
+            raise ValueError(f"q {tuple(q.shape)} does not match k {tuple(shape)}")
     if out is not None:
         if q is None:
             raise ValueError("out without q")
-        os_ = _check_heads("out", out, dt, dev)
-        if out.shape != q.shape:
-            raise ValueError(f"out must have q's shape {tuple(q.shape)}, got {tuple(out.shape)}")
+        os_, o_shape = _check_heads("out", out, dt, index)
+        if o_shape != q.shape:
+            raise ValueError(f"out must have q's shape {tuple(q.shape)}, got {tuple(o_shape)}")
     _check_cuda("k", k)
     if q is not None:
         if out is None:
-            out = torch.empty(T, H, D, dtype=dt, device=dev)
+            out = q.new_empty((T, H, D))
             os_ = (H * D, D)
         q_ptr, o_ptr = q.data_ptr(), out.data_ptr()
     if T == 0:
         return out
-    _call(dev, _lib.load().ffts_rope_append, _ROPE.pack(
+    _call(index, _lib.load().ffts_rope_append, _ROPE.pack(
         _ROPE.size, q_ptr, k.data_ptr(), v.data_ptr(), positions.data_ptr(), slot_map.data_ptr(), freq, o_ptr,
         k_pages.data_ptr(), v_pages.data_ptr(), *qs, *ks, *vs, *os_, *kps, *vps, T, H, Hkv, D, rd, P, page_size,
         _DTYPES[dt], interleaved, attn_factor, 0))
@@ -311,21 +318,19 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     A bounded wait that runs out in the kernel raises WaitTimeout at a later call or at ``check_status()``.  Before a
     capture into a CUDA graph make one call outside of it (it sets up the device's status word).
     """
-    dev, dt = q.device, q.dtype
+    index, dt = q.get_device(), q.dtype
     if dt not in _DTYPES:
         raise TypeError(f"paged attention supports bfloat16 and float16, got {dt}")
-    qs = _check_heads("q", q, dt, dev)
-    kps, vps = _check_pool(k_pages, v_pages, dt, dev)
-    T, H, D = q.shape
-    P, Hkv, page_size, dim = k_pages.shape
+    qs, (T, H, D) = _check_heads("q", q, dt, index)
+    kps, vps, (P, Hkv, page_size, dim) = _check_pool(k_pages, v_pages, dt, index)
     if dim != D or Hkv == 0 or H % Hkv:
         raise ValueError(f"pages {tuple(k_pages.shape)} do not match q {tuple(q.shape)}")
     if kv_lens.dim() != 1:
         raise ValueError("kv_lens must be 1-D")
     R = kv_lens.shape[0]
-    _check_ints("kv_lens", kv_lens, R, dev)
-    _check_ints("cu_q", cu_q, R + 1, dev)
-    table_ld = _check_table(block_table, R, dev)
+    _check_ints("kv_lens", kv_lens, R, index)
+    _check_ints("cu_q", cu_q, R + 1, index)
+    table_ld, width = _check_table(block_table, R, index)
     if window is None:
         if sinks:
             raise ValueError("sinks need a window")
@@ -335,25 +340,24 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     if sinks < 0:
         raise ValueError(f"sinks must not be negative, got {sinks}")
     if out is not None:
-        os_ = _check_heads("out", out, dt, dev)
-        if out.shape != q.shape:
-            raise ValueError(f"out must have q's shape {tuple(q.shape)}, got {tuple(out.shape)}")
+        os_, o_shape = _check_heads("out", out, dt, index)
+        if o_shape != q.shape:
+            raise ValueError(f"out must have q's shape {tuple(q.shape)}, got {tuple(o_shape)}")
     if P == 0:
         raise ValueError("the pool has no pages")
     _check_cuda("q", q)
     if out is None:
-        out = torch.empty(T, H, D, dtype=dt, device=dev)
+        out = q.new_empty((T, H, D))
         os_ = (H * D, D)
     if T == 0 or R == 0:
         return out
     lib = _lib.load()
-    status = device_status(dev)
+    status = device_status(q.device)
     status.poll_direct()
     nbytes = lib.ffts_paged_workspace_bytes(T, R, H, Hkv, D)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    _call(dev, lib.ffts_paged_attn, _ATTN.pack(
+    ws = q.new_empty(nbytes, dtype=torch.uint8)
+    _call(index, lib.ffts_paged_attn, _ATTN.pack(
         _ATTN.size, q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(), cu_q.data_ptr(),
         kv_lens.data_ptr(), out.data_ptr(), ws.data_ptr(), status.direct_ptr, *qs, *kps, *vps, *os_, T, R, H, Hkv, D, P,
-        page_size, table_ld, block_table.shape[1], window, sinks, nbytes, _DTYPES[dt],
-        D ** -0.5 if scale is None else scale))
+        page_size, table_ld, width, window, sinks, nbytes, _DTYPES[dt], D ** -0.5 if scale is None else scale))
     return out

@@ -14,9 +14,8 @@
 // workspace, no order between CTAs.  The tokens of a CTA find their request by a binary search in
 // the chunk's prefix in shared memory.  Nothing a CTA reads is written by another one: tokens read
 // table entries below have_r, the new entries lie at or above it, and a token in a new page takes its
-// page from the free list.  Latency bound: 4.2 us for
-// 64 requests of one token, 7.4 us for 1024 of 1 to 256 (256 threads 3.5 and 9.6, 1024 6.6 and 7.5; 1024 tokens
-// per CTA 8.0).
+// page from the free list.  Latency bound: 4.2 us for 64 requests of one token, 7.4 us for 1024 of 1 to
+// 256 (256 threads 3.5 and 9.6, 1024 threads 6.6 and 7.5; 1024 tokens per CTA 4.3 and 8.0).
 
 #include "ffts_common.cuh"
 

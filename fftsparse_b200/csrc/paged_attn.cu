@@ -483,7 +483,9 @@ __global__ void __launch_bounds__(kThreads, 2)
       if (active) {
         const bool whole = w.j0 == 0 && w.j1 == g.n;
         const int slot = 2 * int(blockIdx.x) + (first_seg ? 0 : 1);
-        const float inv_l = l_run > 0.0f ? 1.0f / l_run : 0.0f;
+        // a row without a key (pos < 0) is zeros; NaN in l, or no key above -inf (l == 0), is NaN as in the formula
+        const bool sees = pos >= 0;
+        const float inv_l = 1.0f / l_run;
         uint16_t *dst = p.out + int64_t(w.t.tok0 + tl) * p.os_t + int64_t(w.h * p.G + hg) * p.os_h;
         float4 *pd = reinterpret_cast<float4 *>(p.part) + int64_t(slot) * (kBM * D / 4) + r;
 #pragma unroll 1
@@ -498,8 +500,7 @@ __global__ void __launch_bounds__(kThreads, 2)
               uint32_t v[4];
 #pragma unroll
               for (int e = 0; e < 4; ++e)
-                v[e] = Num<E>::pack(l_run > 0.0f ? o[q * 8 + 2 * e] * inv_l : 0.0f,
-                                    l_run > 0.0f ? o[q * 8 + 2 * e + 1] * inv_l : 0.0f);
+                v[e] = Num<E>::pack(sees ? o[q * 8 + 2 * e] * inv_l : 0.0f, sees ? o[q * 8 + 2 * e + 1] * inv_l : 0.0f);
               *reinterpret_cast<uint4 *>(dst + c * 32 + q * 8) = make_uint4(v[0], v[1], v[2], v[3]);
             }
           }
@@ -516,6 +517,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       if (w.opens && w.j1 - w.j0 < g.n && r == 0 && FFTS_IN_RANGE(blockIdx.x, p.ctas)) {
         Cut cut;
         cut.tok0 = w.t.tok0;
+        cut.pos0 = w.t.pos0;
         cut.nrows = nrows;
         cut.head0 = w.h * p.G;
         cut.s1 = int((u0 + w.begin + p.overhead + g.n - 1) / per);
@@ -549,7 +551,7 @@ constexpr int kJoinThreads = 512;
 // 1, 2 and 4 blocks: 16.5, 11.5, 11.2 us after ragged chunks, 4.5, 4.4, 5.7 us after 64 decoding requests
 constexpr int kJoinBlocks = 2;
 
-// (m, l, o) of some shares, o a piece of a row; m = -inf: none of them sees a key.
+// (m, l, o) of some shares, o a piece of a row; m = -inf: no score above -inf among them (l is 0, or NaN if one was).
 struct Part {
   float m, l;
   float4 o;
@@ -585,9 +587,9 @@ __global__ void __launch_bounds__(kJoinThreads, 2) join_kernel(const __grid_cons
   auto store = [&](int r, int piece, const Part &t) {
     const int tl = r / p.G, hg = r - tl * p.G;
     if (!FFTS_IN_RANGE(cut.tok0 + tl, p.T)) return;
-    const float inv_l = t.l > 0.0f ? 1.0f / t.l : 0.0f;
+    const float inv_l = 1.0f / t.l;
     uint2 o = make_uint2(0u, 0u);
-    if (t.l > 0.0f)
+    if (cut.pos0 + tl >= 0)  // the row sees a key
       o = make_uint2(Num<E>::pack(t.o.x * inv_l, t.o.y * inv_l), Num<E>::pack(t.o.z * inv_l, t.o.w * inv_l));
     *reinterpret_cast<uint2 *>(p.out + int64_t(cut.tok0 + tl) * p.os_t + int64_t(cut.head0 + hg) * p.os_h + piece * 4) = o;
   };
@@ -620,7 +622,7 @@ __global__ void __launch_bounds__(kJoinThreads, 2) join_kernel(const __grid_cons
       }
 #pragma unroll
       for (int k = 0; k < JS; ++k) {
-        if (ml[k].x == -INFINITY) continue;  // no share, or one whose keys the row does not see
+        if (ml[k].x == -INFINITY && ml[k].y == 0.0f) continue;  // no share, or none of its keys counts (NaN does)
         const float f = exp2f(ml[k].x - top);
 #pragma unroll
         for (int i = 0; i < JP; ++i)

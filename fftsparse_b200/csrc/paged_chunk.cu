@@ -432,7 +432,8 @@ __global__ void __launch_bounds__(cThreads, 1)
       if (active) {
         const bool whole = w.j0 == 0 && w.j1 == g.n;
         const bool live = r < qrows && row < nrows;
-        const float inv_l = l_run > 0.0f ? 1.0f / l_run : 0.0f;
+        const bool sees = pos >= 0;  // a row without a key is zeros; NaN in l, or l == 0, is NaN as in the formula
+        const float inv_l = 1.0f / l_run;
         uint16_t *dst = p.out + int64_t(w.t.tok0 + tl) * p.os_t + int64_t(w.h * p.G + hg) * p.os_h;
         float4 *pd = reinterpret_cast<float4 *>(p.part) + int64_t(slot) * (2 * cBM * D / 4) + row;
 #pragma unroll 1
@@ -447,8 +448,7 @@ __global__ void __launch_bounds__(cThreads, 1)
               uint32_t v[4];
 #pragma unroll
               for (int e = 0; e < 4; ++e)
-                v[e] = Num<E>::pack(l_run > 0.0f ? o[q * 8 + 2 * e] * inv_l : 0.0f,
-                                    l_run > 0.0f ? o[q * 8 + 2 * e + 1] * inv_l : 0.0f);
+                v[e] = Num<E>::pack(sees ? o[q * 8 + 2 * e] * inv_l : 0.0f, sees ? o[q * 8 + 2 * e + 1] * inv_l : 0.0f);
               *reinterpret_cast<uint4 *>(dst + c * 32 + q * 8) = make_uint4(v[0], v[1], v[2], v[3]);
             }
           }
@@ -465,6 +465,7 @@ __global__ void __launch_bounds__(cThreads, 1)
       if (w.opens && w.j1 - w.j0 < g.n && threadIdx.x == 0 && FFTS_IN_RANGE(blockIdx.x, p.ctas)) {
         Cut cut;
         cut.tok0 = w.t.tok0;
+        cut.pos0 = w.t.pos0;
         cut.nrows = nrows;
         cut.head0 = w.h * p.G;
         cut.s1 = int((u0 + w.begin + p.overhead + g.n - 1) / per);

@@ -26,10 +26,10 @@ struct __align__(16) Tile {
   int tok0, pos0, ntok, r;
 };
 
-// A (q tile, head) that several shares cut: rows nrows from token tok0 and head head0 on; its partials lie in
-// first_slot and in the first slots of the shares behind it up to s1.  nrows 0: none.
+// A (q tile, head) that several shares cut: rows nrows from token tok0 (at position pos0) and head head0 on; its
+// partials lie in first_slot and in the first slots of the shares behind it up to s1.  nrows 0: none.
 struct Cut {
-  int tok0, nrows, head0, s1, first_slot;
+  int tok0, pos0, nrows, head0, s1, first_slot;
 };
 
 struct Params {

@@ -96,6 +96,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                 const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ Params p) {
   using Lay = Layout<D>;
+  constexpr int kSum = Num<E>::sum_keys / kBN;  // key tiles after which O is parked
   extern __shared__ __align__(16) uint8_t smem[];
   if (smem_u32(smem) & 1023u) {  // SWIZZLE_128B tiles need 1024-byte alignment
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -276,7 +277,7 @@ __global__ void __launch_bounds__(kThreads, 2)
                      dv0 = uint32_t(dv_) + (Lay::v >> 4);
       bool ok = true;
       // S runs up to two tiles ahead of PV.  s_left: S tiles left in the walked segment; the PV side
-      // needs only to know which tiles begin a segment and which have few rows (bit n % 32 of firsts and smalls).
+      // needs only to know which tiles begin a sum and which have few rows (bit n % 32 of firsts and smalls).
       int s = 0, seg = 0, s_left = 0;
       uint32_t firsts = 0, smalls = 0;
       bool small = false;
@@ -293,6 +294,7 @@ __global__ void __launch_bounds__(kThreads, 2)
             small = w.t.ntok * p.G <= kSmallRows;
             ++seg;
           }
+          const bool fresh = (w.j1 - w.j0 - s_left) % kSum == 0;  // O starts from zero
           const int ks = s % kKStages;
           ok = mbar_wait(bar(BKF + ks), (s / kKStages) & 1, abort_flag, p.wait_cycles);
           if (!ok) break;
@@ -312,7 +314,7 @@ __global__ void __launch_bounds__(kThreads, 2)
             umma_commit(bar(BQE));
             more = w.segment();
           }
-          firsts = (firsts & ~(1u << (s & 31))) | (uint32_t(first) << (s & 31));
+          firsts = (firsts & ~(1u << (s & 31))) | (uint32_t(fresh) << (s & 31));
           ++s;
         }
         if (!ok) break;
@@ -355,123 +357,135 @@ __global__ void __launch_bounds__(kThreads, 2)
       const int pos = w.t.pos0 + min(tl, w.t.ntok - 1);
       // and their P is 0, by an offset of -inf
       float m_ref = live ? -INFINITY : 0.0f, l_run = 0.0f;
-      for (int j = w.j0; j < w.j1; ++j, ++n) {
-        const int b = n & 1;
-        const uint32_t parity = (n >> 1) & 1;
-        if (!__all_sync(0xffffffffu, mbar_wait(bar(BSF + b), parity, abort_flag, p.wait_cycles))) { ok = false; break; }
-        fence_after();
-        const int c0 = w.key(j) * kBN;
-        if (c0 + kBN > g.hi || (c0 < g.lo && c0 + kBN > p.sinks)) {
-          // V rows that no row sees
-          if (!__all_sync(0xffffffffu, mbar_wait(bar(BVF + b), parity, abort_flag, p.wait_cycles))) { ok = false; break; }
-          const int key = c0 + (r & 63);
-          if (r < 64 * Lay::halves && (key >= g.hi || (key < g.lo && key >= p.sinks))) {
-            uint8_t *vr = smem + Lay::v + b * Lay::kv_bytes + (r >> 6) * Lay::kv_half + (r & 63) * 128;
+      for (int j = w.j0, stop; ok && j < w.j1;) {
+        stop = min(w.j1, j + kSum);
+        for (; j < stop; ++j, ++n) {
+          const int b = n & 1;
+          const uint32_t parity = (n >> 1) & 1;
+          if (!__all_sync(0xffffffffu, mbar_wait(bar(BSF + b), parity, abort_flag, p.wait_cycles))) { ok = false; break; }
+          fence_after();
+          const int c0 = w.key(j) * kBN;
+          if (c0 + kBN > g.hi || (c0 < g.lo && c0 + kBN > p.sinks)) {
+            // V rows that no row sees
+            if (!__all_sync(0xffffffffu, mbar_wait(bar(BVF + b), parity, abort_flag, p.wait_cycles))) { ok = false; break; }
+            const int key = c0 + (r & 63);
+            if (r < 64 * Lay::halves && (key >= g.hi || (key < g.lo && key >= p.sinks))) {
+              uint8_t *vr = smem + Lay::v + b * Lay::kv_bytes + (r >> 6) * Lay::kv_half + (r & 63) * 128;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4 *>(vr + i * 16) = make_uint4(0, 0, 0, 0);
-          }
-          fence_proxy_async();
-        }
-        if (active) {
-          uint64_t mask = below(pos + 1 - c0);
-          if (p.window > 0) mask &= ~below(pos - p.window + 1 - c0) | below(p.sinks - c0);
-          const bool edge = __any_sync(0xffffffffu, mask != ~0ull);
-          const uint32_t s_addr = tmem + b * kBN + lane_off;
-          float x[kBN];
-          tmem_ld32(s_addr, x);
-          tmem_wait_ld();
-          tmem_ld32(s_addr + 32, x + 32);  // lands while the first half is processed
-          if (edge) {
-#pragma unroll
-            for (int c = 0; c < 32; ++c)
-              if (!((uint32_t(mask) >> c) & 1u)) x[c] = -INFINITY;
-          }
-          // P = exp2(s * scale - m_ref) as pairs over the first 32 columns of this S buffer (columns
-          // already read).  The common path takes m_ref as it stands and keeps the result when every
-          // P of the row is small enough (by the tile's row sum); a row's first tile with a key, or one
-          // that outgrows m_ref, takes the max path: new m_ref, O and l rescaled, P again.
-          float2 rs2[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
-          float alpha = 1.0f;
-          bool fast = !__any_sync(0xffffffffu, m_ref == -INFINITY);
-          auto exp_half = [&](int cc, float2 off2) {
-            uint32_t pk[16];
-#pragma unroll
-            for (int e = 0; e < 32; e += 2) {
-              const int c = cc * 32 + e;
-              const float2 a = __ffma2_rn(make_float2(x[c], x[c + 1]), sc2, off2);
-              float2 ex;
-              ex.x = fast_exp2(a.x);
-              ex.y = fast_exp2(a.y);
-              rs2[(e >> 1) & 1] = __fadd2_rn(rs2[(e >> 1) & 1], ex);
-              pk[e >> 1] = Num<E>::pack(ex.x, ex.y);
+              for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4 *>(vr + i * 16) = make_uint4(0, 0, 0, 0);
             }
-            tmem_st16u(s_addr + cc * 16, pk);
-          };
-          auto mask_high = [&]() {
+            fence_proxy_async();
+          }
+          if (active) {
+            uint64_t mask = below(pos + 1 - c0);
+            if (p.window > 0) mask &= ~below(pos - p.window + 1 - c0) | below(p.sinks - c0);
+            const bool edge = __any_sync(0xffffffffu, mask != ~0ull);
+            const uint32_t s_addr = tmem + b * kBN + lane_off;
+            float x[kBN];
+            tmem_ld32(s_addr, x);
+            tmem_wait_ld();
+            tmem_ld32(s_addr + 32, x + 32);  // lands while the first half is processed
             if (edge) {
 #pragma unroll
               for (int c = 0; c < 32; ++c)
-                if (!((uint32_t(mask >> 32) >> c) & 1u)) x[32 + c] = -INFINITY;
+                if (!((uint32_t(mask) >> c) & 1u)) x[c] = -INFINITY;
             }
-          };
-          if (fast) {
-            const float moff = live ? m_ref * p.scale_log2 : INFINITY;
-            exp_half(0, make_float2(-moff, -moff));
-            tmem_wait_ld();
-            mask_high();
-            exp_half(1, make_float2(-moff, -moff));
-            const float tsum = (rs2[0].x + rs2[0].y) + (rs2[1].x + rs2[1].y);
-            if (__any_sync(0xffffffffu, !(tsum <= Num<E>::pmax))) {
-              fast = false;
-              tmem_wait_st();  // the max path below rewrites P
-              rs2[0] = rs2[1] = make_float2(0.0f, 0.0f);
-            }
-          } else {
-            tmem_wait_ld();
-            mask_high();
-          }
-          if (!fast) {
-            float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-            for (int c = 0; c < kBN; c += 2) mx4[(c >> 1) & 3] = max3f(mx4[(c >> 1) & 3], x[c], x[c + 1]);
-            const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
-            if (mx > m_ref && (m_ref == -INFINITY || (mx - m_ref) * p.scale_log2 > Num<E>::rescale)) {
-              alpha = m_ref == -INFINITY ? 0.0f : fast_exp2((m_ref - mx) * p.scale_log2);
-              m_ref = mx;
-            }
-            const float moff = live ? (m_ref == -INFINITY ? 0.0f : m_ref) * p.scale_log2 : INFINITY;
-            exp_half(0, make_float2(-moff, -moff));
-            exp_half(1, make_float2(-moff, -moff));
-          }
-          const float2 rsum = __fadd2_rn(rs2[0], rs2[1]);
-          l_run = l_run * alpha + (rsum.x + rsum.y);
-          tmem_wait_st();
-          if (j > w.j0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
-            // O must hold PV(n-1) before it is rescaled; its barrier's next phase needs P(n+1)
-            if (!__all_sync(0xffffffffu,
-                            mbar_wait(bar(BPV + (n - 1) % 2), ((n - 1) >> 1) & 1, abort_flag, p.wait_cycles))) {
-              ok = false;
-              break;
-            }
-            fence_after();
-#pragma unroll 1
-            for (int c = 0; c < D / 32; ++c) {
-              float o[32];
-              tmem_ld32(tm_o + lane_off + c * 32, o);
-              tmem_wait_ld();
+            // P = exp2(s * scale - m_ref) as pairs over the first 32 columns of this S buffer (columns
+            // already read).  The common path takes m_ref as it stands and keeps the result when every
+            // P of the row is small enough (by the tile's row sum); a row's first tile with a key, or one
+            // that outgrows m_ref, takes the max path: new m_ref, O and l rescaled, P again.
+            float2 rs2[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+            float alpha = 1.0f;
+            bool fast = !__any_sync(0xffffffffu, m_ref == -INFINITY);
+            auto exp_half = [&](int cc, float2 off2) {
+              uint32_t pk[16];
 #pragma unroll
               for (int e = 0; e < 32; e += 2) {
-                const float2 v = __fmul2_rn(make_float2(o[e], o[e + 1]), make_float2(alpha, alpha));
-                o[e] = v.x;
-                o[e + 1] = v.y;
+                const int c = cc * 32 + e;
+                const float2 a = __ffma2_rn(make_float2(x[c], x[c + 1]), sc2, off2);
+                float2 ex;
+                ex.x = fast_exp2(a.x);
+                ex.y = fast_exp2(a.y);
+                rs2[(e >> 1) & 1] = __fadd2_rn(rs2[(e >> 1) & 1], ex);
+                pk[e >> 1] = Num<E>::pack(ex.x, ex.y);
               }
-              tmem_st32(tm_o + lane_off + c * 32, o);
+              tmem_st16u(s_addr + cc * 16, pk);
+            };
+            auto mask_high = [&]() {
+              if (edge) {
+#pragma unroll
+                for (int c = 0; c < 32; ++c)
+                  if (!((uint32_t(mask >> 32) >> c) & 1u)) x[32 + c] = -INFINITY;
+              }
+            };
+            if (fast) {
+              const float moff = live ? m_ref * p.scale_log2 - Num<E>::bias : INFINITY;
+              exp_half(0, make_float2(-moff, -moff));
+              tmem_wait_ld();
+              mask_high();
+              exp_half(1, make_float2(-moff, -moff));
+              const float tsum = (rs2[0].x + rs2[0].y) + (rs2[1].x + rs2[1].y);
+              if (__any_sync(0xffffffffu, !(tsum <= Num<E>::pmax))) {
+                fast = false;
+                tmem_wait_st();  // the max path below rewrites P
+                rs2[0] = rs2[1] = make_float2(0.0f, 0.0f);
+              }
+            } else {
+              tmem_wait_ld();
+              mask_high();
             }
+            if (!fast) {
+              float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+              for (int c = 0; c < kBN; c += 2) mx4[(c >> 1) & 3] = max3f(mx4[(c >> 1) & 3], x[c], x[c + 1]);
+              const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+              if (mx > m_ref && (m_ref == -INFINITY || (mx - m_ref) * p.scale_log2 > Num<E>::rescale)) {
+                alpha = m_ref == -INFINITY ? 0.0f : fast_exp2((m_ref - mx) * p.scale_log2);
+                m_ref = mx;
+              }
+              const float moff = live ? (m_ref == -INFINITY ? 0.0f : m_ref) * p.scale_log2 - Num<E>::bias : INFINITY;
+              exp_half(0, make_float2(-moff, -moff));
+              exp_half(1, make_float2(-moff, -moff));
+            }
+            const float2 rsum = __fadd2_rn(rs2[0], rs2[1]);
+            l_run = l_run * alpha + (rsum.x + rsum.y);
             tmem_wait_st();
+            if (j > w.j0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
+              // O must hold PV(n-1) before it is rescaled; its barrier's next phase needs P(n+1)
+              if (!__all_sync(0xffffffffu,
+                              mbar_wait(bar(BPV + (n - 1) % 2), ((n - 1) >> 1) & 1, abort_flag, p.wait_cycles))) {
+                ok = false;
+                break;
+              }
+              fence_after();
+#pragma unroll 1
+              for (int c = 0; c < D / 32; ++c) {
+                float o[32];
+                tmem_ld32(tm_o + lane_off + c * 32, o);
+                tmem_wait_ld();
+#pragma unroll
+                for (int e = 0; e < 32; e += 2) {
+                  const float2 v = __fmul2_rn(make_float2(o[e], o[e + 1]), make_float2(alpha, alpha));
+                  o[e] = v.x;
+                  o[e + 1] = v.y;
+                }
+                tmem_st32(tm_o + lane_off + c * 32, o);
+              }
+              tmem_wait_st();
+            }
           }
+          fence_before();
+          mbar_arrive(bar(BPF + b));
         }
-        fence_before();
-        mbar_arrive(bar(BPF + b));
+        if (ok && j < w.j1) {
+          // PV(n - 1), whose barrier's next phase needs P(n + 1)
+          ok = __all_sync(0xffffffffu, mbar_wait(bar(BPV + (n - 1) % 2), ((n - 1) >> 1) & 1, abort_flag, p.wait_cycles));
+          if (!ok) break;
+          fence_after();
+          const int slot = 2 * int(blockIdx.x) + (first_seg ? 0 : 1);
+          if (active && FFTS_IN_RANGE(slot, 2 * p.ctas))
+            park_o<D, kBM>(p, slot, r, live, j - w.j0 > kSum, m_ref * p.scale_log2, tm_o + lane_off);
+        }
       }
       if (!ok) break;
       // O is final once the segment's last PV is complete (its barrier's next phase needs our P)
@@ -480,20 +494,24 @@ __global__ void __launch_bounds__(kThreads, 2)
         break;
       }
       fence_after();
+      const int slot = 2 * int(blockIdx.x) + (first_seg ? 0 : 1);
       if (active) {
         const bool whole = w.j0 == 0 && w.j1 == g.n;
-        const int slot = 2 * int(blockIdx.x) + (first_seg ? 0 : 1);
         // a row without a key (pos < 0) is zeros; NaN in l, or no key above -inf (l == 0), is NaN as in the formula
         const bool sees = pos >= 0;
         const float inv_l = 1.0f / l_run;
         uint16_t *dst = p.out + int64_t(w.t.tok0 + tl) * p.os_t + int64_t(w.h * p.G + hg) * p.os_h;
         float4 *pd = reinterpret_cast<float4 *>(p.part) + int64_t(slot) * (kBM * D / 4) + r;
+        float2 *pml = p.part_ml + int64_t(slot) * kBM + r;
+        const bool parked = w.j1 - w.j0 > kSum && live && FFTS_IN_RANGE(slot, 2 * p.ctas);
+        const float f = parked ? weight(pml->x, m_ref * p.scale_log2) : 0.0f;
 #pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {
           float o[32];
           __syncwarp();
           tmem_ld32(tm_o + lane_off + c * 32, o);
           tmem_wait_ld();
+          if (parked) unpark<kBM>(o, pd, c, f);
           if (live && whole && FFTS_IN_RANGE(w.t.tok0 + tl, p.T)) {
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
@@ -504,14 +522,9 @@ __global__ void __launch_bounds__(kThreads, 2)
               *reinterpret_cast<uint4 *>(dst + c * 32 + q * 8) = make_uint4(v[0], v[1], v[2], v[3]);
             }
           }
-          if (live && !whole && FFTS_IN_RANGE(slot, 2 * p.ctas)) {
-#pragma unroll
-            for (int q = 0; q < 8; ++q)
-              pd[(c * 8 + q) * kBM] = make_float4(o[q * 4], o[q * 4 + 1], o[q * 4 + 2], o[q * 4 + 3]);
-          }
+          if (live && !whole && FFTS_IN_RANGE(slot, 2 * p.ctas)) park<kBM>(o, pd, c);
         }
-        if (live && !whole && FFTS_IN_RANGE(slot, 2 * p.ctas))
-          p.part_ml[int64_t(slot) * kBM + r] = make_float2(m_ref * p.scale_log2, l_run);
+        if (live && !whole && FFTS_IN_RANGE(slot, 2 * p.ctas)) *pml = make_float2(m_ref * p.scale_log2, l_run);
       }
       // the share that opens a (q tile, head) and does not end it leaves a note for the join
       if (w.opens && w.j1 - w.j0 < g.n && r == 0 && FFTS_IN_RANGE(blockIdx.x, p.ctas)) {
@@ -555,8 +568,6 @@ constexpr int kJoinBlocks = 2;
 struct Part {
   float m, l;
   float4 o;
-  // the weight of a part with maximum mm in a sum scaled to top
-  static __device__ __forceinline__ float weight(float mm, float top) { return mm == -INFINITY ? 0.0f : exp2f(mm - top); }
   __device__ __forceinline__ void scale(float f) {
     l *= f;
     o.x *= f;
@@ -614,7 +625,7 @@ __global__ void __launch_bounds__(kJoinThreads, 2) join_kernel(const __grid_cons
       float top = t[0].m;
 #pragma unroll
       for (int k = 0; k < JS; ++k) top = fmaxf(top, ml[k].x);
-      const float old = Part::weight(t[0].m, top);
+      const float old = weight(t[0].m, top);
 #pragma unroll
       for (int i = 0; i < JP; ++i) {
         t[i].m = top;
@@ -660,7 +671,7 @@ __global__ void __launch_bounds__(kJoinThreads, 2) join_kernel(const __grid_cons
   Part sum = none;
   for (int k = 0; k < groups; ++k) {
     const Part &q = met[k * items + tid];
-    sum.add(Part::weight(q.m, top), q.l, q.o);
+    sum.add(weight(q.m, top), q.l, q.o);
   }
   store(r, piece, sum);
 }

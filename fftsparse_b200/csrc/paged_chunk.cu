@@ -66,6 +66,7 @@ __global__ void __launch_bounds__(cThreads, 1)
     chunk_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                  const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ Params p) {
   using Lay = ChunkLayout<D>;
+  constexpr int kSum = Num<E>::sum_keys / cBN;  // key tiles after which O is parked
   extern __shared__ __align__(16) uint8_t smem[];
   if (smem_u32(smem) & 1023u) {  // SWIZZLE_128B tiles need 1024-byte alignment
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -268,7 +269,7 @@ __global__ void __launch_bounds__(cThreads, 1)
           // PV of key tile n and S of the one behind it, which may be the next segment's first: then a half's S
           // goes ahead of the other half's PV only if its Q is there
           const int now = halves, kv = nl + 1, kn = nl + 2;
-          const bool first = n == 0, end = n + 1 == n1;
+          const bool first = n % kSum == 0, end = n + 1 == n1;  // first: O starts from zero
           if (end) segment();
           n = end ? 0 : n + 1;
           const bool last = n + 1 == n1;
@@ -328,99 +329,111 @@ __global__ void __launch_bounds__(cThreads, 1)
       const int pos = w.t.pos0 + min(tl, w.t.ntok - 1);
       float m_ref = -INFINITY, l_run = 0.0f;
       if (!mine) kvn += w.j1 - w.j0;
-      for (int j = w.j0; mine && j < w.j1; ++j, ++n, ++kvn) {
-        if (!__all_sync(0xffffffffu, mbar_wait(bar(CSF + x), n & 1, abort_flag, p.wait_cycles))) { ok = false; break; }
-        fence_after();
-        const int c0 = w.key(j) * cBN;
-        if (x == 0 && (c0 + cBN > g.hi || (c0 < g.lo && c0 + cBN > p.sinks))) {
-          // V rows that no row sees, for both halves (A's product is issued before B's)
-          const int v = 2 * kvn + 1, stage = v % cStages;
-          if (!__all_sync(0xffffffffu, mbar_wait(bar(CKF + stage), (v / cStages) & 1, abort_flag, p.wait_cycles))) { ok = false; break; }
-          const int key = c0 + r;
-          if (key >= g.hi || (key < g.lo && key >= p.sinks)) {
+      for (int j = w.j0, stop; mine && ok && j < w.j1;) {
+        stop = min(w.j1, j + kSum);
+        for (; j < stop; ++j, ++n, ++kvn) {
+          if (!__all_sync(0xffffffffu, mbar_wait(bar(CSF + x), n & 1, abort_flag, p.wait_cycles))) { ok = false; break; }
+          fence_after();
+          const int c0 = w.key(j) * cBN;
+          if (x == 0 && (c0 + cBN > g.hi || (c0 < g.lo && c0 + cBN > p.sinks))) {
+            // V rows that no row sees, for both halves (A's product is issued before B's)
+            const int v = 2 * kvn + 1, stage = v % cStages;
+            if (!__all_sync(0xffffffffu, mbar_wait(bar(CKF + stage), (v / cStages) & 1, abort_flag, p.wait_cycles))) { ok = false; break; }
+            const int key = c0 + r;
+            if (key >= g.hi || (key < g.lo && key >= p.sinks)) {
 #pragma unroll
-            for (int hf = 0; hf < Lay::halves; ++hf)
+              for (int hf = 0; hf < Lay::halves; ++hf)
 #pragma unroll
-              for (int i = 0; i < 8; ++i)
-                *reinterpret_cast<uint4 *>(smem + Lay::kv + stage * Lay::tile + hf * Lay::box + r * 128 + i * 16) = make_uint4(0, 0, 0, 0);
+                for (int i = 0; i < 8; ++i)
+                  *reinterpret_cast<uint4 *>(smem + Lay::kv + stage * Lay::tile + hf * Lay::box + r * 128 + i * 16) = make_uint4(0, 0, 0, 0);
+            }
+            fence_proxy_async();
           }
-          fence_proxy_async();
-        }
-        if (active) {
-          // whole: the row sees all keys of the tile
-          const int lim = pos + 1 - c0, from = p.window > 0 ? pos - p.window + 1 - c0 : 0, sink = p.sinks - c0;
-          const bool edge = __any_sync(0xffffffffu, lim < cBN || (from > 0 && sink < cBN));
-          float xs[cBN];
-          auto mask_chunk = [&](int c) {  // 32 columns; from and sink only matter with a window
-            const uint64_t m = (below(lim - 32 * c) & (p.window > 0 ? ~below(from - 32 * c) | below(sink - 32 * c) : ~0ull));
+          if (active) {
+            // whole: the row sees all keys of the tile
+            const int lim = pos + 1 - c0, from = p.window > 0 ? pos - p.window + 1 - c0 : 0, sink = p.sinks - c0;
+            const bool edge = __any_sync(0xffffffffu, lim < cBN || (from > 0 && sink < cBN));
+            float xs[cBN];
+            auto mask_chunk = [&](int c) {  // 32 columns; from and sink only matter with a window
+              const uint64_t m = (below(lim - 32 * c) & (p.window > 0 ? ~below(from - 32 * c) | below(sink - 32 * c) : ~0ull));
 #pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (!((uint32_t(m) >> e) & 1u)) xs[c * 32 + e] = -INFINITY;
-          };
-          float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-          tmem_ld32(s_addr, xs);
+              for (int e = 0; e < 32; ++e)
+                if (!((uint32_t(m) >> e) & 1u)) xs[c * 32 + e] = -INFINITY;
+            };
+            float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            tmem_ld32(s_addr, xs);
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            tmem_wait_ld();
-            if (c < 3) tmem_ld32(s_addr + 32 * (c + 1), xs + 32 * (c + 1));  // lands while this chunk is looked through
-            if (edge) mask_chunk(c);
-#pragma unroll
-            for (int e = 0; e < 32; e += 2) mx4[(e >> 1) & 3] = max3f(mx4[(e >> 1) & 3], xs[c * 32 + e], xs[c * 32 + e + 1]);
-          }
-          const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
-          // P and O stay scaled to m_ref until a score outgrows it by 2^rescale
-          float alpha = 1.0f;
-          if (mx > m_ref && (m_ref == -INFINITY || (mx - m_ref) * p.scale_log2 > Num<E>::rescale)) {
-            alpha = m_ref == -INFINITY ? 0.0f : fast_exp2((m_ref - mx) * p.scale_log2);
-            m_ref = mx;
-          }
-          if (j > w.j0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
-            // O holds PV(n - 1): S(n) was issued after it and is there
-#pragma unroll 1
-            for (int c = 0; c < D / 16; ++c) {
-              float o[16];
-              tmem_ld16(o_addr + c * 16, o);
+            for (int c = 0; c < 4; ++c) {
               tmem_wait_ld();
+              if (c < 3) tmem_ld32(s_addr + 32 * (c + 1), xs + 32 * (c + 1));  // lands while this chunk is looked through
+              if (edge) mask_chunk(c);
 #pragma unroll
-              for (int e = 0; e < 16; ++e) o[e] *= alpha;
-              tmem_st16(o_addr + c * 16, o);
+              for (int e = 0; e < 32; e += 2) mx4[(e >> 1) & 3] = max3f(mx4[(e >> 1) & 3], xs[c * 32 + e], xs[c * 32 + e + 1]);
             }
-            tmem_wait_st();
-          }
-          const float moff = (m_ref == -INFINITY ? 0.0f : m_ref) * p.scale_log2;
-          const float2 off2 = make_float2(-moff, -moff);
-          float2 rs2[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
-          auto exp_chunk = [&](int c) {
-            uint32_t pk[16];
-#pragma unroll
-            for (int e = 0; e < 32; e += 2) {
-              const float2 a = __ffma2_rn(make_float2(xs[c * 32 + e], xs[c * 32 + e + 1]), sc2, off2);
-              float2 ex;
-              ex.x = fast_exp2(a.x);
-              ex.y = fast_exp2(a.y);
-              rs2[(e >> 1) & 1] = __fadd2_rn(rs2[(e >> 1) & 1], ex);
-              pk[e >> 1] = Num<E>::pack(ex.x, ex.y);
+            const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+            // P and O stay scaled to m_ref until a score outgrows it by 2^rescale
+            float alpha = 1.0f;
+            if (mx > m_ref && (m_ref == -INFINITY || (mx - m_ref) * p.scale_log2 > Num<E>::chunk_rescale)) {
+              alpha = m_ref == -INFINITY ? 0.0f : fast_exp2((m_ref - mx) * p.scale_log2);
+              m_ref = mx;
             }
-            tmem_st16u(s_addr + c * 16, pk);
-          };
+            if (j > w.j0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
+              // O holds PV(n - 1): S(n) was issued after it and is there
+#pragma unroll 1
+              for (int c = 0; c < D / 16; ++c) {
+                float o[16];
+                tmem_ld16(o_addr + c * 16, o);
+                tmem_wait_ld();
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            exp_chunk(c);
-            if (c == 1) {  // the first 64 keys' product can start
+                for (int e = 0; e < 16; ++e) o[e] *= alpha;
+                tmem_st16(o_addr + c * 16, o);
+              }
               tmem_wait_st();
-              fence_before();
-              mbar_arrive(bar(CPF + 2 * x));
             }
+            const float moff = (m_ref == -INFINITY ? 0.0f : m_ref) * p.scale_log2 - Num<E>::bias;
+            const float2 off2 = make_float2(-moff, -moff);
+            float2 rs2[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+            auto exp_chunk = [&](int c) {
+              uint32_t pk[16];
+#pragma unroll
+              for (int e = 0; e < 32; e += 2) {
+                const float2 a = __ffma2_rn(make_float2(xs[c * 32 + e], xs[c * 32 + e + 1]), sc2, off2);
+                float2 ex;
+                ex.x = fast_exp2(a.x);
+                ex.y = fast_exp2(a.y);
+                rs2[(e >> 1) & 1] = __fadd2_rn(rs2[(e >> 1) & 1], ex);
+                pk[e >> 1] = Num<E>::pack(ex.x, ex.y);
+              }
+              tmem_st16u(s_addr + c * 16, pk);
+            };
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              exp_chunk(c);
+              if (c == 1) {  // the first 64 keys' product can start
+                tmem_wait_st();
+                fence_before();
+                mbar_arrive(bar(CPF + 2 * x));
+              }
+            }
+            const float2 rsum = __fadd2_rn(rs2[0], rs2[1]);
+            l_run = l_run * alpha + (rsum.x + rsum.y);
+            tmem_wait_st();
+          } else {
+            fence_before();
+            mbar_arrive(bar(CPF + 2 * x));
           }
-          const float2 rsum = __fadd2_rn(rs2[0], rs2[1]);
-          l_run = l_run * alpha + (rsum.x + rsum.y);
-          tmem_wait_st();
-        } else {
           fence_before();
-          mbar_arrive(bar(CPF + 2 * x));
+          mbar_arrive(bar(CPF + 2 * x + 1));
         }
-        fence_before();
-        mbar_arrive(bar(CPF + 2 * x + 1));
+        if (ok && j < w.j1) {
+          // O holds PV(n - 1) once S(n) is there, which was issued after it
+          ok = __all_sync(0xffffffffu, mbar_wait(bar(CSF + x), n & 1, abort_flag, p.wait_cycles));
+          if (!ok) break;
+          fence_after();
+          const int slot = 2 * int(blockIdx.x) + (first_seg ? 0 : 1);
+          if (active && FFTS_IN_RANGE(slot, 2 * p.ctas))
+            park_o<D, 2 * cBM>(p, slot, row, r < qrows && row < nrows, j - w.j0 > kSum, m_ref * p.scale_log2, o_addr);
+        }
       }
       if (!ok) break;
       if (mine) {
@@ -430,18 +443,22 @@ __global__ void __launch_bounds__(cThreads, 1)
       }
       const int slot = 2 * int(blockIdx.x) + (first_seg ? 0 : 1);
       if (active) {
-        const bool whole = w.j0 == 0 && w.j1 == g.n;
         const bool live = r < qrows && row < nrows;
+        const bool whole = w.j0 == 0 && w.j1 == g.n;
         const bool sees = pos >= 0;  // a row without a key is zeros; NaN in l, or l == 0, is NaN as in the formula
         const float inv_l = 1.0f / l_run;
         uint16_t *dst = p.out + int64_t(w.t.tok0 + tl) * p.os_t + int64_t(w.h * p.G + hg) * p.os_h;
         float4 *pd = reinterpret_cast<float4 *>(p.part) + int64_t(slot) * (2 * cBM * D / 4) + row;
+        float2 *pml = p.part_ml + int64_t(slot) * (2 * cBM) + row;
+        const bool parked = w.j1 - w.j0 > kSum && live && FFTS_IN_RANGE(slot, 2 * p.ctas);
+        const float f = parked ? weight(pml->x, m_ref * p.scale_log2) : 0.0f;
 #pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {
           float o[32];
           __syncwarp();
           tmem_ld32(o_addr + c * 32, o);
           tmem_wait_ld();
+          if (parked) unpark<(2 * cBM)>(o, pd, c, f);
           if (live && whole && FFTS_IN_RANGE(w.t.tok0 + tl, p.T)) {
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
@@ -452,14 +469,9 @@ __global__ void __launch_bounds__(cThreads, 1)
               *reinterpret_cast<uint4 *>(dst + c * 32 + q * 8) = make_uint4(v[0], v[1], v[2], v[3]);
             }
           }
-          if (live && !whole && FFTS_IN_RANGE(slot, 2 * p.ctas)) {
-#pragma unroll
-            for (int q = 0; q < 8; ++q)
-              pd[(c * 8 + q) * (2 * cBM)] = make_float4(o[q * 4], o[q * 4 + 1], o[q * 4 + 2], o[q * 4 + 3]);
-          }
+          if (live && !whole && FFTS_IN_RANGE(slot, 2 * p.ctas)) park<(2 * cBM)>(o, pd, c);
         }
-        if (live && !whole && FFTS_IN_RANGE(slot, 2 * p.ctas))
-          p.part_ml[int64_t(slot) * (2 * cBM) + row] = make_float2(m_ref * p.scale_log2, l_run);
+        if (live && !whole && FFTS_IN_RANGE(slot, 2 * p.ctas)) *pml = make_float2(m_ref * p.scale_log2, l_run);
       }
       // the share that opens a (q tile, head) and does not end it leaves a note for the join
       if (w.opens && w.j1 - w.j0 < g.n && threadIdx.x == 0 && FFTS_IN_RANGE(blockIdx.x, p.ctas)) {

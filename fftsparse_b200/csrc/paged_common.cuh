@@ -258,6 +258,12 @@ struct Walk {
 
 __device__ __forceinline__ uint64_t below(int k) { return k <= 0 ? 0ull : (k >= 64 ? ~0ull : (1ull << k) - 1ull); }
 
+// sum_keys: the tensor core cuts every product p v off at 2^-25 of the sum it is added to (so it measured: behind a
+// key of weight 1, products of 2^-25 count and those of 0.53 of that do not), while the divisor is summed exactly.
+// Behind one heavy key many light ones would be lost, 131072 of them 2^-8 of the result.  So O is parked after so
+// many keys and starts again from zero, which bounds the loss by one rounding of the result; what is parked is
+// added up in fp32.  2048 tokens over 131072, 32 / 8 heads: fp16 4.37 ms without, 4.46 with, 4.52 with half as
+// many keys to a sum; bf16 4.22 all three.
 template <typename E>
 struct Num;
 template <>
@@ -265,7 +271,8 @@ struct Num<__nv_bfloat16> {
   static constexpr uint32_t fmt = 1;
   static constexpr CUtensorMapDataType map = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   // P <= 2^64 against the reference max: bf16 and the fp32 O have the exponents for it
-  static constexpr float rescale = 64.0f, pmax = 18446744073709551616.0f;
+  static constexpr float rescale = 64.0f, pmax = 18446744073709551616.0f, bias = 0.0f, chunk_rescale = 64.0f;
+  static constexpr int sum_keys = 131072;
   static __device__ __forceinline__ uint32_t pack(float a, float b) {
     const __nv_bfloat162 r = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const uint32_t *>(&r);
@@ -275,9 +282,13 @@ template <>
 struct Num<__half> {
   static constexpr uint32_t fmt = 0;
   static constexpr CUtensorMapDataType map = CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-  // fp16 ends at 65504: P <= 2^8 after a rescale, 2^14 (a tile's row sum) before the next one; the row's
-  // top has P >= 1, so what is lost below 2^-24 is that far under it
-  static constexpr float rescale = 8.0f, pmax = 16384.0f;
+  // fp16 ends at 65504, and its smallest step is 2^-24: P is off by up to 2^-25, and the errors of many small ones add
+  // up (the divisor sums them unrounded).  So the reference maximum stands at 2^bias: an error is 2^-32 of the
+  // row's top at most.  What outgrows the reference by 2^rescale resets it.  The smaller tiles exponentiate before they
+  // look, and look when 64 keys sum to more than pmax, which takes one that has (2^9.99 < 65504 / 64); the larger
+  // tiles look first, and rescale seldom (at 2^2.99: 2048 tokens over 32768 1112 -> 1150 us).
+  static constexpr float rescale = 2.99f, pmax = 65504.0f, bias = 7.0f, chunk_rescale = 8.0f;
+  static constexpr int sum_keys = 16384;
   static __device__ __forceinline__ uint32_t pack(float a, float b) {
     const __half2 r = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t *>(&r);
@@ -367,6 +378,47 @@ static int launch_early(void (*kernel)(Ts...), dim3 grid, int threads, int smem,
   cfg.numAttrs = 1;
   FFTS_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
   return FFTS_OK;
+}
+
+// The weight of a partial with maximum m (log2 units) in a sum scaled to top; NaN stays NaN in what it multiplies.
+__device__ __forceinline__ float weight(float m, float top) { return m == -INFINITY ? 0.0f : exp2f(m - top); }
+
+// 32 channels of a row's O, from channel 32 c on, to a slot of the partials (rows side by side).
+template <int ROWS>
+__device__ __forceinline__ void park(const float *o, float4 *pd, int c) {
+#pragma unroll
+  for (int q = 0; q < 8; ++q) pd[(c * 8 + q) * ROWS] = make_float4(o[q * 4], o[q * 4 + 1], o[q * 4 + 2], o[q * 4 + 3]);
+}
+// o += f * what the slot holds of them.
+template <int ROWS>
+__device__ __forceinline__ void unpark(float *o, const float4 *pd, int c, float f) {
+#pragma unroll
+  for (int q = 0; q < 8; ++q) {
+    const float4 old = pd[(c * 8 + q) * ROWS];
+    o[q * 4] = fmaf(f, old.x, o[q * 4]);
+    o[q * 4 + 1] = fmaf(f, old.y, o[q * 4 + 1]);
+    o[q * 4 + 2] = fmaf(f, old.z, o[q * 4 + 2]);
+    o[q * 4 + 3] = fmaf(f, old.w, o[q * 4 + 3]);
+  }
+}
+// Adds a row's O in TMEM to what the slot holds (again), or puts it there; m: what it is scaled to, at least the
+// slot's.  Not inlined: inside the softmax loop its registers cost 5% (2048 tokens over 32768 1085 -> 1145 us).
+template <int D, int ROWS>
+__device__ __noinline__ void park_o(const Params &p, int slot, int row, bool live, bool again, float m,
+                                    uint32_t o_addr) {
+  float4 *pd = reinterpret_cast<float4 *>(p.part) + int64_t(slot) * (ROWS * D / 4) + row;
+  float2 *pml = p.part_ml + int64_t(slot) * ROWS + row;
+  const float f = again && live ? weight(pml->x, m) : 0.0f;
+#pragma unroll 1
+  for (int c = 0; c < D / 32; ++c) {
+    float o[32];
+    __syncwarp();
+    tmem_ld32(o_addr + c * 32, o);
+    tmem_wait_ld();
+    if (again && live) unpark<ROWS>(o, pd, c, f);
+    if (live) park<ROWS>(o, pd, c);
+  }
+  if (live) pml->x = m;
 }
 
 // The kernel of paged_chunk.cu: p with tiles of 256 rows, K and V maps with boxes of up to 128 keys.

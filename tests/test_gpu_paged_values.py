@@ -8,7 +8,7 @@ import pytest
 import torch
 
 import fftsparse_b200 as F
-from test_gpu_paged import BF, NAN, Batch
+from test_gpu_paged import BF, FP, NAN, Batch, ints
 
 pytestmark = pytest.mark.gpu
 
@@ -60,4 +60,95 @@ def test_broken_scores_reach_their_rows_and_no_others(last):
     got = b.run()
     assert check_broken(b, got) > 0
     assert bool(got[840:, :4].isnan().all()) and bool(got[840:, 4:].isfinite().all())
+    F.check_status()
+
+
+# ------------------------------------------------------------------ sums of many small weights
+SUM_KEYS = {FP: 16384, BF: 131072}  # keys that the tensor core sums up before the sum is taken over
+
+
+def sum_error(dt):
+    """Of such a sum, relative to what its terms' sizes sum to: 16 products at a time, each cut at 2^-25 of the sum,
+    then the sum at its last step, 2^-23."""
+    return SUM_KEYS[dt] * (2.0 ** -25 + 2.0 ** -23 / 16)
+
+
+@pytest.mark.parametrize("deficit,keys", [(24.9, 131072), (25.01, 131072), (25.9, 131072), (31.9, 131072),
+                                          (32.01, 131072), (25.01, 1 << 20), (25.9, 1 << 20)])
+@pytest.mark.parametrize("top", [1.0, 0.0])
+@pytest.mark.parametrize("chunk", [False, True])
+@pytest.mark.parametrize("dt", [FP, BF])
+def test_many_keys_far_below_the_first_one(dt, chunk, top, deficit, keys):
+    """The first key outweighs each of the others by 2^deficit, together they count: sum p v with v = top for the
+    first key, 1 for the others.
+
+    One rounding of the result.  P in fp16 is off by at most half of its smallest step, 2^-25; a row's maximum stands at
+    2^7 or above, so each of the keys is off by at most 2^-32 of the first one's weight.  P in bf16 is off by one
+    rounding.  The tensor core's sums, at most 1 of the total weight each, are off by sum_error; the ones without the
+    first key in proportion to their own keys."""
+    D, page = 64, 256
+    k = torch.zeros(keys // page + 1, 1, page, D, dtype=dt, device="cuda")
+    k[..., 0] = -16.0
+    k[0, 0, 0, 0] = 0.0
+    v = torch.ones_like(k)
+    v[0, 0, 0] = top
+    # as many (q tile, head)s as CTAs, so that a share holds a whole one
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    R, T = (1, 256 * sms) if chunk else (2 * sms, 2 * sms)
+    if chunk:
+        lens, cu = [keys + T], [0, T]
+        more = T // page + 1
+        k, v = (torch.cat([x, x[1:2].expand(more, -1, -1, -1)]) for x in (k, v))
+        n = torch.arange(keys, keys + T, device="cuda").double()  # keys that a row sees besides the first one
+    else:
+        lens, cu = [keys] * R, list(range(R + 1))
+        n = torch.full((T,), keys - 1.0, device="cuda", dtype=torch.float64)
+    table = torch.arange(k.shape[0], dtype=torch.int32, device="cuda").repeat(R, 1)
+    q = torch.zeros(T, 1, D, dtype=dt, device="cuda")
+    q[..., 0] = 1.0
+    scale = deficit * math.log(2.0) / 16.0
+    got = F.paged_attention(q, k, v, table, ints(cu), ints(lens), scale=scale)[:, 0].double()
+    rest = n * 2.0 ** -deficit
+    want, u = (top + rest) / (1.0 + rest), torch.finfo(dt).eps / 2
+    tol = u * want + sum_error(dt) + (n * 2.0 ** -32 if dt == FP else u * want)
+    err = (got - want[:, None]).abs()
+    assert bool((err <= tol[:, None]).all()), (float(err.max()), float(tol.min()))
+    F.check_status()
+
+
+@pytest.mark.parametrize("dt,keys", [(FP, 30011), (BF, 150001)])
+@pytest.mark.parametrize("chunk", [False, True])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (0.6, 70)])
+def test_long_rows_in_one_share(chunk, dt, keys, window, sinks):
+    """Rows of several sums each, whole in one share: random values against 64 bits, at the tolerance of test_gpu_paged.py
+    with the sums' own error instead of one that grows with the keys."""
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    D, page, T = 64, 64, (256 * sms if chunk else 2 * sms)
+    if chunk and dt == BF:
+        keys = 90001
+    window = window and int(window * keys)
+    g = torch.Generator(device="cuda").manual_seed(keys)
+    first = keys - T if chunk else 0  # position of the first row; a decoding row is at keys - 1
+    pages = -(-keys // page)
+    k, v = (torch.randn(pages, 1, page, D, generator=g, device="cuda").to(dt) for _ in range(2))
+    q = (torch.randn(T, 1, D, generator=g, device="cuda") * 2).to(dt)
+    R = 1 if chunk else T
+    table = torch.arange(pages, dtype=torch.int32, device="cuda").repeat(R, 1)
+    got = F.paged_attention(q, k, v, table, ints([0, T] if chunk else list(range(T + 1))), ints([keys] * R), window=window,
+                            sinks=sinks if window else 0)
+    u = torch.finfo(dt).eps / 2
+    k, v = k.double().flatten(0, 2)[:keys], v.double().flatten(0, 2)[:keys]
+    rows = torch.randperm(T, generator=torch.Generator().manual_seed(1))[:300].cuda()
+    s = q[rows, 0].double() @ k.T * D ** -0.5
+    S = float((q[rows, 0].double().abs() @ k.abs().T).max()) * D ** -0.5
+    i, j = (rows + first if chunk else torch.full_like(rows, keys - 1))[:, None], torch.arange(keys, device="cuda")
+    seen = j <= i
+    if window:
+        seen &= (j > i - window) | (j < sinks)
+    p = s.masked_fill(~seen, -math.inf).softmax(-1)
+    p = torch.where(seen.any(-1, keepdim=True), p, 0.0)  # a row before the first key: zeros
+    want, A = p @ v, p @ v.abs()
+    e = 2 * ((D + 2) * 2.0 ** -23 * S + 2.0 ** -20)
+    tol = u * want.abs() + (u + e + sum_error(dt)) * A + (keys * 2.0 ** -32 * float(v.abs().max()) if dt == FP else 0.0)
+    assert bool(((got[rows, 0].double() - want).abs() <= tol).all())
     F.check_status()

@@ -138,6 +138,23 @@ __host__ __device__ __forceinline__ int ilog2_ceil(int64_t m) {
   return r;
 }
 
+// Whether the rows of inner elements at the sums of i_k * strides[k], i_k < sizes[k] (n of them, at most 3), are apart
+// from one another, as a tensor that kernels write needs: each axis steps over all that the axes of smaller strides span.
+inline bool rows_apart(const int64_t *sizes, const int64_t *strides, int n, int64_t inner) {
+  bool used[3] = {};
+  int64_t span = inner;
+  for (int k = 0; k < n; ++k) {
+    int at = -1;  // the axis of the next larger stride
+    for (int i = 0; i < n; ++i)
+      if (!used[i] && (at < 0 || strides[i] < strides[at])) at = i;
+    used[at] = true;
+    if (sizes[at] <= 1) continue;  // its stride says nothing
+    if (strides[at] < span) return false;
+    span += (sizes[at] - 1) * strides[at];
+  }
+  return true;
+}
+
 // ----------------------------------------------------- bounds-checked build
 // Compute-sanitizer is not available where this library is tested, so the
 // library has a second build, libfftsparse_b200_checked.so, compiled with

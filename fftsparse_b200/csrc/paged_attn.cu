@@ -794,7 +794,9 @@ int paged_attn(const ffts_paged_attn_args &a, cudaStream_t stream) {
     FFTS_REQUIRE((reinterpret_cast<uintptr_t>(x) & 15) == 0, "paged_attn: tensors must be 16-byte aligned");
   const int64_t *qs = a.q_strides, *os = a.out_strides;
   FFTS_REQUIRE(qs[0] > 0 && qs[1] > 0 && qs[0] % 8 == 0 && qs[1] % 8 == 0 && os[0] % 8 == 0 && os[1] % 8 == 0,
-               "paged_attn: q and out strides must be positive multiples of 8 elements (16 bytes)");
+               "paged_attn: q and out strides must be multiples of 8 elements (16 bytes), q's positive");
+  const int64_t out_sizes[2] = {T, H};
+  FFTS_REQUIRE(rows_apart(out_sizes, os, 2, D), "paged_attn: rows of out overlap");
   for (const int64_t *st : {a.kp_strides, a.vp_strides})
     for (int i = 0; i < 3; ++i)
       FFTS_REQUIRE(st[i] > 0 && st[i] % 8 == 0 && st[i] < (int64_t(1) << 38),

@@ -208,6 +208,10 @@ int rope_append(const ffts_rope_append_args &a, cudaStream_t stream) {
   for (const int64_t *st : {a.kp_strides, a.vp_strides})
     FFTS_REQUIRE(st[0] % 8 == 0 && st[1] % 8 == 0 && st[2] % 8 == 0,
                  "rope_append: page strides must be multiples of 8 elements (16 bytes)");
+  const int64_t out_sizes[2] = {T, H}, pool_sizes[3] = {a.n_pages, Hkv, a.page_size};
+  FFTS_REQUIRE(!a.q || rows_apart(out_sizes, a.out_strides, 2, D), "rope_append: rows of the rotated q overlap");
+  FFTS_REQUIRE(rows_apart(pool_sizes, a.kp_strides, 3, D) && rows_apart(pool_sizes, a.vp_strides, 3, D),
+               "rope_append: rows of the pages overlap");
   Params p{};
   p.q = static_cast<const uint16_t *>(a.q);
   p.k = static_cast<const uint16_t *>(a.k);

@@ -245,7 +245,8 @@ FFTS_API int32_t ffts_page_plan(const ffts_page_plan_args *args, void *stream);
  *     copied.  rotary_dim a multiple of 16 up to D; 0 copies k and v as they are.
  *   k_pages, v_pages [n_pages, Hkv, page_size, D]: strides (page, head, row).
  * Angles are reduced in 64 bits, the rest is fp32, rounded once.  bf16 or fp16, D 64
- * or 128; all strides multiples of 8 elements, tensors 16-byte aligned.
+ * or 128; all strides multiples of 8 elements, tensors 16-byte aligned; the rows of
+ * what is written (q_out, the pages) may not overlap one another.
  */
 typedef struct ffts_rope_append_args {
   int64_t struct_bytes;
@@ -282,8 +283,8 @@ FFTS_API int32_t ffts_rope_append(const ffts_rope_append_args *args, void *strea
  *     misaligned shared memory; the output is then invalid.
  * fp32 scores, softmax and accumulation, P rounded to the inputs' type for the
  * second product.  bf16 or fp16, D 64 or 128, H / Hkv <= 128, page_size 16 to 256
- * (a power of two); q and page strides multiples of 8 elements, tensors 16-byte
- * aligned.
+ * (a power of two); q, out and page strides multiples of 8 elements, tensors 16-byte
+ * aligned; the rows of out may not overlap one another.
  */
 typedef struct ffts_paged_attn_args {
   int64_t struct_bytes;

@@ -152,3 +152,37 @@ def test_long_rows_in_one_share(chunk, dt, keys, window, sinks):
     tol = u * want.abs() + (u + e + sum_error(dt)) * A + (keys * 2.0 ** -32 * float(v.abs().max()) if dt == FP else 0.0)
     assert bool(((got[rows, 0].double() - want).abs() <= tol).all())
     F.check_status()
+
+
+# ------------------------------------------------------------------ tensors whose rows overlap
+def test_outputs_whose_rows_overlap_are_refused():
+    z = lambda *s: torch.zeros(*s, dtype=BF, device="cuda")  # noqa: E731
+    T, H, Hkv, D, P, page = 3, 4, 2, 64, 2, 16
+    q, k, pool = z(T, H, D), z(T, Hkv, D), z(P, Hkv, page, D)
+
+    def attend(out):
+        F.paged_attention(q, pool, pool.clone(), ints([[0]]), ints([0, T]), ints([T]), out=out)
+
+    def append(out=None, kp=pool, vp=pool.clone()):
+        F.rope_append(q, k, k.clone(), ints([0, 1, 2]), ints([0, 1, 2]), kp, vp, None, out=out)
+
+    wide = z(H, T + 1, D + 8)
+    for out in (q, z(T, H, D), wide[:, :T, :D].transpose(0, 1), wide[:, 1:, 8:].transpose(0, 1)):
+        attend(out)
+        append(out)
+    for out in (z(1, H, D).expand(T, H, D), z(T, 1, D).expand(T, H, D), z(1000).as_strided((T, H, D), (D, D, 1)),
+                z(1000).as_strided((T, H, D), (H * D - 8, D, 1)), z(1000).as_strided((T, H, D), (H * D, D - 8, 1))):
+        with pytest.raises(ValueError, match="overlap"):
+            attend(out)
+        with pytest.raises(ValueError, match="overlap"):
+            append(out)
+    append(kp=z(P, page, Hkv, D).transpose(1, 2))
+    for bad in (z(1, Hkv, page, D).expand(P, -1, -1, -1), z(P, 1, page, D).expand(-1, Hkv, -1, -1),
+                z(P, Hkv, 1, D).expand(-1, -1, page, -1), z(9000).as_strided((P, Hkv, page, D), (page * D, page * D, D, 1))):
+        with pytest.raises(ValueError, match="overlap"):
+            append(kp=bad)
+        with pytest.raises(ValueError, match="overlap"):
+            append(vp=bad)
+    # inputs may be broadcast
+    F.rope_append(z(1, H, D).expand(T, H, D), z(T, 1, D).expand(T, Hkv, D), k, ints([0, 1, 2]), ints([0, 1, 2]), pool,
+                  pool.clone(), None)

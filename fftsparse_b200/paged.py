@@ -172,7 +172,8 @@ def plan_pages(cached_lens: torch.Tensor, new_lens: torch.Tensor, block_table: t
 
 
 def rotary_inv_freq(rotary_dim: int, base: float = 10000.0, scaling: Optional[dict] = None,
-                    seq_len: Optional[int] = None, device=None) -> Tuple[torch.Tensor, float]:
+                    seq_len: Optional[int] = None, device=None, *,
+                    max_position_embeddings: Optional[int] = None) -> Tuple[torch.Tensor, float]:
     """(inv_freq fp32 [rotary_dim / 2], attn_factor) of a rotary embedding, as ``rope_append`` takes them.
 
     ``scaling`` is a model configuration's ``rope_scaling`` dict; its ``rope_type`` is one of
@@ -186,7 +187,8 @@ def rotary_inv_freq(rotary_dim: int, base: float = 10000.0, scaling: Optional[di
                (whole channels unless truncate is false); attn_factor = attention_factor, or m(mscale) / m(mscale_all_dim)
                where both are given, or m(1), with m(x) = 0.1 x ln(factor) + 1
 
-    with L0 = ``original_max_position_embeddings``.  Computed in 64 bits, rounded once.
+    with L0 = the dict's ``original_max_position_embeddings``, or, where it has none, ``max_position_embeddings`` (the
+    configuration's own).  Computed in 64 bits, rounded once.
     """
     if rotary_dim <= 0 or rotary_dim % 2:
         raise ValueError(f"rotary_dim must be a positive even number, got {rotary_dim}")
@@ -198,25 +200,30 @@ def rotary_inv_freq(rotary_dim: int, base: float = 10000.0, scaling: Optional[di
     attn = 1.0
 
     def need(key):
-        if key not in scaling:
+        if scaling.get(key) is None:
             raise ValueError(f"rope scaling '{kind}' needs '{key}'")
         return float(scaling[key])
 
+    def context():
+        if scaling.get("original_max_position_embeddings") is None and max_position_embeddings is not None:
+            return float(max_position_embeddings)
+        return need("original_max_position_embeddings")
+
     if kind == "dynamic":
-        L0, s = need("original_max_position_embeddings"), need("factor")
+        L0, s = context(), need("factor")
         L = max(float(seq_len or 0), L0)
         base = base * (s * L / L0 - (s - 1.0)) ** (d / (d - 2))
     f = float(base) ** (-i / d)
     if kind == "linear":
         f = f / need("factor")
     elif kind == "llama3":
-        L0, s = need("original_max_position_embeddings"), need("factor")
+        L0, s = context(), need("factor")
         low, high = need("low_freq_factor"), need("high_freq_factor")
         turns = L0 * f / (2.0 * math.pi)  # within the original context
         keep = ((turns - low) / (high - low)).clamp(0.0, 1.0)
         f = keep * f + (1.0 - keep) * f / s
     elif kind == "yarn":
-        L0, s = need("original_max_position_embeddings"), need("factor")
+        L0, s = context(), need("factor")
 
         def channel(turns):  # the pair that turns so often within L0
             return d * math.log(L0 / (turns * 2.0 * math.pi)) / (2.0 * math.log(base))

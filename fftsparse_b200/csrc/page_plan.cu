@@ -4,7 +4,7 @@
 //   have_r = ceil(c_r / ps), last_r = ceil((c_r + n_r) / ps), need_r = last_r - have_r
 //   start_r = sum of need over the requests before r        (its first entry of the free list)
 //   table[r][have_r + i] = free[start_r + i], i < need_r
-//   token t of request r: pos = c_r + (t - cu_q[r]), slot = table[r][pos / ps] * ps + pos % ps
+//   token t of request r: pos = c_r + (t - cu_q[r]), slot = table[r][pos / ps] * ps + pos % ps, -1 if that is no int32
 // A request is served if its pages fit the table row, its tokens fit num_tokens and its pages fit the
 // free list (start_r + need_r <= n_free, or it needs none).  An unserved request gets kv_len 0 and slots
 // -1; one that fails the first two conditions asks for no pages, so the later requests' do not move.
@@ -130,7 +130,8 @@ __global__ void __launch_bounds__(kThreads) page_plan_kernel(const __grid_consta
         const int page = col < have_i
                              ? p.table[int64_t(r0 + i) * p.table_ld + FFTS_INDEX(col, p.width)]
                              : p.free_pages[FFTS_INDEX(int(s_pages[i] - s_need[i]) + col - have_i, p.n_free)];
-        slot = int(uint32_t(page) << p.ps_shift) + (pos & (ps - 1));
+        // a number of no pool (negative, or its slots pass 31 bits) gives no slot, not another page's
+        if (uint32_t(page) < (0x80000000u >> p.ps_shift)) slot = int(uint32_t(page) << p.ps_shift) + (pos & (ps - 1));
       }
       p.positions[t] = pos;
       p.slots[t] = slot;

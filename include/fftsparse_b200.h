@@ -214,8 +214,9 @@ FFTS_API int32_t ffts_decode_attn(const void *q, int64_t q_stride_b, int64_t q_s
  *   cu_q [R + 1]: first token of each request (at most num_tokens); kv_lens [R]:
  *     cached + new.
  *   positions, slots [num_tokens]: each token's position in its request, and
- *     page * page_size + row of its place in the pool.  Rows behind the last
- *     request's tokens get position 0 and slot -1.
+ *     page * page_size + row of its place in the pool (-1 for a page number that is
+ *     negative or whose slots pass 31 bits).  Rows behind the last request's tokens
+ *     get position 0 and slot -1.
  *   info [2]: pages taken from the list, requests not served.
  * A request is served if its pages fit its table row, its tokens fit num_tokens and
  * its new pages, counted on from the requests before it, fit the list; one that

@@ -186,3 +186,22 @@ def test_outputs_whose_rows_overlap_are_refused():
     # inputs may be broadcast
     F.rope_append(z(1, H, D).expand(T, H, D), z(T, 1, D).expand(T, Hkv, D), k, ints([0, 1, 2]), ints([0, 1, 2]), pool,
                   pool.clone(), None)
+
+
+# ------------------------------------------------------------------ page numbers of no pool
+@pytest.mark.parametrize("page", [1, 16, 4096])
+def test_page_numbers_outside_every_pool_give_no_slot(page):
+    """A slot is an int32: a page number whose slots do not fit, or a negative one, gives -1 and never another page's slot."""
+    most = 2 ** 31 // page
+    pages = [x for x in (-1, -most, -2 ** 31, most, most + 5, 2 ** 31 - 1, 0, most - 1) if x < 2 ** 31]
+    R, have = len(pages), -(-(page - 1) // page)
+    new = page + 2  # ends in the third page; the first one is in the table unless a page is a token
+    free = ints([x for p in pages for x in (p, p, 3)[have:]])
+    p = F.plan_pages(ints([page - 1] * R), ints([new] * R), ints([[x, -9, -9] for x in pages]), free, page, new * R)
+    assert p.info.tolist() == [(3 - have) * R, 0]
+    want = []
+    for x in pages:
+        for pos in range(page - 1, 2 * page + 1):
+            at = (x, x, 3)[pos // page]
+            want.append(at * page + pos % page if 0 <= at < most else -1)
+    assert p.slot_map.tolist() == want

@@ -179,15 +179,18 @@ static __device__ __noinline__ void note(int line) {
   atomicAdd(&g_count, 1u);
 }
 
-static __device__ __forceinline__ bool in_range(long long i, long long n, int line) {
+// (functions that the host calls too record nothing there)
+static __host__ __device__ __forceinline__ bool in_range(long long i, long long n, int line) {
   const bool ok = i >= 0 && i < n;
+#ifdef __CUDA_ARCH__
   if (!ok) note(line);
+#endif
   return ok;
 }
 
 // i when 0 <= i < n, else (after recording the failure) 0, a valid index of any
 // non-empty extent: for loads whose address the caller cannot skip
-static __device__ __forceinline__ long long checked_index(long long i, long long n, int line) {
+static __host__ __device__ __forceinline__ long long checked_index(long long i, long long n, int line) {
   return in_range(i, n, line) ? i : 0;
 }
 

@@ -533,7 +533,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         cut.pos0 = w.t.pos0;
         cut.nrows = nrows;
         cut.head0 = w.h * p.G;
-        cut.s1 = int((u0 + w.begin + p.overhead + g.n - 1) / per);
+        cut.s1 = w.last_share(u0, per);
         cut.first_slot = 2 * int(blockIdx.x) + (first_seg ? 0 : 1);
         p.cuts[blockIdx.x] = cut;
         noted = true;

@@ -480,7 +480,7 @@ __global__ void __launch_bounds__(cThreads, 1)
         cut.pos0 = w.t.pos0;
         cut.nrows = nrows;
         cut.head0 = w.h * p.G;
-        cut.s1 = int((u0 + w.begin + p.overhead + g.n - 1) / per);
+        cut.s1 = w.last_share(u0, per);
         cut.first_slot = slot;
         p.cuts[blockIdx.x] = cut;
         noted = true;

@@ -65,7 +65,7 @@ struct Keys {
 };
 
 template <int BN>
-__device__ __forceinline__ Keys keys_of(int pos0, int ntok, int window, int sinks) {
+__host__ __device__ __forceinline__ Keys keys_of(int pos0, int ntok, int window, int sinks) {
   Keys g;
   g.hi = max(0, pos0 + ntok);
   g.lo = window > 0 ? max(0, pos0 - window + 1) : 0;
@@ -77,9 +77,9 @@ __device__ __forceinline__ Keys keys_of(int pos0, int ntok, int window, int sink
 }
 
 // The j-th of them.
-__device__ __forceinline__ int key_tile(const Keys &g, int j) { return j < g.st ? j : j - g.st + g.wt0; }
+__host__ __device__ __forceinline__ int key_tile(const Keys &g, int j) { return j < g.st ? j : j - g.st + g.wt0; }
 
-__device__ __forceinline__ long long share_of(const Params &p, long long length) {
+__host__ __device__ __forceinline__ long long share_of(const Params &p, long long length) {
   const long long per = (length + p.ctas - 1) / p.ctas;
   return per < kMinShare ? kMinShare : per;
 }
@@ -177,15 +177,14 @@ __global__ void __launch_bounds__(kSchedThreads) schedule_kernel(const __grid_co
   if (threadIdx.x == 0) p.header[0] = n;
 }
 
-// Walks a share segment by segment; the same in every lane.  Positions are kept relative to the share and to the q
-// tile, in 32 bits: the host refuses a q tile whose heads' line passes 2^31, and a share that did would run for
-// days.
+// Walks a share segment by segment; the same in every lane.  Positions are kept relative to the share, in 64 bits, and
+// to the q tile, in 32: the host refuses a q tile whose heads' line passes 2^31.
 template <int BN>
 struct Walk {
   const Params &p;
   const Tile *tiles;
   const long long *cum;
-  int left, done;        // of the share: what is ahead, what lies behind
+  long long left, done;  // of the share: what is ahead, what lies behind
   int rem, all;          // in q tile x: position and length, all heads
   int x;
   Tile t;
@@ -197,14 +196,14 @@ struct Walk {
   int h, j0, j1;
   bool opens;            // the (q tile, head) begins in this share
   // A whole one begins where the share would be after so many key tiles, for the same reason, and goes round.
-  int turn, seen;
-  int begin;             // where its (q tile, head) begins, relative to the share (may be negative)
-  __device__ __forceinline__ Walk(const Params &prm, const Tile *t_, const long long *c_) : p(prm), tiles(t_), cum(c_) {}
+  int turn;
+  unsigned seen;
+  long long begin;       // where its (q tile, head) begins, relative to the share (may be negative)
+  __host__ __device__ __forceinline__ Walk(const Params &prm, const Tile *t_, const long long *c_)
+      : p(prm), tiles(t_), cum(c_) {}
 
   // Finds the q tile at u0 (whole warp; u0 < length).
   __device__ __forceinline__ void seek(long long u0, long long u1, int ntiles) {
-    left = int(u1 - u0);
-    done = seen = 0;
     int lo = 0, n = ntiles;  // x is in [lo, lo + n): cum[lo] * Hkv <= u0
     const int lane = threadIdx.x & 31;
     while (n > 1) {
@@ -216,19 +215,26 @@ struct Walk {
       lo += off;
       n = min(step, n - off);
     }
-    x = lo;
+    start(u0, u1, lo);
+  }
+  // u0 lies in q tile at.
+  __host__ __device__ __forceinline__ void start(long long u0, long long u1, int at) {
+    left = u1 - u0;
+    done = 0;
+    seen = 0;
+    x = at;
     rem = int(u0 - cum[x] * p.Hkv);
     load();
   }
-  __device__ __forceinline__ void load() {
+  __host__ __device__ __forceinline__ void load() {
     t = tiles[FFTS_INDEX(x, p.max_tiles)];
     g = keys_of<BN>(t.pos0, t.ntok, p.window, p.sinks);
     all = (g.n + p.overhead) * p.Hkv;
   }
   // The key tile at step j of [j0, j1).
-  __device__ __forceinline__ int key(int j) const { return key_tile(g, j + turn < j1 ? j + turn : j + turn - g.n); }
+  __host__ __device__ __forceinline__ int key(int j) const { return key_tile(g, j + turn < j1 ? j + turn : j + turn - g.n); }
   // The next segment with key tiles; false behind the share's end.
-  __device__ __forceinline__ bool segment() {
+  __host__ __device__ __forceinline__ bool segment() {
     while (left > 0) {
       if (rem >= all) {
         rem = 0;
@@ -238,7 +244,7 @@ struct Walk {
       const int len = g.n + p.overhead;
       h = rem / len;
       const int at = rem - h * len;
-      const int to = min(len, at + left);
+      const int to = int(min((long long)len, at + left));
       begin = done - at;
       rem += to - at;
       done += to - at;
@@ -248,11 +254,15 @@ struct Walk {
       opens = o0 == 0;
       j0 = g.n - o1;
       j1 = g.n - o0;
-      turn = j1 - j0 == g.n ? seen % g.n : 0;
-      seen += j1 - j0;
+      turn = j1 - j0 == g.n ? int(seen % unsigned(g.n)) : 0;
+      seen += unsigned(j1 - j0);
       return true;
     }
     return false;
+  }
+  // The share that ends the segment's (q tile, head), from where this one begins and the length of all.
+  __host__ __device__ __forceinline__ int last_share(long long u0, long long per) const {
+    return int((u0 + begin + p.overhead + g.n - 1) / per);
   }
 };
 

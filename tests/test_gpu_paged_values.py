@@ -205,3 +205,42 @@ def test_page_numbers_outside_every_pool_give_no_slot(page):
             at = (x, x, 3)[pos // page]
             want.append(at * page + pos % page if 0 <= at < most else -1)
     assert p.slot_map.tolist() == want
+
+
+# ------------------------------------------------------------------ schedules
+def schedule_bound(lens, G):
+    """The q tiles that a call makes room for; up to 1024 of them every CTA builds the schedule itself."""
+    T = sum(n for _, n in lens)
+    return T // (128 // G) + min(len(lens), T)
+
+
+@pytest.mark.parametrize("R,G,bound", [(193, 8, 205), (400, 4, 412), (964, 8, 1024), (965, 8, 1025), (512, 128, 1024)])
+def test_schedules_of_many_requests(R, G, bound):
+    """More requests than a CTA scans at a time (192), up to the last size whose schedule it builds itself and the next."""
+    lens = [(i * 37 % 131, 1) for i in range(R)]
+    assert schedule_bound(lens, G) == bound
+    b = Batch(lens, G, 1, 64, BF, 16)
+    b.check(b.run())
+    F.check_status()
+
+
+@pytest.mark.parametrize("lens,G,bound", [
+    ([(7, 460)], 64, 231), ([(7, 1900), (0, 1), (300, 90)], 64, 998),
+    ([(i * 11 % 90, i % 3) for i in range(450)], 64, 675)])
+def test_schedules_of_many_q_tiles(lens, G, bound):
+    """More q tiles than the threads that scan them, and idle requests among them."""
+    assert schedule_bound(lens, G) == bound
+    b = Batch(lens, G, 1, 64, BF, 16)
+    b.check(b.run())
+
+
+@pytest.mark.parametrize("lens,G,bound", [
+    ([(7, 1700)], 64, 851), ([(7, 1700), (90, 30), (0, 64)], 64, 900), ([(0, 2046)], 64, 1024), ([(5, 2048)], 64, 1025),
+    ([(i % 90, 8) for i in range(113)], 128, 1017)])
+def test_schedules_of_the_larger_tiles(lens, G, bound):
+    """Tiles of 256 rows: more of them than the 384 that a CTA scans at a time."""
+    T = sum(n for _, n in lens)
+    assert schedule_bound(lens, G) == bound and T * G >= 1024 * len(lens)
+    b = Batch(lens, G, 1, 64, BF, 16, width=20000)
+    b.check(b.run())
+    F.check_status()

@@ -76,7 +76,9 @@ struct Layout {
   static constexpr int nbars = 2 + 2 * kKStages + kVStages + 2 + 2 + 2 + 1;
   static constexpr int tmem_slot = bars + nbars * 8;
   static constexpr int abort = tmem_slot + 8;
-  static constexpr int bytes = abort + 8;
+  static constexpr int odd = (abort + 8 + 15) / 16 * 16;  // OddTile [2]
+  static constexpr int noted = odd + 32;                   // the segment of the rows' notes, counted from 1
+  static constexpr int bytes = noted + 8;
   static_assert(2 * (bytes + 1024) <= 228 * 1024, "two CTAs must fit in an SM's shared memory");
 };
 
@@ -90,6 +92,75 @@ constexpr int BSF = BVF + kVStages;     // S(n) in buffer n % 2 [2]
 constexpr int BPV = BSF + 2;            // PV(n) complete, frees V stage n % 2 [2]
 constexpr int BPF = BPV + 2;            // P(n) written (128 arrivals) [2]
 constexpr int BDRAIN = BPF + 2;
+
+// A V tile with elements that are not finite, where rows differ in what they see of it: the softmax threads that find
+// some say so before they hand P over, and the MMA issuer sees to them before it uses the tile.  Looking costs ragged
+// chunks 77 -> 81 us (as many for a meeting of the softmax warps on top: 85; looked through by the producer 95; by a
+// warp of its own, with fewer registers for each, 82, and decoding 165 -> 172).
+struct __align__(16) OddTile {
+  int seg, pos0, ntok, c0;  // segment, counted from 1; 0: none
+};
+
+// Whether the thread's part of a V tile (key, one half) has such elements.
+template <typename E>
+__device__ __noinline__ bool has_odd(const uint8_t *row) {
+  uint32_t acc[4] = {0, 0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {  // in another order in each lane: no bank conflicts
+    const uint4 w = *reinterpret_cast<const uint4 *>(row + (((i ^ threadIdx.x) & 7) << 4));
+    Num<E>::probe(w.x, acc[0]);
+    Num<E>::probe(w.y, acc[1]);
+    Num<E>::probe(w.z, acc[2]);
+    Num<E>::probe(w.w, acc[3]);
+  }
+  return ((acc[0] | acc[1] | acc[2] | acc[3]) & 0x7fff7fffu) != 0;
+}
+
+// Notes the elements for the rows that see them and zeroes them (one thread; the rows of earlier segments have put
+// theirs back when P of this one is there).
+template <typename E, int D>
+__device__ __noinline__ void note_odd(const Params &p, uint8_t *v, const OddTile &o, volatile int *notes_seg) {
+  constexpr uint32_t top = Num<E>::exponent;
+  uint32_t *notes = p.notes + int64_t(blockIdx.x) * p.rows * 8;
+  const bool again = *notes_seg == o.seg;
+  for (int ch = 0; ch < 4; ++ch) {  // 32 channels
+    uint32_t up[kBN], down[kBN];
+    for (int key = 0; key < kBN; ++key) {
+      up[key] = down[key] = 0;
+      for (int i = 0; ch < D / 32 && i < 16; ++i) {
+        uint32_t *at = reinterpret_cast<uint32_t *>(v + ((ch >> 1) * kBN + key) * 128 + (((ch & 1) * 64 + i * 4) ^ ((key & 7) << 4)));
+        uint32_t w = *at;
+        for (int e = 0; e < 2; ++e) {
+          const uint32_t x = (w >> (16 * e)) & 0xffffu;
+          if ((x & top) != top) continue;
+          const bool nan = (x & 0x7fffu) != top;
+          up[key] |= uint32_t(nan || !(x & 0x8000u)) << (2 * i + e);
+          down[key] |= uint32_t(nan || (x & 0x8000u)) << (2 * i + e);
+          w &= ~(0xffffu << (16 * e));
+        }
+        *at = w;
+      }
+    }
+    for (int t = 0; t < o.ntok; ++t) {
+      const int pos = o.pos0 + t;
+      uint32_t u = 0, d = 0;
+      for (int key = 0; key < kBN; ++key) {
+        const int c = o.c0 + key;
+        if (c > pos || (p.window > 0 && c <= pos - p.window && c >= p.sinks)) continue;
+        u |= up[key];
+        d |= down[key];
+      }
+      for (int row = t * p.G; row < (t + 1) * p.G; ++row) {
+        if (!FFTS_IN_RANGE(row, p.rows)) continue;
+        notes[row * 8 + ch] = again ? notes[row * 8 + ch] | u : u;
+        notes[row * 8 + 4 + ch] = again ? notes[row * 8 + 4 + ch] | d : d;
+      }
+    }
+  }
+  *notes_seg = o.seg;
+  __threadfence_block();
+  fence_proxy_async();
+}
 
 template <typename E, int D>
 __global__ void __launch_bounds__(kThreads, 2)
@@ -109,12 +180,14 @@ __global__ void __launch_bounds__(kThreads, 2)
   const uint32_t sbase = smem_u32(smem);
   auto bar = [&](int i) { return sbase + Lay::bars + 8u * uint32_t(i); };
   volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + Lay::abort);
+  volatile OddTile *odd = reinterpret_cast<volatile OddTile *>(smem + Lay::odd);
+  volatile int *notes_seg = reinterpret_cast<volatile int *>(smem + Lay::noted);
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + Lay::tmem_slot);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int qrows = p.tpt * p.G;  // rows a Q load fills
 
   if (threadIdx.x == 0) {
-    *abort_flag = 0;
+    *abort_flag = *notes_seg = odd[0].seg = odd[1].seg = 0;
     for (int i = 0; i < Lay::nbars; ++i) mbar_init(bar(i), (i == BPF || i == BPF + 1) ? 128u : 1u);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -323,6 +396,11 @@ __global__ void __launch_bounds__(kThreads, 2)
              mbar_wait(bar(BPF + b), (n >> 1) & 1, abort_flag, p.wait_cycles);
         if (!ok) break;
         fence_after();
+        if (odd[b].seg) {
+          const OddTile o{odd[b].seg, odd[b].pos0, odd[b].ntok, odd[b].c0};
+          odd[b].seg = 0;
+          note_odd<E, D>(p, smem + Lay::v + b * Lay::kv_bytes, o, notes_seg);
+        }
         const bool first = (firsts >> (n & 31)) & 1u;
         const uint32_t dv = dv0 + ((b * Lay::kv_bytes) >> 4);
         const uint32_t pt = tmem + b * kBN;  // P(n): pairs in the first 32 columns of S buffer n % 2
@@ -349,7 +427,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     const float2 sc2 = make_float2(p.scale_log2, p.scale_log2);
     bool ok = true, first_seg = true, noted = false;
     int n = 0;
-    while (ok && w.segment()) {
+    for (int seg = 1; ok && w.segment(); ++seg) {
       const Keys g = w.g;
       const int nrows = w.t.ntok * p.G;
       const bool active = warp * 32 < nrows, live = r < nrows;
@@ -357,15 +435,15 @@ __global__ void __launch_bounds__(kThreads, 2)
       const int pos = w.t.pos0 + min(tl, w.t.ntok - 1);
       // and their P is 0, by an offset of -inf
       float m_ref = live ? -INFINITY : 0.0f, l_run = 0.0f;
-      for (int j = w.j0, stop; ok && j < w.j1;) {
-        stop = min(w.j1, j + kSum);
+      for (int j = w.j0, stop = j; ok && j < w.j1;) {
+        if (j == stop) stop = min(w.j1, j + kSum);
         for (; j < stop; ++j, ++n) {
           const int b = n & 1;
           const uint32_t parity = (n >> 1) & 1;
           if (!__all_sync(0xffffffffu, mbar_wait(bar(BSF + b), parity, abort_flag, p.wait_cycles))) { ok = false; break; }
           fence_after();
           const int c0 = w.key(j) * kBN;
-          if (c0 + kBN > g.hi || (c0 < g.lo && c0 + kBN > p.sinks)) {
+          if (has_unseen<kBN>(g, p.sinks, c0)) {
             // V rows that no row sees
             if (!__all_sync(0xffffffffu, mbar_wait(bar(BVF + b), parity, abort_flag, p.wait_cycles))) { ok = false; break; }
             const int key = c0 + (r & 63);
@@ -474,10 +552,27 @@ __global__ void __launch_bounds__(kThreads, 2)
               tmem_wait_st();
             }
           }
+          if (rows_differ<kBN>(w.t.pos0, w.t.ntok, p.window, p.sinks, c0)) break;
           fence_before();
           mbar_arrive(bar(BPF + b));
         }
-        if (ok && j < w.j1) {
+        if (ok && j < stop) {  // the same for a tile that rows differ in; outside of the loop, which has no registers to give
+          const int b = n & 1, key = w.key(j) * kBN + (r & 63);
+          ok = __all_sync(0xffffffffu, mbar_wait(bar(BVF + b), (n >> 1) & 1, abort_flag, p.wait_cycles));
+          if (!ok) break;
+          if (r < 64 * Lay::halves && key < g.hi && (key >= g.lo || key < p.sinks) &&
+              has_odd<E>(smem + Lay::v + b * Lay::kv_bytes + (r >> 6) * Lay::kv_half + (r & 63) * 128)) {
+            odd[b].pos0 = w.t.pos0;
+            odd[b].ntok = w.t.ntok;
+            odd[b].c0 = w.key(j) * kBN;
+            odd[b].seg = seg;
+          }
+          fence_before();
+          mbar_arrive(bar(BPF + b));
+          ++j;
+          ++n;
+        }
+        if (ok && j == stop && j < w.j1) {
           // PV(n - 1), whose barrier's next phase needs P(n + 1)
           ok = __all_sync(0xffffffffu, mbar_wait(bar(BPV + (n - 1) % 2), ((n - 1) >> 1) & 1, abort_flag, p.wait_cycles));
           if (!ok) break;
@@ -525,6 +620,10 @@ __global__ void __launch_bounds__(kThreads, 2)
           if (live && !whole && FFTS_IN_RANGE(slot, 2 * p.ctas)) park<kBM>(o, pd, c);
         }
         if (live && !whole && FFTS_IN_RANGE(slot, 2 * p.ctas)) *pml = make_float2(m_ref * p.scale_log2, l_run);
+        if (live && *notes_seg == seg) {
+          if (whole && FFTS_IN_RANGE(w.t.tok0 + tl, p.T)) put_back<E, D, kBM>(p, r, reinterpret_cast<E *>(dst));
+          if (!whole && FFTS_IN_RANGE(slot, 2 * p.ctas)) put_back<E, D, kBM>(p, r, reinterpret_cast<float *>(pd));
+        }
       }
       // the share that opens a (q tile, head) and does not end it leaves a note for the join
       if (w.opens && w.j1 - w.j0 < g.n && r == 0 && FFTS_IN_RANGE(blockIdx.x, p.ctas)) {
@@ -709,9 +808,9 @@ static int encode(CUtensorMap *map, CUtensorMapDataType type, int rank, const vo
 
 __device__ int g_status_sink;
 
-// Workspace: cum, tiles, header, cuts, partial (m, l), partial O; every part a multiple of 16 bytes.
+// Workspace: cum, tiles, header, cuts, notes, partial (m, l), partial O; every part a multiple of 16 bytes.
 struct Space {
-  int64_t max_tiles, cum, tiles, header, cuts, ml, part, bytes;
+  int64_t max_tiles, cum, tiles, header, cuts, notes, ml, part, bytes;
   Space(int64_t T, int64_t R, int64_t G, int64_t D) {
     const int64_t tpt = kBM / G;  // of the smaller tiles; the larger ones are fewer
     max_tiles = T / tpt + std::min(R, T);  // sum of ceil(len / tpt)
@@ -720,7 +819,8 @@ struct Space {
     tiles = cum + (copies * (max_tiles + 1) + 1) / 2 * 16;
     header = tiles + copies * max_tiles * 16;
     cuts = header + 16;
-    ml = cuts + kMaxCtas * int64_t(sizeof(Cut));
+    notes = cuts + kMaxCtas * int64_t(sizeof(Cut));
+    ml = notes + int64_t(kMaxCtas) * kBM * 32;
     part = ml + int64_t(2 * kMaxCtas) * kBM * 8;
     bytes = part + int64_t(2 * kMaxCtas) * kBM * D * 4;
   }
@@ -830,6 +930,7 @@ int paged_attn(const ffts_paged_attn_args &a, cudaStream_t stream) {
   p.tiles = reinterpret_cast<Tile *>(base + sp.tiles);
   p.header = reinterpret_cast<int *>(base + sp.header);
   p.cuts = reinterpret_cast<Cut *>(base + sp.cuts);
+  p.notes = reinterpret_cast<uint32_t *>(base + sp.notes);
   p.part_ml = reinterpret_cast<float2 *>(base + sp.ml);
   p.part = reinterpret_cast<float *>(base + sp.part);
   int sms = 0;

@@ -11,7 +11,8 @@
 // Roles (384 threads; registers are split for the softmax warps, which hold a row's 128 scores):
 //   warps 0-3 / 4-7  softmax of half A / B: thread r owns row r; P goes over the S columns already read.
 //   warp 8           producer: Q of each half, then K(0), V(0), K(1), ... through one five-stage ring.
-//   warps 10, 11     none (registers are split by warpgroup)
+//   warp 10          keeper of V tiles with keys that not all rows see (paged_common.cuh).
+//   warp 11          none (registers are split by warpgroup)
 //   warp 9           MMA issuer (one thread): S_A, S_B, then per key tile n: PV_A(n), S_A(n + 1), PV_B(n), S_B(n + 1).
 //                    The product of a half's first 64 keys starts while the exponentials of the others are computed.
 // A commit tracks all earlier products of the issuing thread, so S_X(n + 1) being there means that PV_X(n) is
@@ -33,7 +34,7 @@ namespace paged {
 constexpr int cBM = 128;       // rows of a half
 constexpr int cBN = 128;       // keys of a key tile
 constexpr int cThreads = 384;   // three warpgroups
-constexpr int cRegsSoftmax = 208, cRegsOther = 80;  // after the split; launched with 168 each, 2 * 208 + 80 <= 3 * 168
+constexpr int cRegsSoftmax = 200, cRegsOther = 104;  // after the split; launched with 168 each, 2 * 200 + 104 <= 3 * 168
 constexpr int cStages = 5;
 constexpr int cTmemCols = 512;
 
@@ -45,21 +46,92 @@ struct ChunkLayout {
   static constexpr int q = 0;
   static constexpr int kv = q + 2 * tile;
   static constexpr int bars = kv + cStages * tile;
-  static constexpr int nbars = 2 * cStages + 2 + 2 + 2 + 4 + 2 + 1;
+  static constexpr int nbars = 3 * cStages + 2 + 2 + 2 + 4 + 2 + 1;
   static constexpr int tmem_slot = bars + nbars * 8;
   static constexpr int abort = tmem_slot + 8;
-  static constexpr int bytes = abort + 8;
+  static constexpr int notes = abort + 8;
+  static constexpr int bytes = notes + 40;
   static_assert(bytes <= 227 * 1024, "one CTA must fit in an SM's shared memory");
 };
 
 constexpr int CKF = 0;              // ring stage loaded [cStages]
 constexpr int CKE = CKF + cStages;  // ring stage free   [cStages]
-constexpr int CQF = CKE + cStages;  // Q of half x loaded
+constexpr int CVX = CKE + cStages;  // ring stage loaded with V, for the keeper [cStages]
+constexpr int CQF = CVX + cStages;  // Q of half x loaded
 constexpr int CQE = CQF + 2;        // the segment's S products have read it
 constexpr int CSF = CQE + 2;        // S of half x
 constexpr int CPF = CSF + 2;        // P of half x written for the first and last 64 keys (128 arrivals) [2 x + part]
 constexpr int COF = CPF + 4;        // O of half x final
 constexpr int CDRAIN = COF + 2;
+
+// The keeper.  V tiles with keys that not all rows see pass through its hands before the MMA issuer gets them: their copies
+// complete a barrier of the keeper's, and its arrival the one that the issuer waits for.
+struct Notes {
+  volatile int *segment;  // the segment of the notes, counted from 1
+  volatile int *done;     // segments that each softmax warp has finished (one without rows runs ahead of the others)
+  int warps;
+};
+
+// The keys of a V tile in shared memory (BN rows of 128 bytes for each 64 channels, swizzled), from c0 on (whole warp).
+// False: the wait for the softmax ran out.
+template <typename E, int D, int BN>
+__device__ __forceinline__ bool keep_values(const Params &p, uint8_t *v, const Tile &t, const Keys &g, int c0, int seg,
+                                            const Notes &notes, volatile int *abort_flag) {
+  constexpr uint32_t top = Num<E>::exponent;
+  const int lane = threadIdx.x & 31;
+  if (has_unseen<BN>(g, p.sinks, c0)) {
+#pragma unroll 4
+    for (int i = lane; i < BN * D / 8; i += 32) {
+      const int c = c0 + (i >> 3) % BN;
+      if (c >= g.hi || (c < g.lo && c >= p.sinks)) *reinterpret_cast<uint4 *>(v + i * 16) = make_uint4(0, 0, 0, 0);
+    }
+    __syncwarp();
+  }
+  if (rows_differ<BN>(t.pos0, t.ntok, p.window, p.sinks, c0)) {
+    uint32_t acc[4] = {0, 0, 0, 0};
+#pragma unroll 8
+    for (int i = lane; i < BN * D / 8; i += 32) {
+      const uint4 w = *reinterpret_cast<const uint4 *>(v + i * 16);
+      Num<E>::probe(w.x, acc[0]);
+      Num<E>::probe(w.y, acc[1]);
+      Num<E>::probe(w.z, acc[2]);
+      Num<E>::probe(w.w, acc[3]);
+    }
+    if (__any_sync(0xffffffffu, ((acc[0] | acc[1] | acc[2] | acc[3]) & 0x7fff7fffu) != 0)) {
+      const int nrows = min(t.ntok * p.G, p.rows);
+      uint32_t *at = p.notes + int64_t(blockIdx.x) * p.rows * 8;
+      if (*notes.segment != seg + 1) {  // the segments before may still need theirs
+        const long long t0 = clock64();
+        while (__any_sync(0xffffffffu, lane < notes.warps && notes.done[lane] < seg))
+          if (__any_sync(0xffffffffu, *abort_flag || clock64() - t0 > p.wait_cycles)) return false;
+        for (int i = lane; i < nrows * 8; i += 32) at[i] = 0;
+        __syncwarp();
+        *notes.segment = seg + 1;
+      }
+#pragma unroll 1
+      for (int i = 0; i < BN * (D / 32); ++i) {
+        const int key = i % BN, c = c0 + key, ch = i / BN;  // channel 32 ch + lane
+        uint16_t *el = reinterpret_cast<uint16_t *>(v + ((ch >> 1) * BN + key) * 128 + (((ch & 1) * 64 + lane * 2) ^ ((key & 7) << 4)));
+        const uint32_t x = *el;
+        const bool odd = (x & top) == top, nan = odd && (x & 0x7fffu) != top;
+        const uint32_t up = __ballot_sync(0xffffffffu, nan || (odd && !(x & 0x8000u)));
+        const uint32_t down = __ballot_sync(0xffffffffu, nan || (odd && (x & 0x8000u)));
+        if (!(up | down)) continue;
+        if (odd) *el = 0;
+        for (int row = lane; row < nrows; row += 32) {
+          const int pos = t.pos0 + row / p.G;
+          if (c > pos || (p.window > 0 && c <= pos - p.window && c >= p.sinks)) continue;
+          at[row * 8 + ch] |= up;
+          at[row * 8 + 4 + ch] |= down;
+        }
+      }
+      __threadfence_block();
+    }
+  }
+  fence_proxy_async();
+  __syncwarp();
+  return true;
+}
 
 template <typename E, int D>
 __global__ void __launch_bounds__(cThreads, 1)
@@ -79,6 +151,8 @@ __global__ void __launch_bounds__(cThreads, 1)
   const uint32_t sbase = smem_u32(smem);
   auto bar = [&](int i) { return sbase + Lay::bars + 8u * uint32_t(i); };
   volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + Lay::abort);
+  volatile int *words = reinterpret_cast<volatile int *>(smem + Lay::notes);
+  const Notes notes{words, words + 1, 8};
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + Lay::tmem_slot);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int tph = cBM / p.G;        // tokens of a half
@@ -86,6 +160,7 @@ __global__ void __launch_bounds__(cThreads, 1)
 
   if (threadIdx.x == 0) {
     *abort_flag = 0;
+    for (int i = 0; i < 1 + notes.warps; ++i) words[i] = 0;
     for (int i = 0; i < Lay::nbars; ++i) mbar_init(bar(i), (i >= CPF && i < CPF + 4) ? 128u : 1u);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -145,8 +220,10 @@ __global__ void __launch_bounds__(cThreads, 1)
       const int boxes = (cBN / box) * Lay::halves;
       const int my_box = lane / Lay::halves, my_half = lane % Lay::halves;
       const uint32_t my_dst = uint32_t(my_half * Lay::box + my_box * box * 128);
+      // kept: its V goes to the keeper
       struct Load {
         int page, row, h;
+        bool kept;
       };
       int j = 0, j1 = 0;
       bool fresh = false;  // the fetched tile is its segment's first
@@ -157,8 +234,9 @@ __global__ void __launch_bounds__(cThreads, 1)
           j = w.j0;
           j1 = w.j1;
         }
-        const int c = w.key(j) * cBN + my_box * box;  // first key of the box
+        const int c0 = w.key(j) * cBN, c = c0 + my_box * box;  // first key of the tile, of the box
         ++j;
+        l.kept = has_unseen<cBN>(w.g, p.sinks, c0) || rows_differ<cBN>(w.t.pos0, w.t.ntok, p.window, p.sinks, c0);
         l.page = -1;
         l.row = c & (ps - 1);
         l.h = w.h;
@@ -168,14 +246,17 @@ __global__ void __launch_bounds__(cThreads, 1)
       };
       bool ok = true;
       int nl = 0, nq[2] = {0, 0};  // loads issued
-      auto load = [&](const Load &l, const CUtensorMap *map) {
+      uint32_t kept = 0, odd = 0;  // load n is one for the keeper: bit n % 32; their number in each stage, modulo 2
+      auto load = [&](const Load &l, const CUtensorMap *map, bool for_keeper) {
         const int s = nl % cStages;
         ok = ok && __all_sync(0xffffffffu, mbar_wait(bar(CKE + s), ((nl / cStages) & 1) ^ 1, abort_flag, p.wait_cycles));
         if (!ok) return;
-        if (lane == 0) mbar_arrive_tx(bar(CKF + s), Lay::tile);
+        const uint32_t full = bar((for_keeper ? CVX : CKF) + s);
+        if (lane == 0) mbar_arrive_tx(full, Lay::tile);
         __syncwarp();
-        if (lane < boxes)
-          tma_load_4d(sbase + Lay::kv + s * Lay::tile + my_dst, map, bar(CKF + s), my_half * 64, l.row, l.h, l.page);
+        if (lane < boxes) tma_load_4d(sbase + Lay::kv + s * Lay::tile + my_dst, map, full, my_half * 64, l.row, l.h, l.page);
+        kept = (kept & ~(1u << (nl & 31))) | (uint32_t(for_keeper) << (nl & 31));
+        odd ^= uint32_t(for_keeper) << s;
         ++nl;
       };
       auto load_q = [&](int x, int tok0, int qh) {
@@ -195,14 +276,14 @@ __global__ void __launch_bounds__(cThreads, 1)
         // whose K and V are all on their way by then.
         const int tok0 = w.t.tok0, qh = w.h * p.G;
         const bool first = fresh, two = w.t.ntok > tph;
-        load(cur, &tm_k);
+        load(cur, &tm_k, false);
         if (first) {
           load_q(0, tok0, qh);
           if (two) load_q(1, tok0, qh);
         }
         Load next = cur;
         more = fetch(next);  // its page numbers arrive while the stages fill
-        load(cur, &tm_v);
+        load(cur, &tm_v, cur.kept);
         cur = next;
       }
       if (!ok) {
@@ -213,8 +294,11 @@ __global__ void __launch_bounds__(cThreads, 1)
           volatile int never = 0;
           for (int x = 0; x < 2; ++x)
             if (nq[x] > 0) mbar_wait(bar(CQF + x), (nq[x] - 1) & 1, &never, p.drain_cycles);
-          for (int n = max(0, nl - cStages); n < nl; ++n)
-            mbar_wait(bar(CKF + n % cStages), (n / cStages) & 1, &never, p.drain_cycles);
+          for (int n = max(0, nl - cStages); n < nl; ++n) {
+            const int s = n % cStages;
+            if ((kept >> (n & 31)) & 1u) mbar_wait(bar(CVX + s), ((odd >> s) & 1u) ^ 1, &never, p.drain_cycles);
+            else mbar_wait(bar(CKF + s), (n / cStages) & 1, &never, p.drain_cycles);
+          }
         }
         __syncwarp();
       }
@@ -307,6 +391,25 @@ __global__ void __launch_bounds__(cThreads, 1)
         volatile int never = 0;
         mbar_wait(bar(CDRAIN), 0, &never, p.drain_cycles);
       }
+    } else if (warp == 10) {
+      // ============================================================ keeper (whole warp)
+      bool ok = true;
+      int n = 0;         // V tiles
+      uint32_t odd = 0;  // tiles kept in each stage, modulo 2
+      for (int seg = 0; ok && w.segment(); ++seg) {
+        for (int j = w.j0; ok && j < w.j1; ++j, ++n) {
+          const int c0 = w.key(j) * cBN, s = (2 * n + 1) % cStages;
+          if (!has_unseen<cBN>(w.g, p.sinks, c0) && !rows_differ<cBN>(w.t.pos0, w.t.ntok, p.window, p.sinks, c0)) continue;
+          ok = __all_sync(0xffffffffu, mbar_wait(bar(CVX + s), (odd >> s) & 1u, abort_flag, p.wait_cycles));
+          odd ^= 1u << s;
+          ok = ok && keep_values<E, D, cBN>(p, smem + Lay::kv + s * Lay::tile, w.t, w.g, c0, seg, notes, abort_flag);
+          if (ok && lane == 0) mbar_arrive(bar(CKF + s));
+        }
+      }
+      if (!ok && lane == 0) {
+        *abort_flag = 1;
+        *reinterpret_cast<volatile int *>(p.status) = kErrProducer;
+      }
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(cRegsSoftmax));
@@ -319,8 +422,8 @@ __global__ void __launch_bounds__(cThreads, 1)
     const uint32_t s_addr = tmem + x * cBN + lane_off, o_addr = tmem + 256 + x * 128 + lane_off;
     const float2 sc2 = make_float2(p.scale_log2, p.scale_log2);
     bool ok = true, first_seg = true, noted = false;
-    int n = 0, nseg = 0, kvn = 0;  // S tiles and segments of this half, key tiles of the share so far
-    while (ok && w.segment()) {
+    int n = 0, nseg = 0;  // S tiles and segments of this half
+    for (int seg = 0; ok && w.segment(); ++seg) {
       const Keys g = w.g;
       const int nrows = w.t.ntok * p.G;
       const bool mine = w.t.ntok > x * tph;                      // this half has rows
@@ -328,27 +431,12 @@ __global__ void __launch_bounds__(cThreads, 1)
       // rows of no token take the last token's mask; nobody reads them
       const int pos = w.t.pos0 + min(tl, w.t.ntok - 1);
       float m_ref = -INFINITY, l_run = 0.0f;
-      if (!mine) kvn += w.j1 - w.j0;
       for (int j = w.j0, stop; mine && ok && j < w.j1;) {
         stop = min(w.j1, j + kSum);
-        for (; j < stop; ++j, ++n, ++kvn) {
+        for (; j < stop; ++j, ++n) {
           if (!__all_sync(0xffffffffu, mbar_wait(bar(CSF + x), n & 1, abort_flag, p.wait_cycles))) { ok = false; break; }
           fence_after();
           const int c0 = w.key(j) * cBN;
-          if (x == 0 && (c0 + cBN > g.hi || (c0 < g.lo && c0 + cBN > p.sinks))) {
-            // V rows that no row sees, for both halves (A's product is issued before B's)
-            const int v = 2 * kvn + 1, stage = v % cStages;
-            if (!__all_sync(0xffffffffu, mbar_wait(bar(CKF + stage), (v / cStages) & 1, abort_flag, p.wait_cycles))) { ok = false; break; }
-            const int key = c0 + r;
-            if (key >= g.hi || (key < g.lo && key >= p.sinks)) {
-#pragma unroll
-              for (int hf = 0; hf < Lay::halves; ++hf)
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                  *reinterpret_cast<uint4 *>(smem + Lay::kv + stage * Lay::tile + hf * Lay::box + r * 128 + i * 16) = make_uint4(0, 0, 0, 0);
-            }
-            fence_proxy_async();
-          }
           if (active) {
             // whole: the row sees all keys of the tile
             const int lim = pos + 1 - c0, from = p.window > 0 ? pos - p.window + 1 - c0 : 0, sink = p.sinks - c0;
@@ -472,7 +560,13 @@ __global__ void __launch_bounds__(cThreads, 1)
           if (live && !whole && FFTS_IN_RANGE(slot, 2 * p.ctas)) park<(2 * cBM)>(o, pd, c);
         }
         if (live && !whole && FFTS_IN_RANGE(slot, 2 * p.ctas)) *pml = make_float2(m_ref * p.scale_log2, l_run);
+        if (live && *notes.segment == seg + 1) {
+          if (whole && FFTS_IN_RANGE(w.t.tok0 + tl, p.T)) put_back<E, D, 2 * cBM>(p, row, reinterpret_cast<E *>(dst));
+          if (!whole && FFTS_IN_RANGE(slot, 2 * p.ctas)) put_back<E, D, 2 * cBM>(p, row, reinterpret_cast<float *>(pd));
+        }
       }
+      __syncwarp();
+      if (lane == 0) notes.done[warp] = seg + 1;
       // the share that opens a (q tile, head) and does not end it leaves a note for the join
       if (w.opens && w.j1 - w.j0 < g.n && threadIdx.x == 0 && FFTS_IN_RANGE(blockIdx.x, p.ctas)) {
         Cut cut;

@@ -51,6 +51,7 @@ struct Params {
   Cut *cuts;                  // [ctas]: the (q tile, head) that share c begins and others go on with
   float *part;                // [2 * ctas][D / 4][rows] float4
   float2 *part_ml;            // [2 * ctas][rows]: m (log2 units) and l
+  uint32_t *notes;            // [ctas][rows][2][4]: channels of a row's o that are +inf, and -inf (NaN: both)
   int max_tiles, ctas;
   int rows;                   // of a q tile: 128 or 256
   int overhead;               // length of a (q tile, head) besides its key tiles
@@ -78,6 +79,17 @@ __host__ __device__ __forceinline__ Keys keys_of(int pos0, int ntok, int window,
 
 // The j-th of them.
 __host__ __device__ __forceinline__ int key_tile(const Keys &g, int j) { return j < g.st ? j : j - g.st + g.wt0; }
+
+// Whether some of the keys [c0, c0 + BN) are seen by no row of the q tile.
+template <int BN>
+__host__ __device__ __forceinline__ bool has_unseen(const Keys &g, int sinks, int c0) {
+  return c0 + BN > g.hi || (c0 < g.lo && c0 + BN > sinks);
+}
+// Whether the rows of a q tile may differ in what they see of them.
+template <int BN>
+__host__ __device__ __forceinline__ bool rows_differ(int pos0, int ntok, int window, int sinks, int c0) {
+  return ntok > 1 && (c0 + BN > pos0 + 1 || (window > 0 && c0 < pos0 + ntok - window && c0 + BN > sinks));
+}
 
 __host__ __device__ __forceinline__ long long share_of(const Params &p, long long length) {
   const long long per = (length + p.ctas - 1) / p.ctas;
@@ -283,6 +295,11 @@ struct Num<__nv_bfloat16> {
   // P <= 2^64 against the reference max: bf16 and the fp32 O have the exponents for it
   static constexpr float rescale = 64.0f, pmax = 18446744073709551616.0f, bias = 0.0f, chunk_rescale = 64.0f;
   static constexpr int sum_keys = 131072;
+  static constexpr uint32_t exponent = 0x7f80;
+  // 0 * each half of w added to acc: NaN once one of them is not finite
+  static __device__ __forceinline__ void probe(uint32_t w, uint32_t &acc) {
+    asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(acc) : "r"(w), "r"(0u));
+  }
   static __device__ __forceinline__ uint32_t pack(float a, float b) {
     const __nv_bfloat162 r = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const uint32_t *>(&r);
@@ -299,6 +316,10 @@ struct Num<__half> {
   // tiles look first, and rescale seldom (at 2^2.99: 2048 tokens over 32768 1112 -> 1150 us).
   static constexpr float rescale = 2.99f, pmax = 65504.0f, bias = 7.0f, chunk_rescale = 8.0f;
   static constexpr int sum_keys = 16384;
+  static constexpr uint32_t exponent = 0x7c00;
+  static __device__ __forceinline__ void probe(uint32_t w, uint32_t &acc) {
+    asm("fma.rn.f16x2 %0, %1, %2, %0;" : "+r"(acc) : "r"(w), "r"(0u));
+  }
   static __device__ __forceinline__ uint32_t pack(float a, float b) {
     const __half2 r = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t *>(&r);
@@ -429,6 +450,30 @@ __device__ __noinline__ void park_o(const Params &p, int slot, int row, bool liv
     if (live) park<ROWS>(o, pd, c);
   }
   if (live) pml->x = m;
+}
+
+// ---------------------------------------------------------------- values that must not count
+// The tensor core multiplies all keys of a V tile, and a P of 0 does not make up for NaN or infinity.  Keys that no row
+// of the q tile sees are zeroed in shared memory (pages hold anything behind a request's last key).  In tiles that
+// rows differ in (the last ones of a q tile, and those at the ends of its window) elements that are not finite are noted for
+// the rows that see them, and zeroed; the rows' results get them back at the segment's end.
+//
+// A row's notes to its result, in the output or (float) in the partials, whose pieces of four channels lie ROWS pieces
+// apart.
+template <typename E, int D, int ROWS, typename T>
+__device__ __noinline__ void put_back(const Params &p, int row, T *o) {
+  if (!FFTS_IN_RANGE(row, p.rows)) return;
+  const uint32_t *at = p.notes + (int64_t(blockIdx.x) * p.rows + row) * 8;
+#pragma unroll 1
+  for (int c = 0; c < D; ++c) {
+    const bool up = (at[c >> 5] >> (c & 31)) & 1u, down = (at[4 + (c >> 5)] >> (c & 31)) & 1u;
+    if (!up && !down) continue;
+    const float x = (up ? INFINITY : 0.0f) - (down ? INFINITY : 0.0f);  // both: NaN
+    if constexpr (std::is_same<T, float>::value)
+      o[(c >> 2) * ROWS * 4 + (c & 3)] += x;
+    else
+      o[c] = E(float(o[c]) + x);
+  }
 }
 
 // The kernel of paged_chunk.cu: p with tiles of 256 rows, K and V maps with boxes of up to 128 keys.

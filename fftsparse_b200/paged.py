@@ -321,7 +321,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     With ``window`` W a token at position p sees the keys p - W + 1 .. p and the first ``sinks`` keys of its
     request (the work does not grow with the rest); pages it does not see may be gone from the table.  Tokens that see
     nothing (kv_len 0) get zeros; a NaN or infinite score among the keys that a token sees makes its row NaN, as the
-    softmax does (a score of -inf has no weight).  Returns [T, H, D] (or fills ``out``); rows of no request are not written.
+    softmax does (a score of -inf has no weight), and a v that is not finite reaches its channels of the tokens that see
+    its key, no others.  Returns [T, H, D] (or fills ``out``); rows of no request are not written.
 
     A bounded wait that runs out in the kernel raises WaitTimeout at a later call or at ``check_status()``.  Before a
     capture into a CUDA graph make one call outside of it (it sets up the device's status word).

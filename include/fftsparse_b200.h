@@ -276,7 +276,8 @@ FFTS_API int32_t ffts_rope_append(const ffts_rope_append_args *args, void *strea
  *   A token at position p sees key c iff c <= p and (window == 0, or c > p - window,
  *   or c < sinks).  Tokens that see nothing get zeros.  window 0: no window.
  *   Scores that are not finite do as in the formula: NaN, +inf or nothing but -inf
- *   among a token's keys gives NaN.
+ *   among a token's keys gives NaN.  Elements of v that are not finite reach their
+ *   channel of the tokens that see their key, and no others.
  *   workspace: ffts_paged_workspace_bytes(T, R, H, Hkv, D) bytes, 16-byte aligned,
  *     used by one call at a time.
  *   status: NULL or an int32 word the device can write; a bounded wait that runs

@@ -63,6 +63,55 @@ def test_broken_scores_reach_their_rows_and_no_others(last):
     F.check_status()
 
 
+# ------------------------------------------------------------------ values that are not finite
+@pytest.mark.parametrize("H,Hkv,D,dt,page", [(8, 2, 128, BF, 16), (4, 4, 64, FP, 64), (14, 2, 128, FP, 32), (3, 1, 64, BF, 256)])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (70, 0), (130, 5), (5000, 100)])
+@pytest.mark.parametrize("width", [0, 20000])
+def test_broken_values_reach_the_tokens_that_see_them_and_no_others(H, Hkv, D, dt, page, window, sinks, width):
+    """v with NaN and infinities in some channels of some keys: a channel is not finite in the rows that see such a key,
+    and as it should be in all others, the tokens before it and those whose window has left it behind."""
+    lens = [(0, 300), (37, 1), (700, 2200 if width else 150), (63, 70), (0, 0), (5, 4)]
+    b = Batch(lens, H, Hkv, D, dt, page, window=window, sinks=sinks, width=width)
+    g = torch.Generator().manual_seed(D + page)
+    for r, (c, n) in enumerate(lens):
+        length = c + n
+        for key in [] if length < 4 else [length - 1, length - 3, c + n // 2, c + n // 3, max(0, c - 60), 0, 3]:
+            h, ch = int(torch.randint(Hkv, (1,), generator=g)), torch.randperm(D, generator=g)[:5]
+            b.v[r][h, key, ch] = torch.tensor([NAN, math.inf, -math.inf, -NAN, math.inf], dtype=dt, device="cuda")
+            b.vp[int(b.table[r, key // page]), h, key % page] = b.v[r][h, key]
+    got = b.run()
+    G, u, at, broken = H // Hkv, torch.finfo(dt).eps / 2, 0, 0
+    for (c, n), k, v in zip(lens, b.k, b.v):
+        if not n:
+            continue
+        q = b.q[at:at + n].double().view(n, Hkv, G, D).permute(1, 2, 0, 3)
+        k, v = k.double()[:, None], v.double()[:, None]
+        i, j = torch.arange(c, c + n, device="cuda")[:, None], torch.arange(c + n, device="cuda")
+        seen = j <= i
+        if window:
+            seen &= (j > i - window) | (j < sinks)
+        s = q @ k.transpose(-1, -2) * D ** -0.5
+        S = float((q.abs() @ k.abs().transpose(-1, -2)).max()) * D ** -0.5
+        p = s.masked_fill(~seen, -math.inf).softmax(-1)
+        fine = v.nan_to_num(0.0, 0.0, 0.0)
+        want, A = p @ fine, p @ fine.abs()
+        up, down = (seen.double() @ (x | v.isnan()).double() > 0 for x in (v == math.inf, v == -math.inf))
+        e = 2 * ((D + 2) * 2.0 ** -23 * S + 2.0 ** -20)
+        tol = u * want.abs() + (u + e) * A + ((c + n) * 2.0 ** -24 * float(fine.abs().max()) if dt == FP else 0.0)
+        o = got[at:at + n].double().view(n, Hkv, G, D).permute(1, 2, 0, 3)
+        bad = (up | down).expand_as(o)
+        assert torch.equal(~o.isfinite(), bad)
+        assert bool(o[(up & down).expand_as(o)].isnan().all())
+        # an infinity is one, or NaN where the weight before it is 0 in the products' type
+        assert bool(((o == math.inf) | o.isnan())[(up & ~down).expand_as(o)].all())
+        assert bool(((o == -math.inf) | o.isnan())[(down & ~up).expand_as(o)].all())
+        assert bool(((o - want).abs() <= tol)[~bad].all())
+        broken += int(bad.sum())
+        at += n
+    assert broken > 0
+    F.check_status()
+
+
 # ------------------------------------------------------------------ sums of many small weights
 SUM_KEYS = {FP: 16384, BF: 131072}  # keys that the tensor core sums up before the sum is taken over
 

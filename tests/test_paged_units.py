@@ -66,6 +66,14 @@ extern "C" long long unit_walk(int bn, const long long *tiles, int n, int Hkv, i
                   : walk<128>(tiles, n, Hkv, window, sinks, ctas, overhead, out, room);
 }
 
+// Whether keys [c0, c0 + bn) hold some that no row sees (bit 0), and some that rows may differ in (bit 1).
+extern "C" int unit_differ(int bn, int pos0, int ntok, int window, int sinks, int c0) {
+  return bn == 64 ? has_unseen<64>(keys_of<64>(pos0, ntok, window, sinks), sinks, c0) +
+                        2 * rows_differ<64>(pos0, ntok, window, sinks, c0)
+                  : has_unseen<128>(keys_of<128>(pos0, ntok, window, sinks), sinks, c0) +
+                        2 * rows_differ<128>(pos0, ntok, window, sinks, c0);
+}
+
 // The key tiles of a q tile in the order in which a whole one with this turn visits them; *bounds its hi, lo.
 extern "C" int unit_keys(int bn, int pos0, int ntok, int window, int sinks, int turn, int *out, int *bounds) {
   Params p{};
@@ -211,3 +219,25 @@ def test_lines_longer_than_31_bits(units):
         for c in range(ctas):  # equal shares
             got = sum(j1 - j0 for s, _, _, j0, j1, *_ in segments if s == c)
             assert abs(got - n * heads * per_head // ctas) <= n * heads * OVERHEAD
+
+
+@pytest.mark.parametrize("bn", [64, 128])
+def test_tiles_whose_values_need_care(units, bn):
+    """A visited tile with a key that no row sees, or one that some rows see and others do not, is known as such."""
+    rng = random.Random(bn)
+    for _ in range(1500):
+        window = rng.choice([0, 0, 1, 3, 64, 100, 400])
+        sinks = rng.choice([0, 4, 64, 130]) if window else 0
+        pos0, ntok = rng.randrange(-20, 700), rng.choice([1, 2, 18, 32, 128, 256])
+        rows = [{c for c in range(max(0, p + 1)) if not window or c > p - window or c < sinks} for p in range(pos0, pos0 + ntok)]
+        some, every = set.union(*rows), set.intersection(*rows)
+        for tile in keys(units, bn, pos0, ntok, window, sinks)[0]:
+            c0 = tile * bn
+            here = set(range(c0, c0 + bn))
+            flags = units.unit_differ(bn, pos0, ntok, window, sinks, c0)
+            if here - some:
+                assert flags & 1, (pos0, ntok, window, sinks, c0)
+            if here & some - every:
+                assert flags & 2, (pos0, ntok, window, sinks, c0)
+            if ntok == 1:
+                assert not flags & 2  # decoding rows share what they see

@@ -7,8 +7,8 @@
 //
 // Work.  The G = H / Hkv query heads of a KV head share one 128-row tile with as many tokens as fit
 // (128 / G, row = token * G + head), so a key tile is loaded once for all of them.  A q tile visits the
-// 64-key tiles that any of its rows can see (the sinks' tiles, then the window's), in order.  All (q tile, KV
-// head)s form one line, each as long as its key tiles plus kOverhead for loading Q and storing the result, and
+// 64-key tiles that any of its rows can see (the sinks' and the window's), in an order that brings shares that run side
+// by side to the same keys (Walk in paged_common.cuh).  All (q tile, KV head)s form one line, each as long as its key tiles plus kOverhead for loading Q and storing the result, and
 // the line is cut into equal shares: CTA c of the persistent grid takes [c * per, (c + 1) * per).  So one
 // decode request and a batch of ragged chunks alike load every SM equally, and nothing about the lengths is
 // needed on the host.  A share that begins or ends between two key tiles of a (q tile, head) leaves fp32
@@ -26,15 +26,15 @@
 //   warp 5      MMA issuer (one thread): S = Q K^T into a double-buffered TMEM accumulator, O += P V with
 //               P from TMEM.
 //   warps 0-3   softmax: thread r owns row r; S(n) is read, masked and exponentiated against a running
-//               reference maximum (O and l rescaled only when a score outgrows it by 2^kRescale) while
+//               reference maximum (O and l rescaled only when a score outgrows it by 2^Num<E>::rescale) while
 //               the tensor core computes S(n+1).  V rows behind a request's last key, or of no key a
 //               row sees, are zeroed in shared memory first: pages hold anything there, and 0 * NaN
-//               would reach the sum.
+//               would reach the sum.  V tiles that rows differ in are looked through for NaN and infinities.
 // Every mbarrier wait is bounded (a status code instead of a hang).
 //
 // Decoding is bound by HBM, or by the power cap before it: 64 requests of 512 to 16384 keys, 32 / 8 heads, pages
-// of 16: 155 us at 1.9 GHz (6.3 TB/s, 0.96 of the measured copy), 161 to 165 us a step in a long loop; 2 x 131072
-// keys 162 us (1.0) and 170.  Chunks are bound by the tensor core and the softmax around it: a key tile takes
+// of 16: 155 us at 1.9 GHz (6.3 TB/s, 0.96 of the measured copy), 161 to 167 us a step in a long loop; 2 x 131072
+// keys 164 us (1.0) and 173.  Chunks are bound by the tensor core and the softmax around it: a key tile takes
 // about 1600 clocks in each of an SM's two CTAs, 640 of them its products (a 64-key S reads 48 KB of shared
 // memory, 384 clocks for 256 of products).
 
@@ -592,6 +592,9 @@ __global__ void __launch_bounds__(kThreads, 2)
       const int slot = 2 * int(blockIdx.x) + (first_seg ? 0 : 1);
       if (active) {
         const bool whole = w.j0 == 0 && w.j1 == g.n;
+        // (l sums the weights before their rounding to E: sums of the rounded ones, which would give a constant v back
+        // exactly, took ragged chunks from 79 to 84 us and windowed ones from 60 to 69, and brought single rows of random
+        // values 4% nearer to 64 bits in the median)
         // a row without a key (pos < 0) is zeros; NaN in l, or no key above -inf (l == 0), is NaN as in the formula
         const bool sees = pos >= 0;
         const float inv_l = 1.0f / l_run;
@@ -830,13 +833,13 @@ template <typename E, int D>
 static int launch(const Params &p, bool chunks, const ffts_paged_attn_args &a, cudaStream_t stream) {
   const int64_t *qs = a.q_strides, *ks = a.kp_strides, *vs = a.vp_strides;
   CUtensorMap mq, mk, mv;
-  const cuuint64_t qd[3] = {D, cuuint64_t(p.H), cuuint64_t(p.T)};
+  const cuuint64_t qd[3] = {D, cuuint64_t(a.H), cuuint64_t(a.T)};
   const cuuint64_t qst[2] = {cuuint64_t(qs[1]) * 2, cuuint64_t(qs[0]) * 2};
   const cuuint32_t qbox[3] = {64, cuuint32_t(p.G), cuuint32_t(kBM / p.G)};
   int rc = encode(&mq, Num<E>::map, 3, a.q, qd, qst, qbox);
   if (rc) return rc;
   const cuuint64_t ps = 1ull << p.ps_shift;
-  const cuuint64_t kd[4] = {D, ps, cuuint64_t(p.Hkv), cuuint64_t(p.n_pages)};
+  const cuuint64_t kd[4] = {D, ps, cuuint64_t(a.Hkv), cuuint64_t(a.n_pages)};
   const cuuint32_t kbox[4] = {64, cuuint32_t(std::min<cuuint64_t>(ps, chunks ? 2 * kBN : kBN)), 1, 1};
   const cuuint64_t kst[3] = {cuuint64_t(ks[2]) * 2, cuuint64_t(ks[1]) * 2, cuuint64_t(ks[0]) * 2};
   const cuuint64_t vst[3] = {cuuint64_t(vs[2]) * 2, cuuint64_t(vs[1]) * 2, cuuint64_t(vs[0]) * 2};
@@ -907,11 +910,10 @@ int paged_attn(const ffts_paged_attn_args &a, cudaStream_t stream) {
   FFTS_REQUIRE(sp.max_tiles < (int64_t(1) << 31) - 1, "paged_attn: too many q tiles");
   uint8_t *base = static_cast<uint8_t *>(a.workspace);
   Params p{};
-  p.T = int(T); p.R = int(R); p.H = int(H); p.Hkv = int(Hkv); p.G = int(G); p.tpt = int(kBM / G);
+  p.T = int(T); p.R = int(R); p.Hkv = int(Hkv); p.G = int(G); p.tpt = int(kBM / G);
   p.table = a.table;
   p.table_ld = a.table_ld;
   p.width = int(width);
-  p.n_pages = int(a.n_pages);
   p.ps_shift = ilog2_ceil(page_size);
   p.cu_q = a.cu_q;
   p.kv_lens = a.kv_lens;
@@ -941,8 +943,10 @@ int paged_attn(const ffts_paged_attn_args &a, cudaStream_t stream) {
   // The larger tiles of paged_chunk.cu: where requests fill several of them on average and the keys that a tile sees,
   // as far as the table and the window bound them, are enough to pay for filling and draining one pipeline per SM
   // instead of two. In long loops under the power cap, against the tiles of paged_attn.cu (32 / 8 heads): 2048
-  // tokens over nothing 61 us both, over 4096 190 and 207, over 32768 1.09 and 1.37 ms; 512 over 8192 91 and 94; 16
-  // ragged chunks of 650 rows on average 85 and 75; window 1024 61 and 54.
+  // tokens over nothing 58 and 63 us, over 4096 177 and 197, over 32768 1.05 and 1.21 ms; 512 over 8192 88 and 92; 16
+  // ragged chunks of 780 rows on average 80 and 79; window 1024 at D = 64 61 and 60.
+  // The average hides a long chunk among many decoding requests (and counts requests without tokens, and padding): 2048
+  // tokens over 32768 beside 63 decoding ones take the smaller tiles, 1.33 ms instead of 1.26, 8192 5.8 instead of 5.0.
   int64_t span = width * page_size;
   if (p.window > 0) span = std::min(span, int64_t(p.window) + p.sinks);
   const bool chunks = T * G >= kLongRows * R && span >= kLongKeys;

@@ -19,8 +19,8 @@
 // complete: O may be rescaled then, and only a segment's end waits for its last PV.
 // Every wait is bounded.
 //
-// 2048 tokens of 32 / 8 heads over 32768 cached: 0.98 ms, 1.15 PFLOP/s (0.70 of the measured bf16 burst), 1.16 ms
-// once the power cap holds the clock at 1.5 GHz.  A key tile of both halves takes about 3000 clocks, 2048 of them
+// 2048 tokens of 32 / 8 heads over 32768 cached: 0.93 ms, 1.21 PFLOP/s (0.74 of the measured bf16 burst), 1.05 to
+// 1.09 ms once the power cap holds the clock.  A key tile of both halves takes about 3300 clocks, 2048 of them
 // products: a half's softmax (about 1850 clocks: scores read and looked through 450, exponentials 1400) and its
 // two products follow one another, and the other half's fill the gap only in part.
 
@@ -34,7 +34,9 @@ namespace paged {
 constexpr int cBM = 128;       // rows of a half
 constexpr int cBN = 128;       // keys of a key tile
 constexpr int cThreads = 384;   // three warpgroups
-constexpr int cRegsSoftmax = 200, cRegsOther = 104;  // after the split; launched with 168 each, 2 * 200 + 104 <= 3 * 168
+// After the split; launched with 168 each, 2 * 200 + 104 <= 3 * 168.  Neither side has enough: 216 bytes are spilled
+// (bf16; 208 and 80: 264), 144 of them by the softmax warps, whose row of scores alone takes 128.
+constexpr int cRegsSoftmax = 200, cRegsOther = 104;
 constexpr int cStages = 5;
 constexpr int cTmemCols = 512;
 

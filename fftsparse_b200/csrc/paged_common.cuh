@@ -33,10 +33,10 @@ struct Cut {
 };
 
 struct Params {
-  int T, R, H, Hkv, G, tpt;   // tpt: tokens per q tile
+  int T, R, Hkv, G, tpt;      // tpt: tokens per q tile
   const int32_t *table;       // [R, width]
   int64_t table_ld;
-  int width, n_pages, ps_shift;
+  int width, ps_shift;
   const int32_t *cu_q, *kv_lens;
   int window, sinks;          // window 0: none
   const uint16_t *q;
@@ -285,7 +285,7 @@ __device__ __forceinline__ uint64_t below(int k) { return k <= 0 ? 0ull : (k >= 
 // Behind one heavy key many light ones would be lost, 131072 of them 2^-8 of the result.  So O is parked after so
 // many keys and starts again from zero, which bounds the loss by one rounding of the result; what is parked is
 // added up in fp32.  2048 tokens over 131072, 32 / 8 heads: fp16 4.37 ms without, 4.46 with, 4.52 with half as
-// many keys to a sum; bf16 4.22 all three.
+// many keys to a sum; bf16 4.22 all three (since then, with registers split otherwise, 4.23 and 4.02).
 template <typename E>
 struct Num;
 template <>

@@ -253,8 +253,8 @@ def rope_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, pos
 
     q [T, H, D] (or None), k / v [T, Hkv, D]: bf16 or fp16, D 64 or 128, unit stride over D (views of one fused
     QKV projection are fine).  ``positions`` / ``slot_map`` int32 [T] (``plan_pages``); a token whose
-    slot lies outside the pool is not appended.  ``inv_freq`` fp32 [rotary_dim / 2] (``rotary_inv_freq``), rotary_dim
-    a multiple of 16: the first rotary_dim channels turn by position * inv_freq, in pairs (i, i + rotary_dim / 2),
+    slot lies outside the pool is not appended; no two tokens have the same slot.  ``inv_freq`` fp32 [rotary_dim / 2]
+    (``rotary_inv_freq``), rotary_dim a multiple of 16: the first rotary_dim channels turn by position * inv_freq, in pairs (i, i + rotary_dim / 2),
     or (2i, 2i + 1) with ``interleaved``; cos and sin are multiplied by ``attn_factor``; the other channels are
     copied.  None copies k (and q) as they are.  ``k_pages`` / ``v_pages`` [pages, Hkv, page_size, D] are
     written in place.  Returns the rotated q [T, H, D] (``out``, which may be q itself, or a new tensor), None

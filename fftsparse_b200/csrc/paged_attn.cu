@@ -123,10 +123,13 @@ __device__ __noinline__ void note_odd(const Params &p, uint8_t *v, const OddTile
   constexpr uint32_t top = Num<E>::exponent;
   uint32_t *notes = p.notes + int64_t(blockIdx.x) * p.rows * 8;
   const bool again = *notes_seg == o.seg;
-  for (int ch = 0; ch < 4; ++ch) {  // 32 channels
-    uint32_t up[kBN], down[kBN];
-    for (int key = 0; key < kBN; ++key) {
-      up[key] = down[key] = 0;
+  constexpr int kKeys = 16;  // at a time: their words lie in local memory, which is set aside for every thread of the GPU
+  for (int step = 0; step < 4 * (kBN / kKeys); ++step) {
+    const int ch = step / (kBN / kKeys), k0 = step % (kBN / kKeys) * kKeys;  // 32 channels of these keys
+    uint32_t up[kKeys], down[kKeys];
+    for (int k = 0; k < kKeys; ++k) {
+      up[k] = down[k] = 0;
+      const int key = k0 + k;
       for (int i = 0; ch < D / 32 && i < 16; ++i) {
         uint32_t *at = reinterpret_cast<uint32_t *>(v + ((ch >> 1) * kBN + key) * 128 + (((ch & 1) * 64 + i * 4) ^ ((key & 7) << 4)));
         uint32_t w = *at;
@@ -134,26 +137,27 @@ __device__ __noinline__ void note_odd(const Params &p, uint8_t *v, const OddTile
           const uint32_t x = (w >> (16 * e)) & 0xffffu;
           if ((x & top) != top) continue;
           const bool nan = (x & 0x7fffu) != top;
-          up[key] |= uint32_t(nan || !(x & 0x8000u)) << (2 * i + e);
-          down[key] |= uint32_t(nan || (x & 0x8000u)) << (2 * i + e);
+          up[k] |= uint32_t(nan || !(x & 0x8000u)) << (2 * i + e);
+          down[k] |= uint32_t(nan || (x & 0x8000u)) << (2 * i + e);
           w &= ~(0xffffu << (16 * e));
         }
         *at = w;
       }
     }
+    const bool more = again || k0 > 0;
     for (int t = 0; t < o.ntok; ++t) {
       const int pos = o.pos0 + t;
       uint32_t u = 0, d = 0;
-      for (int key = 0; key < kBN; ++key) {
-        const int c = o.c0 + key;
+      for (int k = 0; k < kKeys; ++k) {
+        const int c = o.c0 + k0 + k;
         if (c > pos || (p.window > 0 && c <= pos - p.window && c >= p.sinks)) continue;
-        u |= up[key];
-        d |= down[key];
+        u |= up[k];
+        d |= down[k];
       }
       for (int row = t * p.G; row < (t + 1) * p.G; ++row) {
         if (!FFTS_IN_RANGE(row, p.rows)) continue;
-        notes[row * 8 + ch] = again ? notes[row * 8 + ch] | u : u;
-        notes[row * 8 + 4 + ch] = again ? notes[row * 8 + 4 + ch] | d : d;
+        notes[row * 8 + ch] = more ? notes[row * 8 + ch] | u : u;
+        notes[row * 8 + 4 + ch] = more ? notes[row * 8 + 4 + ch] | d : d;
       }
     }
   }
